@@ -8,7 +8,7 @@ OUT="$HERE/../lib"
 mkdir -p "$OUT"
 FORCE=0; [ "${1:-}" = "--force" ] && FORCE=1
 HIPCC="${HIPCC:-/opt/rocm/bin/hipcc}"
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -fvisibility=hidden -munsafe-fp-atomics -Wall -Wno-unused-function"
+FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -fvisibility=hidden -munsafe-fp-atomics -Wall -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops"
 OBJS=(); PIDS=()
 for f in "$HERE"/*.hip; do
   o="$OUT/$(basename "${f%.hip}").o"

@@ -35,6 +35,7 @@ EXPORTS = (
     "bflow_flow_metrics_accumulate", "bflow_traj_len", "bflow_pad_replicate", "bflow_voxel_grid_rectified", "bflow_voxel_grid_rectified_window", "bflow_maxabs_diff",
     "bflow_corr_lookup_bwd", "bflow_corr_lookup_bezier_bwd", "bflow_corr_pool2x2_bwd", "bflow_cvx_upsample_bwd", "bflow_l1_masked_accumulate",
     "bflow_l1_masked_grad", "bflow_conv_split_pair", "bflow_corr_lookup_im2col", "bflow_cvx_upsample_blocked",
+    "bflow_ns_workspace_bytes", "bflow_ns_orthogonalize", "bflow_muon_step",
 )
 
 
@@ -94,6 +95,10 @@ class NormDesc(ctypes.Structure):
                 ("B", ctypes.c_int), ("HW", ctypes.c_int), ("C", ctypes.c_int), ("eps", ctypes.c_float), ("rows_per_image", ctypes.c_int),
                 ("stats_replicas", ctypes.c_int), ("act_b", ctypes.c_int)]
 
+
+# struct bflow_ns_matrix (include/bflow_hip.h), as rows of a host table
+NS_MATRIX = np.dtype([("src", np.uint64), ("dst", np.uint64), ("momentum", np.uint64), ("src_ld", np.int64), ("dst_ld", np.int64), ("rows", np.int32),
+                      ("cols", np.int32)])
 
 _lib = None
 
@@ -190,12 +195,15 @@ def lib() -> ctypes.CDLL:
         "bflow_cvx_upsample_bwd": [vp, vp, vp, vp, vp, vp, i, i, i, i, vp],
         "bflow_l1_masked_accumulate": [vp, vp, vp, i, i, ll, vp, vp],
         "bflow_l1_masked_grad": [vp, vp, vp, i, i, ll, vp, vp, f, vp, vp],
+        "bflow_ns_workspace_bytes": [vp, i],
+        "bflow_ns_orthogonalize": [vp, i, i, i, f, f, f, f, vp, ll, vp],
+        "bflow_muon_step": [vp, i, i, f, f, f, f, f, i, f, vp, f, vp, ll, vp],
     }
     for name, args in sig.items():
         if _ABI_ANY and not hasattr(L, name):
             continue
         fn = getattr(L, name)
-        fn.restype = ll if name == "bflow_voxel_workspace_bytes" else i
+        fn.restype = ll if name.endswith("_workspace_bytes") else i
         fn.argtypes = args
     _lib = L
     return L
@@ -858,3 +866,35 @@ def gru_blend_bwd(dhn: torch.Tensor, q: torch.Tensor, z: torch.Tensor, h: torch.
     _check(lib().bflow_gru_blend_bwd(_dev(dhn, name="dh_new"), _dev(q), _dev(z), _dev(h), _dev(dq), _dev(dz), _dev(dh), B, C, H * W, _stream()),
            "bflow_gru_blend_bwd")
     return dq, dz, dh
+
+
+# ------------------------------------------------------------------------------------------------ Newton-Schulz / Muon (csrc/newton_schulz.hip)
+NS_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _ns_workspace(table: np.ndarray, device: torch.device) -> torch.Tensor:
+    need = lib().bflow_ns_workspace_bytes(table.ctypes.data, len(table))
+    if need < 0:
+        _check(int(need), "bflow_ns_workspace_bytes")
+    return torch.empty(need, dtype=torch.uint8, device=device)
+
+
+def ns_orthogonalize(table: np.ndarray, dtype: torch.dtype, device: torch.device, steps: int, coefficients: Sequence[float], eps: float):
+    """table: NS_MATRIX rows (src, dst, leading dimensions, rows, cols) of matrices of one dtype on `device`."""
+    a, b, c = coefficients
+    with torch.cuda.device(device):
+        ws = _ns_workspace(table, device)
+        _check(lib().bflow_ns_orthogonalize(table.ctypes.data, len(table), NS_DTYPES[dtype], steps, a, b, c, eps, ws.data_ptr(), ws.numel(), _stream()),
+               "bflow_ns_orthogonalize")
+
+
+def muon_step(table: np.ndarray, device: torch.device, steps: int, coefficients: Sequence[float], eps: float, momentum: float, nesterov: bool, lr,
+              weight_decay: float):
+    """table: NS_MATRIX rows (src = gradient, dst = weights, momentum), fp32.  lr: a float, or a float32 scalar tensor on `device`, read by the
+    kernels when they run."""
+    a, b, c = coefficients
+    on_device = isinstance(lr, torch.Tensor)
+    with torch.cuda.device(device):
+        ws = _ns_workspace(table, device)
+        _check(lib().bflow_muon_step(table.ctypes.data, len(table), steps, a, b, c, eps, momentum, int(nesterov), 0.0 if on_device else lr,
+                                     _dev(lr, name="lr") if on_device else None, weight_decay, ws.data_ptr(), ws.numel(), _stream()), "bflow_muon_step")

@@ -33,6 +33,7 @@ from . import conv_train, hip
 from . import split as S
 from .bezier import BezierCurves
 from .corr import CorrBlockParallelMultiTarget, CorrComputation
+from .muon import Muon
 from .validation import DataLoading, DataSetType, _get
 
 
@@ -421,11 +422,23 @@ def forward_train(model, voxel_grid: Optional[torch.Tensor], images: Optional[Li
 # ----------------------------------------------------------------------------------------------- the training step
 def configure_optimizers(model: torch.nn.Module, train_params: Dict[str, Any], capturable: bool = False):
     """modules/raft_spline.py:321-356: AdamW (+ linear OneCycleLR stepped per optimiser step).  capturable: the step counters and the
-    learning rate live on the device, so that `GraphedTrainStep` can record the optimiser step into its hipGraph."""
+    learning rate live on the device, so that `GraphedTrainStep` can record the optimiser step into its hipGraph.
+
+    An OPTIONAL key `optimizer` of train_params (absent from the reference's YAML files): "adamw" (the default) or "muon" -- every convolution
+    filter by `muon.Muon`, biases and norm parameters by AdamW, one learning rate and schedule for both; `muon` holds further arguments of
+    `muon.Muon` (momentum, nesterov, steps, ...)."""
     lr = train_params["learning_rate"]
     if capturable:
         lr = torch.tensor(float(lr), dtype=torch.float32, device=next(model.parameters()).device)
-    opt = torch.optim.AdamW(model.parameters(), lr=lr, weight_decay=train_params["weight_decay"], capturable=capturable)
+    kind = train_params.get("optimizer", "adamw")
+    if kind == "muon":
+        params = list(model.parameters())
+        groups = [{"params": [p for p in params if p.dim() >= 2]}, {"params": [p for p in params if p.dim() < 2], "adamw": True}]
+        opt = Muon([g for g in groups if g["params"]], lr=lr, weight_decay=train_params["weight_decay"], capturable=capturable, **(train_params.get("muon") or {}))
+    elif kind == "adamw":
+        opt = torch.optim.AdamW(model.parameters(), lr=lr, weight_decay=train_params["weight_decay"], capturable=capturable)
+    else:
+        raise ValueError(f"optimizer {kind!r}: expected 'adamw' or 'muon'")
     sch_p = train_params["lr_scheduler"]
     if not sch_p["use"]:
         return opt, None

@@ -1,0 +1,356 @@
+"""Newton-Schulz orthogonalisation and the Muon step (bflow_amd/muon.py, csrc/newton_schulz.hip) against plain 64-bit forms.
+
+Tolerances (relative, Frobenius norm).  The arithmetic of a step is fp16 pairs: an operand is off by at most 2^-22 (lo is rounded at 2^-11 of a
+residue of 2^-11), lo * lo is left out (2^-22), so a product of two is off by 3 * 2^-22 in the worst case, and a sum of K products in 32 bits by
+another 2^-24 a term in the worst case, sqrt(K) 2^-24 as rounding goes.  A step has three products behind one another: about 9 * 2^-22 = 2e-6.
+The step's map x -> a x + b x^3 + c x^5 has a slope of 3.45 at 0 and at most 3.9 on [0, 1.2]; a relative error grows only by what the map bends
+(slope * x / value <= 3.9 in absolute value, near or below 1 on most of the interval), so five steps leave a few times 2e-6.  F32_TOL = 2e-5 is
+ten times the error of one step.  That holds where no direction is empty.  In a matrix of rank one all others are: there the rounding of the
+strong direction, 2^-22 of |X| = 1 in the worst case, is all there is, and five steps multiply it by a^5 = 3.4445^5 = 485, while the strong
+direction ends at no less than 0.68 (the least of the map on the interval the steps end in): RANK_ONE_TOL = 485 * 2^-22 / 0.68 = 1.7e-4.  Results in 16 bits add their own half step: 2^-11 (fp16), 2^-8 (bf16)."""
+import copy
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import bflow_amd
+from bflow_amd import hip, muon, training
+from bflow_amd.validation import DataLoading, DataSetType
+
+DEV = "cuda:0"
+F32_TOL = 2e-5
+RANK_ONE_TOL = 485 * 2.0 ** -22 / 0.68
+TOL = {torch.float32: F32_TOL, torch.float16: F32_TOL + 2.0 ** -11, torch.bfloat16: F32_TOL + 2.0 ** -8}
+gpu = pytest.mark.gpu
+
+
+def plain(x, steps=5, coefficients=muon.COEFFICIENTS, eps=1e-7):
+    """The definition, in 64 bits on the CPU, on a (rows, everything else) matrix."""
+    a, b, c = coefficients
+    y = x.detach().cpu().double().reshape(x.shape[0], -1)
+    tall = y.shape[0] > y.shape[1]
+    y = y.t() if tall else y
+    y = y / (y.norm() + eps)
+    for _ in range(steps):
+        g = y @ y.t()
+        y = a * y + (b * g + c * g @ g) @ y
+    return (y.t() if tall else y).reshape(x.shape)
+
+
+def off(got, want):
+    got, want = got.detach().cpu().double(), want.double()
+    return float((got - want).norm() / want.norm())
+
+
+def gradient(*shape, seed=0, size=1e-3):
+    """A few strong directions, a tail of weak ones, noise."""
+    rs = np.random.RandomState(seed)
+    m, n = shape[0], int(np.prod(shape[1:]))
+    r = max(1, min(m, n) // 4)
+    x = (rs.standard_normal((m, r)) * np.logspace(0, -3, r)) @ rs.standard_normal((r, n)) + 0.03 * rs.standard_normal((m, n))
+    return torch.from_numpy((size * x).astype(np.float32).reshape(shape))
+
+
+# ------------------------------------------------------------------------------------------------------------------------- refusals (CPU)
+def test_refuses_what_it_cannot_take():
+    x = torch.zeros(4, 4)
+    with pytest.raises(hip.BflowHipError, match="no CPU fallback"):
+        muon.orthogonalize([x])
+    with pytest.raises(hip.BflowHipError, match="list"):
+        muon.orthogonalize(x)
+    for bad in (0, 33, 2.5):
+        with pytest.raises(hip.BflowHipError, match="steps"):
+            muon.orthogonalize([], steps=bad)
+    for bad in (0.0, 1.0, float("nan")):
+        with pytest.raises(hip.BflowHipError, match="eps"):
+            muon.orthogonalize([], eps=bad)
+    with pytest.raises(hip.BflowHipError, match="three"):
+        muon.orthogonalize([], coefficients=(1.0, 2.0))
+    assert muon.orthogonalize([]) == []
+
+
+def test_c_entry_refuses_bad_tables():
+    """The C entry's own checks, before any launch: no GPU is touched."""
+    lib = hip.lib()
+
+    def call(rows=4, cols=8, src=256, dst=256, src_ld=8, dst_ld=8, momentum=256, steps=5, abc=muon.COEFFICIENTS, eps=1e-7, dtype=0, ws=256, ws_bytes=1 << 30, step=False):
+        t = muon._table([(src, dst, momentum, src_ld, dst_ld, rows, cols)])
+        if step:
+            return lib.bflow_muon_step(t.ctypes.data, 1, steps, *abc, eps, 0.9, 1, 0.1, None, 0.0, ws, ws_bytes, None)
+        return lib.bflow_ns_orthogonalize(t.ctypes.data, 1, dtype, steps, *abc, eps, ws, ws_bytes, None)
+
+    for kw in (dict(rows=0), dict(cols=0), dict(cols=hip_limit() + 1), dict(rows=-1), dict(rows=1 << 16, cols=1 << 16, src_ld=1 << 16, dst_ld=1 << 16), dict(src=0), dict(dst=0),
+               dict(src_ld=7), dict(dst_ld=7), dict(steps=0), dict(steps=33), dict(eps=0.0), dict(eps=1.0), dict(dtype=3), dict(dtype=-1), dict(ws=0), dict(ws=128),
+               dict(ws_bytes=1024), dict(abc=(5.0, 0.0, 0.0)), dict(abc=(float("nan"), 0.0, 0.0)), dict(step=True, momentum=0)):
+        assert call(**kw) == -1, kw
+        assert b"newton_schulz" in lib.bflow_last_error_string() or b"ns_orthogonalize" in lib.bflow_last_error_string()
+    assert lib.bflow_ns_workspace_bytes(None, 1) == -1
+    empty = muon._table([])
+    assert lib.bflow_ns_workspace_bytes(empty.ctypes.data, 0) == 0
+
+
+def hip_limit():
+    return 1 << 20
+
+
+def test_optimizer_checks_its_arguments():
+    w = torch.nn.Parameter(torch.zeros(4, 4))
+    for kw in (dict(lr=-1.0), dict(momentum=1.0), dict(momentum=-0.1), dict(weight_decay=-1.0)):
+        with pytest.raises(ValueError):
+            muon.Muon([w], **kw)
+    with pytest.raises(hip.BflowHipError, match="adamw=True"):
+        muon.Muon([torch.nn.Parameter(torch.zeros(4))])
+    with pytest.raises(hip.BflowHipError, match="adamw=True"):
+        muon.Muon([torch.nn.Parameter(torch.zeros(4, 6).t())])
+    with pytest.raises(hip.BflowHipError, match="float32"):
+        muon.Muon([torch.nn.Parameter(torch.zeros(4, 4, dtype=torch.float16))])
+    opt = muon.Muon([{"params": [w]}, {"params": [torch.nn.Parameter(torch.zeros(4))], "adamw": True}])
+    opt.step()                                                       # no gradients: nothing to do, on any device
+    w.grad = torch.zeros(4, 4)
+    with pytest.raises(hip.BflowHipError, match="no CPU fallback"):
+        opt.step()
+
+
+def test_configure_optimizers_chooses():
+    from bflow_amd import configs
+    m = bflow_amd.RAFTSpline(configs.model_config("E_LU4_BD2"))
+    tp = dict(learning_rate=1e-4, weight_decay=1e-4, lr_scheduler=dict(use=True, total_steps=10, pct_start=0.1))
+    opt, _ = training.configure_optimizers(m, tp)
+    assert type(opt) is torch.optim.AdamW
+    opt, sch = training.configure_optimizers(m, dict(tp, optimizer="muon", muon=dict(momentum=0.9, steps=4)))
+    assert type(opt) is muon.Muon and sch is not None
+    filters, rest = opt.param_groups
+    assert not filters["adamw"] and rest["adamw"] and filters["momentum"] == 0.9 and filters["steps"] == 4
+    assert all(p.dim() == 4 for p in filters["params"]) and all(p.dim() == 1 for p in rest["params"])
+    assert len(filters["params"]) + len(rest["params"]) == len(list(m.parameters()))
+    with pytest.raises(ValueError, match="optimizer"):
+        training.configure_optimizers(m, dict(tp, optimizer="sgd"))
+
+
+# ------------------------------------------------------------------------------------------------------------------------------- matrices
+SHAPES = [(1, 1), (1, 77), (77, 1), (2, 2049), (5, 3), (63, 64), (64, 64), (64, 65), (65, 63), (128, 1152), (129, 513), (517, 131), (300, 300), (256, 567), (700, 1500)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", list(TOL))
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: f"{s[0]}x{s[1]}")
+def test_one_matrix(shape, dtype):
+    x = gradient(*shape, seed=sum(shape)).to(dtype)
+    before = x.clone()
+    dev = x.to(DEV)
+    (y,) = muon.orthogonalize([dev])
+    assert y.shape == x.shape and y.dtype == dtype and y.is_contiguous()
+    assert off(y, plain(x)) < TOL[dtype]
+    assert torch.equal(dev.cpu(), before)
+
+
+@gpu
+@pytest.mark.parametrize("steps", [1, 2, 3, 6])
+def test_steps_and_coefficients(steps):
+    x = gradient(96, 200, seed=steps)
+    for abc in (muon.COEFFICIENTS, (1.5, -0.5, 0.0), (1.875, -1.25, 0.375)):
+        (y,) = muon.orthogonalize([x.to(DEV)], steps=steps, coefficients=abc)
+        assert off(y, plain(x, steps, abc)) < F32_TOL
+
+
+@gpu
+def test_a_list_equals_its_plain_forms_and_repeats_bit_for_bit():
+    """More matrices than one round of launches takes, types mixed, filters among them, an empty one: each right, in order, and the same bits twice."""
+    shapes = [(1 + 7 * k % 130, 1 + 13 * k % 90) for k in range(75)] + [(64, 5, 7, 7), (96, 64, 1, 1), (4, 256, 3, 3)]
+    kinds = list(TOL)
+    xs = [gradient(*s, seed=k).to(kinds[k % 3] if k < 70 else torch.float32) for k, s in enumerate(shapes)]
+    xs.insert(3, torch.zeros(0, 5))
+    xs.insert(9, torch.zeros(5, 0))
+    dev = [x.to(DEV) for x in xs]
+    ys, again = muon.orthogonalize(dev), muon.orthogonalize(dev)
+    for x, y, z in zip(xs, ys, again):
+        assert y.shape == x.shape and torch.equal(y, z)
+        if x.numel():
+            assert off(y, plain(x)) < TOL[x.dtype]
+
+
+@gpu
+def test_strides():
+    """Rows further apart than they are long, a transposed view, a slice that starts at an odd element."""
+    big = gradient(150, 401, seed=1)
+    dev = big.to(DEV)
+    cases = [(dev[:70, :100], big[:70, :100]), (dev[3:90, 7:], big[3:90, 7:]), (dev.t(), big.t()), (dev[::2, 1:60], big[::2, 1:60]), (dev[:1, 5:9], big[:1, 5:9]),
+             (dev[:, ::3], big[:, ::3]), (dev[0].expand(6, 401), big[0].expand(6, 401))]
+    ys = muon.orthogonalize([d for d, _ in cases])
+    for y, (_, x) in zip(ys, cases):
+        assert y.is_contiguous() and off(y, plain(x)) < F32_TOL
+
+
+@gpu
+def test_zero_tiny_huge_and_lost_values():
+    x = gradient(40, 100, seed=2)
+    nan, inf, rank1 = x.clone(), x.clone(), torch.outer(x[:, 0], x[0])
+    nan[3, 5], inf[39, 99] = float("nan"), float("-inf")
+    zero, tiny, huge = torch.zeros(33, 70), x * 1e-30, x * 1e30
+    one_row = torch.zeros(40, 100)
+    one_row[17] = x[17]
+    ys = muon.orthogonalize([t.to(DEV) for t in (zero, tiny, huge, nan, inf, rank1, one_row)])
+    assert not ys[0].any()
+    assert off(ys[1], plain(tiny)) < F32_TOL and off(ys[2], plain(huge)) < F32_TOL
+    assert torch.isnan(ys[3]).all() and torch.isnan(ys[4]).all()
+    assert off(ys[5], plain(rank1)) < RANK_ONE_TOL and off(ys[6], plain(one_row)) < F32_TOL      # (one row: the others hold no rounding either)
+    assert not ys[6][:17].any() and not ys[6][18:].any()
+
+
+@gpu
+def test_refuses_on_the_device():
+    x = torch.zeros(4, 4, device=DEV)
+    with pytest.raises(hip.BflowHipError, match="two dimensions"):
+        muon.orthogonalize([x[0]])
+    with pytest.raises(hip.BflowHipError, match="dtype"):
+        muon.orthogonalize([x.double()])
+    with pytest.raises(hip.BflowHipError, match="coefficients"):
+        muon.orthogonalize([x], coefficients=(5.0, 0.0, 0.0))
+
+
+@gpu
+def test_on_another_stream_and_in_a_graph():
+    """Two streams at once (a workspace each), then a captured call: replays follow the input, also between eager calls of other lists."""
+    xs = [gradient(64, 576, seed=1), gradient(256, 567, seed=2), gradient(300, 40, seed=3)]
+    a, b = [x.to(DEV) for x in xs], [(2 * x.flip(1)).to(DEV) for x in xs]
+    want_a, want_b = muon.orthogonalize(a), muon.orthogonalize(b)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s1):
+        ya = [muon.orthogonalize(a) for _ in range(3)]
+    with torch.cuda.stream(s2):
+        yb = [muon.orthogonalize(b) for _ in range(3)]
+    torch.cuda.synchronize()
+    for got, want in ((ya, want_a), (yb, want_b)):
+        for y in got:
+            assert all(torch.equal(p, q) for p, q in zip(y, want))
+    static = [x.clone() for x in a]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = muon.orthogonalize(static)
+    for source, want in ((a, want_a), (b, want_b), (a, want_a)):
+        for s, x in zip(static, source):
+            s.copy_(x)
+        graph.replay()
+        muon.orthogonalize([x.to(DEV) for x in xs[:2]])
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, want))
+
+
+# ------------------------------------------------------------------------------------------------------------------------------- the step
+def plain_step(p, g, v, lr, decay, mu, nesterov, **kw):
+    p, g, v = (t.detach().cpu().double() for t in (p, g, v))
+    v = mu * v + g
+    m, n = p.shape[0], p[0].numel()
+    return p * (1 - lr * decay) - lr * 0.2 * math.sqrt(max(m, n)) * plain(g + mu * v if nesterov else v, **kw), v
+
+
+@gpu
+@pytest.mark.parametrize("nesterov,mu,decay", [(True, 0.95, 0.1), (False, 0.9, 0.0), (True, 0.0, 0.01)])
+def test_steps_of_the_optimizer(nesterov, mu, decay):
+    """Three steps on filters, matrices, tall and wide; the update itself is held to the tolerance, not only the weights."""
+    shapes = [(64, 5, 7, 7), (4, 256, 3, 3), (96, 64, 1, 1), (576, 256), (1, 9), (130, 70)]
+    lr = 0.02
+    ps = [torch.nn.Parameter(gradient(*s, seed=k, size=1.0).to(DEV)) for k, s in enumerate(shapes)]
+    frozen = torch.nn.Parameter(torch.ones(3, 3, device=DEV))
+    opt = muon.Muon(ps + [frozen], lr=lr, momentum=mu, weight_decay=decay, nesterov=nesterov)
+    vs = [torch.zeros(p.shape, dtype=torch.float64) for p in ps]
+    for t in range(3):
+        before = [p.detach().clone() for p in ps]
+        versions = [p._version for p in ps]
+        for k, p in enumerate(ps):
+            p.grad = gradient(*shapes[k], seed=10 * t + k).to(DEV)
+        opt.step()
+        for k, p in enumerate(ps):
+            want, vs[k] = plain_step(before[k], p.grad, vs[k], lr, decay, mu, nesterov)
+            v = opt.state[p]["momentum_buffer"]
+            assert off(v, vs[k]) < 2.0 ** -22                       # a rounding for each step, 2^-24 each
+            moved, wanted = p.detach().cpu().double() - before[k].cpu().double(), want - before[k].cpu().double()
+            # weights are stored in 32 bits: 2^-24 of a weight on top of the update's own error (momentum: 3 * 2^-24, inside it)
+            assert float((moved - wanted).norm()) < F32_TOL * float(wanted.norm()) + 2.0 ** -23 * float(want.norm())
+            assert p._version > versions[k]
+            vs[k] = v.cpu().double()
+    assert torch.equal(frozen, torch.ones_like(frozen)) and frozen not in opt.state
+
+
+@gpu
+def test_optimizer_takes_strided_gradients_and_a_rate_on_the_device():
+    p = torch.nn.Parameter(gradient(64, 96, 3, 3, seed=1, size=1.0).to(DEV))
+    q = torch.nn.Parameter(p.detach().clone())
+    g = gradient(64, 96, 3, 3, seed=2).to(DEV)
+    p.grad, q.grad = g, g.to(memory_format=torch.channels_last)
+    rate = torch.tensor(0.5, device=DEV)
+    a, b = muon.Muon([p], lr=0.02), muon.Muon([q], lr=rate)
+    a.step()
+    rate.fill_(0.02)
+    b.zero_grad(set_to_none=False)
+    q.grad = g.to(memory_format=torch.channels_last)
+    q.data.copy_(gradient(64, 96, 3, 3, seed=1, size=1.0))
+    b.step()
+    assert torch.equal(p, q)
+    b.load_state_dict(copy.deepcopy(a.state_dict()))
+    assert torch.equal(b.state[q]["momentum_buffer"], a.state[p]["momentum_buffer"])
+
+
+@gpu
+def test_adamw_group_is_adamw():
+    w, x = torch.nn.Parameter(torch.randn(7, 5, device=DEV)), torch.nn.Parameter(torch.randn(9, device=DEV))
+    y = torch.nn.Parameter(x.detach().clone())
+    opt = muon.Muon([{"params": [w]}, {"params": [x], "adamw": True}], lr=0.01, weight_decay=0.1)
+    ref = torch.optim.AdamW([y], lr=0.01, weight_decay=0.1)
+    for t in range(3):
+        w.grad = torch.randn(7, 5, device=DEV)
+        x.grad = torch.randn(9, device=DEV)
+        y.grad = x.grad.clone()
+        opt.step()
+        ref.step()
+        assert torch.equal(x, y)
+
+
+@gpu
+def test_training_steps_with_muon_eager_and_graphed():
+    """configure_optimizers(optimizer: muon) through the whole training step, eager against one captured graph; a plain update beside it."""
+    from bflow_amd import configs, synthetic
+    from bflow_amd.weights import deterministic_state_dict
+    cfg = configs.model_config("E_LU4_BD2")
+    B, H, W = 1, 64, 96
+    tp = dict(learning_rate=2e-4, weight_decay=1e-4, optimizer="muon", lr_scheduler=dict(use=True, total_steps=50, pct_start=0.3))
+
+    def batch(seed):
+        rs = np.random.RandomState(seed)
+        to = lambda a: torch.from_numpy(a).to(DEV)
+        return {DataLoading.EV_REPR: to(synthetic.voxel_grid(B, 9, H, W, seed=seed)), DataLoading.FLOW: to(rs.standard_normal((B, 2, H, W)).astype(np.float32) * 4),
+                DataLoading.FLOW_VALID: to(rs.rand(B, H, W) > 0.2), DataLoading.DATASET_TYPE: [DataSetType.DSEC] * B}
+
+    def make(capturable):
+        m = bflow_amd.RAFTSpline(cfg)
+        m.load_state_dict(deterministic_state_dict(m, seed=0))
+        m.to(DEV).train()
+        opt, sch = training.configure_optimizers(m, tp, capturable=capturable)
+        return m, opt, sch, training.TrainStep(m, num_iter_train=2)
+
+    batches = [batch(5), batch(6), batch(7)]
+    m1, opt1, sch1, step1 = make(False)
+    eager = []
+    for k, b in enumerate(batches):
+        opt1.zero_grad(set_to_none=True)
+        out = step1(b)
+        out["loss"].backward()
+        if k == 0:
+            p = m1.update_block.gru.convz1.weight
+            before, lr = p.detach().clone(), opt1.param_groups[0]["lr"]
+            want, _ = plain_step(before, p.grad, torch.zeros_like(p), lr, 1e-4, 0.95, True)
+        opt1.step()
+        if k == 0:
+            moved, wanted = p.detach().cpu().double() - before.cpu().double(), want - before.cpu().double()
+            assert float((moved - wanted).norm()) < F32_TOL * float(wanted.norm()) + 2.0 ** -23 * float(want.norm())
+        sch1.step()
+        eager.append(float(out["loss"].detach()))
+    m2, opt2, sch2, step2 = make(True)
+    gstep = training.GraphedTrainStep(step2, opt2, sch2)
+    graphed = [float(gstep(b)["loss"].detach()) for b in batches]
+    # the same kernels on the same numbers, but for the order of the look-up adjoint's sums (2^-24 each, through three updates)
+    assert graphed == pytest.approx(eager, rel=1e-3)
+    assert all(bool(torch.isfinite(p).all()) for p in m2.parameters())

@@ -11,13 +11,14 @@ Everything is allocated with torch (caller-owned memory); the kernels only see p
 """
 from __future__ import annotations
 
+import math
 import os
 from typing import List, Optional, Sequence, Tuple, Union
 
 import numpy as np
 import torch
 
-from . import hip
+from . import hip, int8
 
 # Correlation arithmetic (all hand-written HIP; override the default with BFLOW_CORR_PRECISION or per block / per model):
 #   "split" : split-fp16 MFMA engine, fp32 volume -- fp32-class accuracy (~2^-22 per product); the default on row-major planes
@@ -29,10 +30,15 @@ from . import hip
 #             data); the cross terms carry 2^-11 of a product, so their 2^-4 operand rounding leaves ~2^-16 per product
 #   "split/h", "split8/h", "f16/w": the same arithmetics with the other storage type (fp16 / fp16 / fp32 volume) -- the decomposition of the
 #             fp16 variant's error into operand and storage rounding (tests/test_hip_parity.py), not product defaults
+#   "i8"    : both feature maps quantised to 8-bit integers with a scale for each pixel, exact integer sums on the int8 matrix rate, fp16 tiled
+#             volume ("i8/w": fp32 tiled volume); feature dims that are multiples of 32 (int8.py, csrc/int8_gemm.hip)
 # name -> (bflow_corr_build_tiled arithmetic, fp16 volume)
+ARITH_I8 = -1      # not an arithmetic of bflow_corr_build_tiled: quantisation, then bflow_i8_gemm
 PRECISIONS = {"split": (hip.ARITH_SPLIT, False), "f32": (None, False), "f16": (hip.ARITH_F16, True), "split8": (hip.ARITH_SPLIT8, False),
-              "split/h": (hip.ARITH_SPLIT, True), "split8/h": (hip.ARITH_SPLIT8, True), "f16/w": (hip.ARITH_F16, False)}
-TILED_ONLY = frozenset(("f16", "split8", "split/h", "split8/h", "f16/w"))      # written by bflow_corr_build_tiled only
+              "split/h": (hip.ARITH_SPLIT, True), "split8/h": (hip.ARITH_SPLIT8, True), "f16/w": (hip.ARITH_F16, False),
+              "i8": (ARITH_I8, True), "i8/w": (ARITH_I8, False)}
+I8 = frozenset(("i8", "i8/w"))
+TILED_ONLY = frozenset(("f16", "split8", "split/h", "split8/h", "f16/w")) | I8      # written by bflow_corr_build_tiled / the 8-bit product only
 
 
 def default_precision(dim: int, tiled: bool = True) -> str:
@@ -165,15 +171,17 @@ class CorrComputation:
                                num_levels_per_target=[torch.tensor(lv) for lv in self._levels + other._levels])
 
     def tiled_supported(self, precision: Optional[str] = None) -> bool:
-        """The tiled-plane volume is written by the streaming K5 kernel only: split operands with D in {64, 128, 256}, fp16 with D in
-        {128, 256}."""
+        """The tiled-plane volume is written by the streaming K5 kernel (split operands with D in {64, 128, 256}, fp16 with D in {128, 256}) and
+        by the 8-bit product (D a multiple of 32)."""
         precision = default_precision(self.dim, True) if precision is None else check_precision(precision)
+        if precision in I8:
+            return self.dim % 32 == 0
         return (precision == "split" and self.dim in (64, 128, 256)) or (precision in TILED_ONLY and self.dim in (128, 256))
 
     def pool1_fusable(self, precision: Optional[str] = None) -> bool:
         """True when the K5 launch of this precision can write the level-1 planes itself (get_correlation_volume(pool1=...))."""
         precision = default_precision(self.dim, True) if precision is None else check_precision(precision)
-        if PRECISIONS[precision][0] is None or not self.tiled_supported(precision):
+        if PRECISIONS[precision][0] is None or precision in I8 or not self.tiled_supported(precision):
             return False
         ar, st16 = PRECISIONS[precision]
         return hip.pool_fusable(ar, st16, self.dim, max(f2.shape[0] for f2 in self._fmap2))
@@ -192,7 +200,7 @@ class CorrComputation:
         precision = default_precision(D, tiled) if precision is None else check_precision(precision)
         if (tiled or precision in TILED_ONLY) and not (tiled and self.tiled_supported(precision)):
             raise hip.BflowHipError(f"correlation volume (tiled={tiled}, precision={precision!r}, D={D}): the tiled layout needs 'split' with D in "
-                                    f"(64, 128, 256) or one of {sorted(TILED_ONLY)} with D in (128, 256), which exist in the tiled layout only")
+                                    f"(64, 128, 256) or one of {sorted(TILED_ONLY)} with D in (128, 256) ({sorted(I8)}: a multiple of 32), which exist in the tiled layout only")
         arithmetic, st16 = PRECISIONS[precision]
         vshape, vdtype = (T, B, N, hip.tiled_plane_size(h, w) if tiled else N), torch.float16 if st16 else torch.float32
         if out is not None:        # a caller-owned volume (double-buffered frames, bflow_amd/pipeline.py)
@@ -202,6 +210,9 @@ class CorrComputation:
             vol = torch.empty(vshape, dtype=vdtype, device=device)
         thw = (h, w) if tiled else None
         split = precision != "f32" and D % 64 == 0
+
+        def build_i8(q1, q2, dst, tg):      # q1: one row for each reference pixel; q2: one for each place of the tiled plane
+            int8.matmul(q1[0].view(B, N, D), q1[1].view(B, N), q2[0].view(tg, B, -1, D), q2[1].view(tg, B, -1), vdtype, 1.0 / math.sqrt(D), out=dst)
 
         def build(p1, p2, dst, tg, t_first):
             if precision in TILED_ONLY or pool1 is not None:
@@ -222,7 +233,14 @@ class CorrComputation:
         for f1, f2, packed in zip(self._fmap1, self._fmap2, self._packed):
             tg = f2.shape[0]
             if packed is not None:
-                build(packed[0], packed[1], vol[t0:t0 + tg], tg, t0)
+                if precision in I8:
+                    build_i8(int8.quantize_packed(packed[0], h, w), int8.quantize_packed(packed[1], h, w, tiled=True), vol[t0:t0 + tg], tg)
+                else:
+                    build(packed[0], packed[1], vol[t0:t0 + tg], tg, t0)
+                t0 += tg
+                continue
+            if precision in I8:
+                build_i8(int8.quantize_pixels(f1.float()), int8.quantize_pixels(f2.float(), tiled=True), vol[t0:t0 + tg], tg)
                 t0 += tg
                 continue
             f1 = f1.float().contiguous().view(B, D, N)

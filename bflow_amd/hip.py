@@ -35,7 +35,7 @@ EXPORTS = (
     "bflow_flow_metrics_accumulate", "bflow_traj_len", "bflow_pad_replicate", "bflow_voxel_grid_rectified", "bflow_voxel_grid_rectified_window", "bflow_maxabs_diff",
     "bflow_corr_lookup_bwd", "bflow_corr_lookup_bezier_bwd", "bflow_corr_pool2x2_bwd", "bflow_cvx_upsample_bwd", "bflow_l1_masked_accumulate",
     "bflow_l1_masked_grad", "bflow_conv_split_pair", "bflow_corr_lookup_im2col", "bflow_cvx_upsample_blocked",
-    "bflow_ns_workspace_bytes", "bflow_ns_orthogonalize", "bflow_muon_step",
+    "bflow_ns_workspace_bytes", "bflow_ns_orthogonalize", "bflow_muon_step", "bflow_i8_gemm", "bflow_i8_quantize_rows", "bflow_i8_quantize_pixels",
 )
 
 
@@ -94,6 +94,14 @@ class NormDesc(ctypes.Structure):
                 ("out_hi", ctypes.c_void_p), ("out_lo", ctypes.c_void_p), ("out_f32", ctypes.c_void_p),
                 ("B", ctypes.c_int), ("HW", ctypes.c_int), ("C", ctypes.c_int), ("eps", ctypes.c_float), ("rows_per_image", ctypes.c_int),
                 ("stats_replicas", ctypes.c_int), ("act_b", ctypes.c_int)]
+
+
+class I8GemmDesc(ctypes.Structure):
+    """struct bflow_i8_gemm_desc (include/bflow_hip.h)."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("a", "b", "scale_a", "scale_b", "out")] + \
+               [(n, ctypes.c_longlong) for n in ("a_stride0", "a_stride1", "b_stride0", "b_stride1", "sa_stride0", "sa_stride1", "sb_stride0", "sb_stride1",
+                                                 "out_stride0", "out_stride1", "ldo")] + \
+               [(n, ctypes.c_int) for n in ("lda", "ldb", "M", "N", "K", "batch0", "batch1", "dtype")] + [("alpha", ctypes.c_float)]
 
 
 # struct bflow_ns_matrix (include/bflow_hip.h), as rows of a host table
@@ -195,6 +203,9 @@ def lib() -> ctypes.CDLL:
         "bflow_cvx_upsample_bwd": [vp, vp, vp, vp, vp, vp, i, i, i, i, vp],
         "bflow_l1_masked_accumulate": [vp, vp, vp, i, i, ll, vp, vp],
         "bflow_l1_masked_grad": [vp, vp, vp, i, i, ll, vp, vp, f, vp, vp],
+        "bflow_i8_gemm": [ctypes.POINTER(I8GemmDesc), vp],
+        "bflow_i8_quantize_rows": [vp, i, ll, ll, i, vp, i, vp, vp],
+        "bflow_i8_quantize_pixels": [vp, vp, vp, i, i, i, i, i, i, vp, vp, vp],
         "bflow_ns_workspace_bytes": [vp, i],
         "bflow_ns_orthogonalize": [vp, i, i, i, f, f, f, f, vp, ll, vp],
         "bflow_muon_step": [vp, i, i, f, f, f, f, f, i, f, vp, f, vp, ll, vp],
@@ -869,7 +880,7 @@ def gru_blend_bwd(dhn: torch.Tensor, q: torch.Tensor, z: torch.Tensor, h: torch.
 
 
 # ------------------------------------------------------------------------------------------------ Newton-Schulz / Muon (csrc/newton_schulz.hip)
-NS_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+FLOAT_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
 def _ns_workspace(table: np.ndarray, device: torch.device) -> torch.Tensor:
@@ -884,7 +895,7 @@ def ns_orthogonalize(table: np.ndarray, dtype: torch.dtype, device: torch.device
     a, b, c = coefficients
     with torch.cuda.device(device):
         ws = _ns_workspace(table, device)
-        _check(lib().bflow_ns_orthogonalize(table.ctypes.data, len(table), NS_DTYPES[dtype], steps, a, b, c, eps, ws.data_ptr(), ws.numel(), _stream()),
+        _check(lib().bflow_ns_orthogonalize(table.ctypes.data, len(table), FLOAT_CODES[dtype], steps, a, b, c, eps, ws.data_ptr(), ws.numel(), _stream()),
                "bflow_ns_orthogonalize")
 
 

@@ -63,8 +63,8 @@ def orthogonalize(matrices: Sequence[torch.Tensor], steps: int = STEPS, coeffici
     held = []                                             # contiguous copies live until the launches are enqueued
     for i, t in enumerate(matrices):
         hip._dev(t, None, f"matrix {i}", contiguous=False)
-        if t.dtype not in hip.NS_DTYPES:
-            raise hip.BflowHipError(f"matrix {i}: dtype {t.dtype}, expected one of {sorted(str(d) for d in hip.NS_DTYPES)}")
+        if t.dtype not in hip.FLOAT_CODES:
+            raise hip.BflowHipError(f"matrix {i}: dtype {t.dtype}, expected one of {sorted(str(d) for d in hip.FLOAT_CODES)}")
         x = _as_matrix(t, f"matrix {i}")
         out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
         results.append(out)

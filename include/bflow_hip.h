@@ -611,6 +611,36 @@ int bflow_ns_orthogonalize(const bflow_ns_matrix_t* m, int count, int dtype, int
 int bflow_muon_step(const bflow_ns_matrix_t* m, int count, int steps, float a, float b, float c, float eps, float momentum, int nesterov,
                     float lr, const float* lr_device, float weight_decay, void* ws, long long ws_bytes, bflow_stream_t stream);
 
+/* 8-bit integers with a scale for each row (csrc/int8_gemm.hip; host side bflow_amd/int8.py).  No counterpart in the reference; the
+ * correlation volume (models/raft_utils/corr.py:264-272) is built on it for `correlation.precision: i8` (bflow_amd/corr.py).
+ *   bflow_i8_gemm          : out[z, i, j] = alpha scale_a[z, i] scale_b[z, j] sum_k a[z, i, k] b[z, j, k], rounded once to dtype (0 fp32, 1 fp16,
+ *                            2 bf16); sums exact in 32-bit integers.  z = (z0, z1) over batch0 x batch1; every operand has its own strides for
+ *                            the two (elements; 0 repeats it).  a: M rows of K bytes, lda apart; b: N rows, ldb apart; addresses, lda, ldb and
+ *                            the strides of a and b are multiples of 16 bytes, and a row is READ up to K rounded up to 16 (what stands behind
+ *                            K does not count).  out: ldo elements from row to row; not a, b or a scale.
+ *   bflow_i8_quantize_rows : x (rows, K) of dtype, ld elements apart -> q (rows, ldq), zeros behind K, scale (rows)
+ *   bflow_i8_quantize_pixels: feature maps -> one row of D channels for each pixel: q (B, rows, D), scale (B, rows).  x (B, D, h, w) fp32, or
+ *                            (x NULL) the fp16-pair operand x_hi, x_lo (B, D/32, np, 32) of bflow_split_pack.  tiled 0: rows = h w, pixels in
+ *                            order; 1: rows = ceil(h/4) ceil(w/8) 32, pixels in the 4 x 8 tile order of the tiled volume (row r of a tile row by
+ *                            row), rows outside the map zero with scale 0.
+ * Quantisation: scale = max|x| / 127, q = the nearest whole number to 127 x / max|x|, halves to even, exactly.  A row of zeros has scale 0; a row
+ * with an infinity or a NaN has q = 0 and an infinite or NaN scale, so that its products are NaN.                                              */
+#define BFLOW_I8_MAX_K  131071
+#define BFLOW_I8_MAX_LD (1 << 22)
+typedef struct bflow_i8_gemm_desc {
+    const void *a, *b;
+    const float *scale_a, *scale_b;
+    void* out;
+    long long a_stride0, a_stride1, b_stride0, b_stride1, sa_stride0, sa_stride1, sb_stride0, sb_stride1, out_stride0, out_stride1, ldo;
+    int lda, ldb, M, N, K, batch0, batch1, dtype;
+    float alpha;
+} bflow_i8_gemm_t;
+int bflow_i8_gemm(const bflow_i8_gemm_t* desc, bflow_stream_t stream);
+int bflow_i8_quantize_rows(const void* x, int dtype, long long ld, long long rows, int K, signed char* q, int ldq, float* scale,
+                           bflow_stream_t stream);
+int bflow_i8_quantize_pixels(const float* x, const void* x_hi, const void* x_lo, int np, int B, int D, int h, int w, int tiled, signed char* q,
+                             float* scale, bflow_stream_t stream);
+
 #pragma GCC visibility pop
 #ifdef __cplusplus
 }

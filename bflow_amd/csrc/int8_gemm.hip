@@ -28,6 +28,7 @@ struct GemmArgs {
     int M, N, K, n1;        // n1: size of the inner batch dimension
     float alpha;
     int tiles_m, tiles_n;
+    int wide;               // the output's rows start at multiples of 16 bytes
 };
 
 // bytes k .. k + 15 of a fragment: those at or behind K become zero
@@ -43,16 +44,17 @@ __device__ __forceinline__ i32x4 cut(i32x4 v, int k, int K) {
 // BM x BN tile; wave (wm, wn) keeps WM x WN of it.
 template <int BM, int BN, int WM, int WN>
 struct ByteTile {
-    static constexpr int ACROSS = BN / WN, WAVES = (BM / WM) * ACROSS, THREADS = 64 * WAVES, MT = WM / 32, NT = WN / 32;
+    static constexpr int M = BM, N = BN, ACROSS = BN / WN, WAVES = (BM / WM) * ACROSS, THREADS = 64 * WAVES, MT = WM / 32, NT = WN / 32;
     static constexpr int STAGE = (BM + BN) * CHUNK, LDS = 2 * STAGE, PIECES = (BM + BN) / 8;
-    static_assert(PIECES % WAVES == 0, "whole pieces for every wave");
+    static_assert(BM / 8 % WAVES == 0 && BN / 8 % WAVES == 0, "whole pieces of either operand for every wave");
+    // B is the instruction's first operand: lane l then holds row l % 32 of a 32 x 32 block, four neighbouring columns in neighbouring registers
     i32x16 acc[MT][NT];
 
     __device__ __forceinline__ void issue(rsrc_t a, int lda, int va, rsrc_t b, int ldb, int vb, int chunk, char* stage, int wave) {
 #pragma unroll
         for (int i = 0; i < PIECES / WAVES; ++i) {
             const int p = wave + i * WAVES;
-            if (p < BM / 8) dma_piece(a, stage + p * 1024, va, p * 8 * lda + chunk * CHUNK);
+            if (i * WAVES < BM / 8) dma_piece(a, stage + p * 1024, va, p * 8 * lda + chunk * CHUNK);
             else dma_piece(b, stage + p * 1024, vb, (p - BM / 8) * 8 * ldb + chunk * CHUNK);
         }
     }
@@ -70,7 +72,7 @@ struct ByteTile {
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(av[i], bv[j], acc[i][j], 0, 0, 0);
+                for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(bv[j], av[i], acc[i][j], 0, 0, 0);
         }
     }
     __device__ __forceinline__ void run(rsrc_t a, int lda, rsrc_t b, int ldb, int K, char* lds) {
@@ -86,52 +88,297 @@ struct ByteTile {
         issue(a, lda, va, b, ldb, vb, 0, lds, wave);
         wait_chunk();
         __builtin_amdgcn_s_barrier();
-        for (int c = 0; c < chunks; ++c) {
+        const char *as = lds + wm * WM * CHUNK, *bs = lds + (BM + wn * WN) * CHUNK;
+        const int whole = K / CHUNK;
+        for (int c = 0; c < whole; ++c) {
             if (c + 1 < chunks) issue(a, lda, va, b, ldb, vb, c + 1, lds + ((c + 1) & 1) * STAGE, wave);
-            const char* as = lds + (c & 1) * STAGE + wm * WM * CHUNK;
-            const char* bs = lds + (c & 1) * STAGE + (BM + wn * WN) * CHUNK;
-            if ((c + 1) * CHUNK <= K) multiply<false>(as, bs, lane, 0, 0);
-            else multiply<true>(as, bs, lane, c * CHUNK, K);
+            multiply<false>(as + (c & 1) * STAGE, bs + (c & 1) * STAGE, lane, 0, 0);
+            wait_chunk();
+            __builtin_amdgcn_s_barrier();
+        }
+        if (whole < chunks) {
+            multiply<true>(as + (whole & 1) * STAGE, bs + (whole & 1) * STAGE, lane, whole * CHUNK, K);
             wait_chunk();
             __builtin_amdgcn_s_barrier();
         }
     }
 };
 
-template <class Tile, int BM, int BN, int DT>
-__global__ __launch_bounds__(Tile::THREADS) void i8_gemm_kernel(GemmArgs g) {
+// Workgroup -> tile.  Workgroups go round the 8 XCDs, each with an L2 of its own: XCD x takes the x-th eighth of the tiles in an order that walks
+// bands of GROUP tile rows column by column, so that the tiles an XCD works on at one time share their rows of A and B.
+constexpr int GROUP = 8;
+__device__ __forceinline__ void place(int id, int tiles_m, int tiles_n, int& tm, int& tn) {
+    const int total = tiles_m * tiles_n, q = total >> 3, r = total & 7, x = id & 7;
+    const int at = x * q + min(x, r) + (id >> 3);
+    const int band = at / (GROUP * tiles_n), in = at - band * GROUP * tiles_n, high = min(GROUP, tiles_m - band * GROUP);
+    tn = in / high;
+    tm = band * GROUP + in - tn * high;
+}
+
+template <class Tile, int DT>
+__global__ __launch_bounds__(Tile::THREADS, 2) void i8_gemm_kernel(GemmArgs g) {
     typedef typename OutT<DT>::T T;
-    __shared__ __attribute__((aligned(1024))) char lds[Tile::LDS];
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int z = blockIdx.y, z0 = z / g.n1, z1 = z - z0 * g.n1;
-    const int tm = blockIdx.x % g.tiles_m, tn = blockIdx.x / g.tiles_m;
-    const int m0 = tm * BM, n0 = tn * BN;
+    int tm, tn;
+    place(blockIdx.x, g.tiles_m, g.tiles_n, tm, tn);
+    const int m0 = tm * Tile::M, n0 = tn * Tile::N;
     const int row_bytes = (g.K + 15) & ~15;
     const signed char* a = g.a + z0 * g.a0 + z1 * g.a1 + (long long)m0 * g.lda;
     const signed char* b = g.b + z0 * g.b0 + z1 * g.b1 + (long long)n0 * g.ldb;
     Tile t;
-    t.run(rows_rsrc(a, min(g.M - m0, BM), g.lda, row_bytes), g.lda, rows_rsrc(b, min(g.N - n0, BN), g.ldb, row_bytes), g.ldb, g.K, lds);
+    t.run(rows_rsrc(a, min(g.M - m0, Tile::M), g.lda, row_bytes), g.lda, rows_rsrc(b, min(g.N - n0, Tile::N), g.ldb, row_bytes), g.ldb, g.K, lds);
     const float *sa = g.sa + z0 * g.sa0 + z1 * g.sa1, *sb = g.sb + z0 * g.sb0 + z1 * g.sb1;
     T* out = (T*)g.out + z0 * g.o0 + z1 * g.o1;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int mw = m0 + wave / Tile::ACROSS * Tile::MT * 32 + (lane >> 5) * 4, nw = n0 + wave % Tile::ACROSS * Tile::NT * 32 + (lane & 31);
+    // The stages are free (every wave is past its last barrier).  A wave turns its tile in a part of LDS of its own, 32 rows at a time: four
+    // columns of a row leave a lane at once, and 16 bytes of a row a lane go to memory, 64 lanes on whole lines.  (Straight from the registers a
+    // 16-bit store instruction covers 128 bytes instead of 1024: 8192 x 4800 x 4800 x 256 took three times as long.)
+    constexpr int ROW = Tile::NT * 32 * (int)sizeof(T) + 16, VEC = 16 / (int)sizeof(T), LANES = Tile::NT * 32 / VEC;   // bytes of a row, elements of a lane, lanes of a row
+    static_assert(Tile::WAVES * 32 * ROW + Tile::N * 4 <= Tile::LDS, "the turning space and the scales of b fit the stages");
+    char* turn = lds + wave * 32 * ROW;
+    float* scale_b = (float*)(lds + Tile::WAVES * 32 * ROW);
+    for (int i = threadIdx.x; i < Tile::N; i += Tile::THREADS) scale_b[i] = n0 + i < g.N ? sb[n0 + i] : 0.f;
+    __syncthreads();
+    const int mw = m0 + wave / Tile::ACROSS * Tile::MT * 32, nw = n0 + wave % Tile::ACROSS * Tile::NT * 32;
+    const int col = nw + (lane % LANES) * VEC;
+    const bool wide = g.wide && col + VEC <= g.N;
 #pragma unroll
-    for (int i = 0; i < Tile::MT; ++i)
+    for (int i = 0; i < Tile::MT; ++i) {
+        const int mine = mw + i * 32 + (lane & 31);
+        const float s = mine < g.M ? sa[mine] * g.alpha : 0.f;
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
+        for (int j = 0; j < Tile::NT; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int row = mw + i * 32 + q * 8 + e;
-                if (row >= g.M) continue;
-                const float s = sa[row] * g.alpha;
+            for (int q = 0; q < 4; ++q) {
+                typedef T T4 __attribute__((ext_vector_type(4)));
+                const f32x4 c = *reinterpret_cast<const f32x4*>(scale_b + nw - n0 + j * 32 + q * 8 + (lane >> 5) * 4);
+                T4 v;
 #pragma unroll
-                for (int j = 0; j < Tile::NT; ++j) {
-                    const int col = nw + j * 32;
-                    if (col < g.N) out[(long long)row * g.ldo + col] = (T)((float)t.acc[i][j][q * 4 + e] * s * sb[col]);
-                }
+                for (int e = 0; e < 4; ++e) v[e] = (T)((float)t.acc[i][j][q * 4 + e] * s * c[e]);
+                *reinterpret_cast<T4*>(turn + (lane & 31) * ROW + (j * 32 + q * 8 + (lane >> 5) * 4) * (int)sizeof(T)) = v;
             }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // the wave's own writes; no other wave touches this part
+#pragma unroll
+        for (int r0 = 0; r0 < 32; r0 += 64 / LANES) {
+            const int r = r0 + lane / LANES, row = mw + i * 32 + r;
+            const char* from = turn + r * ROW + (lane % LANES) * 16;
+            if (row < g.M) {
+                T* o = out + (long long)row * g.ldo + col;
+                if (wide) *reinterpret_cast<i32x4*>(o) = *reinterpret_cast<const i32x4*>(from);
+                else
+                    for (int e = 0; e < VEC && col + e < g.N; ++e) o[e] = reinterpret_cast<const T*>(from)[e];
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
 }
 
 typedef ByteTile<64, 64, 32, 32> Small;
+typedef ByteTile<128, 128, 64, 64> Middle;
+typedef ByteTile<256, 256, 128, 64> Large;
+
+// Short rows (K <= 256) and many of them on both sides -- the correlation volume: what is written dwarfs what is read and computed, so the stores
+// have to run all the time.  A workgroup keeps 256 rows of b (the output's columns) in registers, 64 in a wave, and lets rows of a stream past:
+// chunks of 32 rows in a ring of SLOTS, filled by LDS-DMA SLOTS - 1 chunks ahead; a chunk's results are turned in LDS and stored 16 bytes a lane.
+// Three workgroups share a CU, so that one's stores run beside another's products (two with a deeper ring: +8 % time).
+// vmcnt counts loads and stores and retires them in order: a wave issues PW pieces and NS stores a chunk, always (what lies outside is dropped by
+// the bounds check), so "chunk c has landed" is a fixed count that leaves the stores of SLOTS - 1 chunks in flight.
+constexpr int STREAM_WGS = 2048;       // workgroups aimed at
+constexpr int STREAM_ROWS = 512;       // rows of a that a workgroup takes at most (their scales wait in LDS)
+struct StreamArgs {
+    GemmArgs g;
+    int panels, ranges, rows;          // column panels, row ranges, rows of a range (a multiple of 32)
+};
+
+template <int KC, int DT>
+__global__ __launch_bounds__(256, 3) void i8_stream_kernel(StreamArgs s) {
+    typedef typename OutT<DT>::T T;
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    const GemmArgs& g = s.g;
+    constexpr int SLOTS = 3, SLOT = 32 * KC * CHUNK, PW = KC, NT = 2;
+    constexpr int TURN = 128 / (int)sizeof(T), TURNS = 64 / TURN;            // columns turned at a time: 128 bytes of a row
+    constexpr int ROW = 128 + 16, VEC = 16 / (int)sizeof(T), NS = 4 * TURNS; // 8 lanes a row, 8 rows a store
+    __shared__ __attribute__((aligned(1024))) char ring[SLOTS * SLOT];
+    __shared__ __attribute__((aligned(16))) char turns[4 * 32 * ROW];
+    __shared__ __attribute__((aligned(16))) float scale_a[STREAM_ROWS], scale_b[256];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int z = blockIdx.y, z0 = z / g.n1, z1 = z - z0 * g.n1;
+    const int range = blockIdx.x / s.panels, n0 = (blockIdx.x - range * s.panels) * 256, m0 = range * s.rows;
+    const int rows = min(s.rows, g.M - m0), chunks = (rows + 31) / 32;
+    const int row_bytes = (g.K + 15) & ~15;
+    const float *sa = g.sa + z0 * g.sa0 + z1 * g.sa1 + m0, *sb = g.sb + z0 * g.sb0 + z1 * g.sb1 + n0;
+    for (int i = threadIdx.x; i < s.rows; i += 256) scale_a[i] = i < rows ? sa[i] * g.alpha : 0.f;
+    scale_b[threadIdx.x] = n0 + (int)threadIdx.x < g.N ? sb[threadIdx.x] : 0.f;
+    // the wave's columns, whole
+    const int nw = n0 + wave * 64;
+    const rsrc_t rb = rows_rsrc(g.b + z0 * g.b0 + z1 * g.b1 + (long long)nw * g.ldb, min(g.N - nw, 64), g.ldb, row_bytes);
+    i32x4 bv[NT][KC * 4];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int u = 0; u < KC * 4; ++u) {
+            const int k = u * 32 + (lane >> 5) * 16;
+            bv[j][u] = cut(__builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rb, (j * 32 + (lane & 31)) * g.ldb + k, 0, 0)), k, g.K);
+        }
+    const rsrc_t ra = rows_rsrc(g.a + z0 * g.a0 + z1 * g.a1 + (long long)m0 * g.lda, rows, g.lda, row_bytes);
+    const rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc((void*)((T*)g.out + z0 * g.o0 + z1 * g.o1 + (long long)m0 * g.ldo), 0, 0x7fffffff, 0x00020000);
+    const int va = lane_offset(lane, g.lda);
+    // a chunk lies as KC columns of 32 rows x 128 bytes; a wave moves eight rows of each
+    auto issue = [&](int c, int slot) {
+#pragma unroll
+        for (int i = 0; i < PW; ++i)
+            dma_piece(ra, ring + slot * SLOT + i * 32 * CHUNK + wave * 1024, va, (c * 32 + wave * 8) * g.lda + i * CHUNK);
+    };
+    __syncthreads();                    // the scales
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int c = 0; c < SLOTS - 1; ++c) issue(c, c);
+    char* turn = turns + wave * 32 * ROW;
+    int slot = 0;
+    for (int c = 0; c < chunks; ++c) {
+        if (c < SLOTS - 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((SLOTS - 2) * PW) : "memory");
+        else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((SLOTS - 2) * PW + (SLOTS - 1) * NS) : "memory");
+        __builtin_amdgcn_s_barrier();
+        issue(c + SLOTS - 1, slot == 0 ? SLOTS - 1 : slot - 1);     // (behind the last chunk: rows outside, zeros into a slot that nobody reads)
+        const char* as = ring + slot * SLOT;
+        slot = slot == SLOTS - 1 ? 0 : slot + 1;
+        i32x16 acc[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) acc[j][k] = 0;
+#pragma unroll
+        for (int u = 0; u < KC * 4; ++u) {
+            const i32x4 av = frag(as + u / 4 * 32 * CHUNK, lane, u & 3);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(bv[j][u], av, acc[j], 0, 0, 0);
+        }
+        const float sr = scale_a[c * 32 + (lane & 31)];
+#pragma unroll
+        for (int t = 0; t < TURNS; ++t) {
+#pragma unroll
+            for (int j = t * NT / TURNS; j < (t + 1) * NT / TURNS; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int at = j * 32 + q * 8 + (lane >> 5) * 4;
+                    const f32x4 sc = *reinterpret_cast<const f32x4*>(scale_b + wave * 64 + at);
+                    T4 v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = (T)((float)acc[j][q * 4 + e] * sr * sc[e]);
+                    *reinterpret_cast<T4*>(turn + (lane & 31) * ROW + (at - t * TURN) * (int)sizeof(T)) = v;
+                }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // the wave's own writes; no other wave touches this part
+            const int col = nw + t * TURN + (lane & 7) * VEC;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = i * 8 + (lane >> 3), row = c * 32 + r;
+                const i32x4 v = *reinterpret_cast<const i32x4*>(turn + r * ROW + (lane & 7) * 16);
+                const unsigned off = row < rows && col < g.N ? (unsigned)(((long long)row * g.ldo + col) * (int)sizeof(T)) : 0x80000000u;
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), ro, off, 0, 2);   // nt: what is written is not read here
+            }
+            if (t + 1 < TURNS) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // no piece lands in LDS that is no longer this workgroup's
+}
+
+// Few rows on one side (R <= 16 * RT), the other side's rows (many) read once: 16 of them for a workgroup, straight from memory into the
+// fragments, the contraction split over its four waves and joined in LDS.  `many` is b (the output's columns) or a, by the strides given.
+struct SkinnyArgs {
+    const signed char *few, *many;
+    const float *sf, *sm;
+    void* out;
+    long long f0, f1, m0, m1, sf0, sf1, sm0, sm1, o0, o1;
+    int ldf, ldm;
+    long long of, om;      // strides of the output along the few and the many rows
+    int F, M, K, n1;
+    float alpha;
+};
+constexpr int SKINNY_AHEAD = 8;    // steps of 64 k in flight
+
+template <int RT, int DT>
+__global__ __launch_bounds__(256) void i8_skinny_kernel(SkinnyArgs g) {
+    typedef typename OutT<DT>::T T;
+    __shared__ i32x4 part[4][RT][64];
+    const int z = blockIdx.y, z0 = z / g.n1, z1 = z - z0 * g.n1;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r0 = blockIdx.x * 16;
+    const int row_bytes = (g.K + 15) & ~15;
+    const rsrc_t many = rows_rsrc(g.many + z0 * g.m0 + z1 * g.m1 + (long long)r0 * g.ldm, min(16, g.M - r0), g.ldm, row_bytes);
+    const rsrc_t few = rows_rsrc(g.few + z0 * g.f0 + z1 * g.f1, g.F, g.ldf, row_bytes);
+    const int steps = (g.K + 63) / 64, per = (steps + 3) / 4, first = wave * per, last = min(steps, first + per);
+    const int k_lane = (lane >> 4) * 16, vm = (lane & 15) * g.ldm + k_lane, vf = (lane & 15) * g.ldf + k_lane;
+    i32x4 acc[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) acc[t] = i32x4{0, 0, 0, 0};
+    for (int s = first; s < last; s += SKINNY_AHEAD) {
+        i32x4 mv[SKINNY_AHEAD], fv[RT][SKINNY_AHEAD];
+#pragma unroll
+        for (int u = 0; u < SKINNY_AHEAD; ++u) {
+            const int k = min(s + u, last - 1) * 64;        // (behind the last step: read again, not counted)
+            mv[u] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(many, vm, k, 0));
+#pragma unroll
+            for (int t = 0; t < RT; ++t) fv[t][u] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(few, vf + t * 16 * g.ldf, k, 0));
+        }
+#pragma unroll
+        for (int u = 0; u < SKINNY_AHEAD; ++u) {
+            const i32x4 m = s + u < last ? cut(mv[u], (s + u) * 64 + k_lane, g.K) : i32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int t = 0; t < RT; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fv[t][u], m, acc[t], 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < RT; ++t) part[wave][t][lane] = acc[t];
+    __syncthreads();
+    // lane: column (of the many) lane % 16, rows (of the few) 4 * (lane / 16) .. + 3
+    const int col = r0 + (lane & 15);
+    if (wave < RT && col < g.M) {
+        const i32x4 v = part[0][wave][lane] + part[1][wave][lane] + part[2][wave][lane] + part[3][wave][lane];
+        const float sm = g.sm[z0 * g.sm0 + z1 * g.sm1 + col];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int row = wave * 16 + (lane >> 4) * 4 + e;
+            if (row < g.F) {
+                const float sf = g.sf[z0 * g.sf0 + z1 * g.sf1 + row];
+                ((T*)g.out)[z0 * g.o0 + z1 * g.o1 + row * g.of + col * g.om] = (T)((float)v[e] * (sf * g.alpha) * sm);
+            }
+        }
+    }
+}
+
+template <class Tile>
+int launch_tiles(GemmArgs g, int dtype, unsigned batch, hipStream_t st) {
+    g.tiles_m = ceil_div(g.M, Tile::M);
+    g.tiles_n = ceil_div(g.N, Tile::N);
+    BFLOW_REQUIRE((long long)g.tiles_m * g.tiles_n < (1LL << 30), BFLOW_E_LIMIT, "i8_gemm: too many tiles");
+    const auto kernel = dtype == F32 ? i8_gemm_kernel<Tile, F32> : dtype == F16 ? i8_gemm_kernel<Tile, F16> : i8_gemm_kernel<Tile, BF16>;
+    if (Tile::LDS > 65536) {
+        const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, Tile::LDS);
+        BFLOW_REQUIRE(e == hipSuccess, (int)e, "i8_gemm: %s", hipGetErrorString(e));
+    }
+    hipLaunchKernelGGL(kernel, dim3(g.tiles_m * g.tiles_n, batch), dim3(Tile::THREADS), Tile::LDS, st, g);
+    return launch_status("i8_gemm");
+}
+int launch_stream(const GemmArgs& g, int dtype, unsigned batch, hipStream_t st) {
+    StreamArgs s = {g, ceil_div(g.N, 256), 0, 0};
+    const long long panels = (long long)s.panels * batch, chunks = ceil_div(g.M, 32);
+    long long ranges = (STREAM_WGS + panels - 1) / panels, per = (chunks + ranges - 1) / ranges;
+    per = per > STREAM_ROWS / 32 ? STREAM_ROWS / 32 : per;
+    s.rows = (int)per * 32;
+    s.ranges = ceil_div(g.M, s.rows);
+    BFLOW_REQUIRE((long long)s.panels * s.ranges < (1LL << 30), BFLOW_E_LIMIT, "i8_gemm: too many panels");
+    const bool one = g.K <= CHUNK;
+    const auto kernel = one ? (dtype == F32 ? i8_stream_kernel<1, F32> : dtype == F16 ? i8_stream_kernel<1, F16> : i8_stream_kernel<1, BF16>)
+                            : (dtype == F32 ? i8_stream_kernel<2, F32> : dtype == F16 ? i8_stream_kernel<2, F16> : i8_stream_kernel<2, BF16>);
+    hipLaunchKernelGGL(kernel, dim3(s.panels * s.ranges, batch), dim3(256), 0, st, s);
+    return launch_status("i8_gemm");
+}
+template <int RT>
+int launch_skinny(const SkinnyArgs& g, int dtype, unsigned batch, hipStream_t st) {
+    const auto kernel = dtype == F32 ? i8_skinny_kernel<RT, F32> : dtype == F16 ? i8_skinny_kernel<RT, F16> : i8_skinny_kernel<RT, BF16>;
+    hipLaunchKernelGGL(kernel, dim3((g.M + 15) / 16, batch), dim3(256), 0, st, g);
+    return launch_status("i8_gemm");
+}
 
 // ---------------------------------------------------------------------------------------------------------------------- quantisation
 // |x| as an integer that orders like it, NaN above all
@@ -182,42 +429,99 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const void* x, long 
     }
 }
 
-// 64 pixels of a workgroup, all D channels.  Row r of q is pixel r, or in the 4 x 8 tile order of the look-up (tiled); rows without a pixel
-// are zero with scale 0.  PACKED: x is the fp16-pair operand (hi, lo planes of 32 channels by `np` pixels), else (B, D, h, w) in 32 bits.
-template <bool PACKED>
-__global__ __launch_bounds__(256) void quantize_pixels_kernel(const float* x, const _Float16* hi, const _Float16* lo, int D, int h, int w, int np, int rows, int tiled,
-                                                              signed char* q, float* scale) {
-    __shared__ unsigned most[4][64];
-    const int b = blockIdx.y, p = threadIdx.x & 63, c = threadIdx.x >> 6, r = blockIdx.x * 64 + p;
-    int pix = -1;
-    if (r < rows) {
-        if (tiled) {
-            const int across = (w + 7) / 8, tile = r >> 5, y = tile / across * 4 + ((r & 31) >> 3), xx = tile % across * 8 + (r & 7);
-            if (y < h && xx < w) pix = y * w + xx;
-        } else pix = r;
-    }
-    auto value = [&](int d) {
-        if constexpr (PACKED) {
-            const long long i = (((long long)b * (D / 32) + d / 32) * np + pix) * 32 + d % 32;
-            return fmaf((float)lo[i], SPLIT_LO_INV, (float)hi[i]);
-        } else return x[((long long)b * D + d) * h * w + pix];
+// Row r of a plane -> its pixel, -1 outside the map: in order, or in the 4 x 8 tile order of the look-up.
+__device__ __forceinline__ int pixel_of(int r, int rows, int tiled, int h, int w) {
+    if (r >= rows) return -1;
+    if (!tiled) return r;
+    const int across = (w + 7) / 8, tile = r >> 5, ty = tile / across, y = ty * 4 + ((r & 31) >> 3), x = (tile - ty * across) * 8 + (r & 7);
+    return y < h && x < w ? y * w + x : -1;
+}
+
+// Maps (B, D, h, w) in 32 bits.  A workgroup takes 64 rows of the result, a lane a row, a wave a sixteenth of the channels (of 256 of them at a
+// time): all loads of a thread are in flight at once and are kept, the whole numbers are turned in LDS and leave as whole rows.  10 us for
+// 4 x 256 x 60 x 80 (19.7 MB in, 4.9 out); four waves walking the channels twice took 43.
+constexpr int SEG = 256;
+__global__ __launch_bounds__(1024) void quantize_pixels_kernel(const float* x, int D, int h, int w, int rows, int tiled, signed char* q, float* scale) {
+    __shared__ unsigned most[16][64];
+    __shared__ __attribute__((aligned(16))) signed char turn[64][SEG + 16];
+    const int b = blockIdx.y, p = threadIdx.x & 63, c = threadIdx.x >> 6, r0 = blockIdx.x * 64, pix = pixel_of(r0 + p, rows, tiled, h, w);
+    const float* from = x + (long long)b * D * h * w + pix;
+    const long long plane = (long long)h * w;
+    float v[16];
+    auto load = [&](int d0) {                       // this thread's channels of the segment: d0 + c * per ..
+        const int n = min(SEG, D - d0), per = n / 16;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = e < per && pix >= 0 ? from[(d0 + c * per + e) * plane] : 0.f;
     };
-    const int per = (D / 4 + 3) / 4 * 4, first = c * per, last = min(D, first + per);     // this thread's channels, in fours
     unsigned m = 0;
-    if (pix >= 0)
-        for (int d = first; d < last; ++d) m = max(m, magnitude(value(d)));
+    for (int d0 = 0; d0 < D; d0 += SEG) {
+        load(d0);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) m = max(m, magnitude(v[e]));
+    }
     most[c][p] = m;
     __syncthreads();
-    const Quant f(max(max(most[0][p], most[1][p]), max(most[2][p], most[3][p])));
+#pragma unroll
+    for (int e = 0; e < 16; ++e) m = max(m, most[e][p]);
+    const Quant f(m);
+    const bool none = f.none();
+    if (c == 0 && r0 + p < rows) scale[(long long)b * rows + r0 + p] = f.scale();
+    for (int d0 = 0; d0 < D; d0 += SEG) {
+        if (D > SEG) load(d0);
+        const int n = min(SEG, D - d0), per = n / 16;
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            if (e < per) turn[p][c * per + e] = none ? 0 : (signed char)f(v[e]);
+        __syncthreads();
+        for (int i = threadIdx.x; i < 64 * per; i += 1024) {
+            const int r = i / per, k = (i - r * per) * 16;
+            if (r0 + r < rows) *reinterpret_cast<i32x4*>(q + ((long long)b * rows + r0 + r) * D + d0 + k) = *reinterpret_cast<const i32x4*>(&turn[r][k]);
+        }
+        __syncthreads();
+    }
+}
+
+// The conv engine's operand: hi and lo planes, 32 channels of a pixel together.  Four lanes a row, eight channels each of a block of 32.
+__global__ __launch_bounds__(256) void quantize_packed_kernel(const _Float16* hi, const _Float16* lo, int KB, int h, int w, int np, int rows, int tiled, signed char* q,
+                                                              float* scale) {
+    const int lane = threadIdx.x & 63, b = blockIdx.y, r = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 16 + (lane >> 2), pix = pixel_of(r, rows, tiled, h, w);
+    const long long at = ((long long)b * KB * np + max(pix, 0)) * 32 + (lane & 3) * 8, step = (long long)np * 32;
+    constexpr int KEEP = 8;                         // blocks of 32 channels kept in registers; further ones are read twice
+    half8 vh[KEEP], vl[KEEP];
+    unsigned m = 0;
+    auto worst = [&](half8 a, half8 l) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = max(m, magnitude(fmaf((float)l[e], SPLIT_LO_INV, (float)a[e])));
+    };
+#pragma unroll
+    for (int k = 0; k < KEEP; ++k)
+        if (k < KB) {
+            vh[k] = *reinterpret_cast<const half8*>(hi + at + k * step);
+            vl[k] = *reinterpret_cast<const half8*>(lo + at + k * step);
+        }
+#pragma unroll
+    for (int k = 0; k < KEEP; ++k)
+        if (k < KB) worst(vh[k], vl[k]);
+    for (int k = KEEP; k < KB; ++k) worst(*reinterpret_cast<const half8*>(hi + at + k * step), *reinterpret_cast<const half8*>(lo + at + k * step));
+    m = max(m, (unsigned)__shfl_xor((int)m, 1, 64));
+    m = max(m, (unsigned)__shfl_xor((int)m, 2, 64));
+    if (pix < 0) m = 0;
+    const Quant f(m);
     const bool none = f.none();
     if (r >= rows) return;
-    if (c == 0) scale[(long long)b * rows + r] = f.scale();
-    for (int d = first; d < last; d += 4) {
-        unsigned v = 0;
-        if (!none)
-            for (int e = 0; e < 4; ++e) v |= (unsigned)(f(value(d + e)) & 255) << (8 * e);
-        *reinterpret_cast<unsigned*>(q + ((long long)b * rows + r) * D + d) = v;
-    }
+    if ((lane & 3) == 0) scale[(long long)b * rows + r] = f.scale();
+    signed char* to = q + ((long long)b * rows + r) * KB * 32 + (lane & 3) * 8;
+    auto put = [&](int k, half8 a, half8 l) {
+        unsigned u[2] = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (!none) u[e >> 2] |= (unsigned)(f(fmaf((float)l[e], SPLIT_LO_INV, (float)a[e])) & 255) << (8 * (e & 3));
+        *reinterpret_cast<uint2*>(to + k * 32) = make_uint2(u[0], u[1]);
+    };
+#pragma unroll
+    for (int k = 0; k < KEEP; ++k)
+        if (k < KB) put(k, vh[k], vl[k]);
+    for (int k = KEEP; k < KB; ++k) put(k, *reinterpret_cast<const half8*>(hi + at + k * step), *reinterpret_cast<const half8*>(lo + at + k * step));
 }
 }  // namespace
 
@@ -235,13 +539,66 @@ extern "C" int bflow_i8_gemm(const bflow_i8_gemm_t* d, bflow_stream_t stream) {
                    (unsigned long long)d->b_stride0 | (unsigned long long)d->b_stride1) % 16 == 0, BFLOW_E_ARG, "i8_gemm: operands and their strides are multiples of 16 bytes");
     const long long batch = (long long)d->batch0 * d->batch1;
     BFLOW_REQUIRE(batch <= 65535, BFLOW_E_LIMIT, "i8_gemm: %lld matrices > 65535", batch);
-    GemmArgs g = {(const signed char*)d->a, (const signed char*)d->b, d->scale_a, d->scale_b, d->out, d->a_stride0, d->a_stride1, d->b_stride0, d->b_stride1,
-                  d->sa_stride0, d->sa_stride1, d->sb_stride0, d->sb_stride1, d->out_stride0, d->out_stride1, d->lda, d->ldb, d->ldo, d->M, d->N, d->K, d->batch1, d->alpha,
-                  ceil_div(d->M, 64), ceil_div(d->N, 64)};
-    BFLOW_REQUIRE((long long)g.tiles_m * g.tiles_n < (1LL << 31), BFLOW_E_LIMIT, "i8_gemm: too many tiles");
-    const auto kernel = d->dtype == F32 ? i8_gemm_kernel<Small, 64, 64, F32> : d->dtype == F16 ? i8_gemm_kernel<Small, 64, 64, F16> : i8_gemm_kernel<Small, 64, 64, BF16>;
-    hipLaunchKernelGGL(kernel, dim3(g.tiles_m * g.tiles_n, (unsigned)batch), dim3(256), 0, (hipStream_t)stream, g);
-    return launch_status("i8_gemm");
+    const int size = d->dtype == F32 ? 4 : 2;
+    const GemmArgs g = {(const signed char*)d->a, (const signed char*)d->b, d->scale_a, d->scale_b, d->out, d->a_stride0, d->a_stride1, d->b_stride0, d->b_stride1,
+                        d->sa_stride0, d->sa_stride1, d->sb_stride0, d->sb_stride1, d->out_stride0, d->out_stride1, d->lda, d->ldb, d->ldo, d->M, d->N, d->K, d->batch1,
+                        d->alpha, 0, 0, ((uintptr_t)d->out | (unsigned long long)size * (unsigned long long)(d->ldo | d->out_stride0 | d->out_stride1)) % 16 == 0};
+    const hipStream_t st = (hipStream_t)stream;
+    // Few rows on one side: 6.4 us against 11.9 for one row at N = K = 4096, 10.0 against 12.1 for 32, 11.9 either way for 48.
+    if (d->M <= 32 || d->N <= 32) {
+        const SkinnyArgs s = d->M <= d->N ? SkinnyArgs{g.a, g.b, g.sa, g.sb, g.out, g.a0, g.a1, g.b0, g.b1, g.sa0, g.sa1, g.sb0, g.sb1, g.o0, g.o1, g.lda, g.ldb, g.ldo, 1, g.M, g.N, g.K, g.n1, g.alpha}
+                                          : SkinnyArgs{g.b, g.a, g.sb, g.sa, g.out, g.b0, g.b1, g.a0, g.a1, g.sb0, g.sb1, g.sa0, g.sa1, g.o0, g.o1, g.ldb, g.lda, 1, g.ldo, g.N, g.M, g.K, g.n1, g.alpha};
+        return s.F <= 16 ? launch_skinny<1>(s, d->dtype, (unsigned)batch, st) : launch_skinny<2>(s, d->dtype, (unsigned)batch, st);
+    }
+    // Short rows, whole 16-byte stores: 55 us against 64 (256 x 256 tiles) for 4 x 4800 x 4800 x 256 in fp16, 81 against 88 in fp32, 709 against 1233
+    // for 6 x 16384 x 16384 x 256; with less than a panel on either side it has nothing to stream.
+    if (d->K <= 256 && d->M >= 256 && d->N >= 256 && g.wide && d->N % (16 / size) == 0 && d->lda <= 1 << 20 && (long long)STREAM_ROWS * d->ldo * size < (1LL << 31))
+        return launch_stream(g, d->dtype, (unsigned)batch, st);
+    // Tiles by the rounds that they take on 256 CUs, priced by what a round took at K = 4096: 256 tiles of 256 x 256 79 us, 512 of 128 x 128 (two on a
+    // CU) 44, 1024 of 64 x 64 (four) 28.  4096^3: 79 / 88 / 112 us; 2048^3: 38 / 19 / 18; 1024^3: 23 / 11 / 6.2; 8192^3: 515 / 576 / 814.
+    auto price = [&](int side, long long room, int us) { return ((long long)ceil_div(d->M, side) * ceil_div(d->N, side) * batch + room - 1) / room * us; };
+    const long long large = price(256, 256, 79), middle = price(128, 512, 44), small = price(64, 1024, 28);
+    if (small <= middle && small <= large) return launch_tiles<Small>(g, d->dtype, (unsigned)batch, st);
+    if (middle <= large) return launch_tiles<Middle>(g, d->dtype, (unsigned)batch, st);
+    return launch_tiles<Large>(g, d->dtype, (unsigned)batch, st);
+}
+
+// Rows at any address -> rows at multiples of 16 bytes: dwords are read where they stand and shifted together.  No word is read that holds none of
+// the row's bytes.
+struct PadArgs { bflow_i8_pad_t v[2]; };
+__global__ __launch_bounds__(256) void pad_rows_kernel(PadArgs p) {
+    const bflow_i8_pad_t d = p.v[blockIdx.y];
+    const int across = d.ldd / 16;
+    const long long n = d.rows * across;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+        const long long row = i / across;
+        const int k = (int)(i - row * across) * 16;
+        const uintptr_t from = (uintptr_t)d.src + row * d.ld + k;
+        const int shift = (int)(from & 3), bytes = min(16, d.K - k) + shift;      // counted from the first word
+        const unsigned* w = (const unsigned*)(from - shift);
+        unsigned x[5];
+#pragma unroll
+        for (int e = 0; e < 5; ++e) x[e] = 4 * e < bytes ? w[e] : 0u;
+        u32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_alignbyte(x[e + 1], x[e], shift);
+        *reinterpret_cast<u32x4*>((char*)d.dst + row * d.ldd + k) = v;
+    }
+}
+
+extern "C" int bflow_i8_pad_rows(const bflow_i8_pad_t* items, int count, bflow_stream_t stream) {
+    BFLOW_REQUIRE(items && count >= 1 && count <= 2, BFLOW_E_ARG, "i8_pad_rows: one or two operands");
+    PadArgs p = {};
+    long long most = 0;
+    for (int i = 0; i < count; ++i) {
+        const bflow_i8_pad_t& d = items[i];
+        BFLOW_REQUIRE(d.src && d.dst && d.rows >= 1 && d.K >= 1 && d.ldd >= d.K && d.ldd % 16 == 0 && (uintptr_t)d.dst % 16 == 0, BFLOW_E_ARG,
+                      "i8_pad_rows: %lld rows of %d, ldd %d", d.rows, d.K, d.ldd);
+        p.v[i] = d;
+        most = d.rows * (d.ldd / 16) > most ? d.rows * (d.ldd / 16) : most;
+    }
+    hipLaunchKernelGGL(pad_rows_kernel, dim3(stream_grid(most, 256), count), dim3(256), 0, (hipStream_t)stream, p);
+    return launch_status("i8_pad_rows");
 }
 
 extern "C" int bflow_i8_quantize_rows(const void* x, int dtype, long long ld, long long rows, int K, signed char* q, int ldq, float* scale, bflow_stream_t stream) {
@@ -264,7 +621,7 @@ extern "C" int bflow_i8_quantize_pixels(const float* x, const void* x_hi, const 
     BFLOW_REQUIRE((uintptr_t)q % 16 == 0, BFLOW_E_ARG, "i8_quantize_pixels: q is not aligned to 16 bytes");
     const int rows = tiled ? (h + 3) / 4 * ((w + 7) / 8) * 32 : h * w;
     const dim3 grid((rows + 63) / 64, B);
-    if (x) hipLaunchKernelGGL(quantize_pixels_kernel<false>, grid, dim3(256), 0, (hipStream_t)stream, x, nullptr, nullptr, D, h, w, 0, rows, tiled, q, scale);
-    else hipLaunchKernelGGL(quantize_pixels_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, nullptr, (const _Float16*)x_hi, (const _Float16*)x_lo, D, h, w, np, rows, tiled, q, scale);
+    if (x) hipLaunchKernelGGL(quantize_pixels_kernel, grid, dim3(1024), 0, (hipStream_t)stream, x, D, h, w, rows, tiled, q, scale);
+    else hipLaunchKernelGGL(quantize_packed_kernel, grid, dim3(256), 0, (hipStream_t)stream, (const _Float16*)x_hi, (const _Float16*)x_lo, D / 32, h, w, np, rows, tiled, q, scale);
     return launch_status("i8_quantize_pixels");
 }

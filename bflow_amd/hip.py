@@ -10,8 +10,10 @@ There is NO fallback: if the shared library is missing or a tensor lives on the 
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
+import struct
 from typing import Optional, Sequence
 
 import numpy as np
@@ -35,7 +37,7 @@ EXPORTS = (
     "bflow_flow_metrics_accumulate", "bflow_traj_len", "bflow_pad_replicate", "bflow_voxel_grid_rectified", "bflow_voxel_grid_rectified_window", "bflow_maxabs_diff",
     "bflow_corr_lookup_bwd", "bflow_corr_lookup_bezier_bwd", "bflow_corr_pool2x2_bwd", "bflow_cvx_upsample_bwd", "bflow_l1_masked_accumulate",
     "bflow_l1_masked_grad", "bflow_conv_split_pair", "bflow_corr_lookup_im2col", "bflow_cvx_upsample_blocked",
-    "bflow_ns_workspace_bytes", "bflow_ns_orthogonalize", "bflow_muon_step", "bflow_i8_gemm", "bflow_i8_quantize_rows", "bflow_i8_quantize_pixels",
+    "bflow_ns_workspace_bytes", "bflow_ns_orthogonalize", "bflow_muon_step", "bflow_i8_gemm", "bflow_i8_pad_rows", "bflow_i8_quantize_rows", "bflow_i8_quantize_pixels",
 )
 
 
@@ -96,12 +98,10 @@ class NormDesc(ctypes.Structure):
                 ("stats_replicas", ctypes.c_int), ("act_b", ctypes.c_int)]
 
 
-class I8GemmDesc(ctypes.Structure):
-    """struct bflow_i8_gemm_desc (include/bflow_hip.h)."""
-    _fields_ = [(n, ctypes.c_void_p) for n in ("a", "b", "scale_a", "scale_b", "out")] + \
-               [(n, ctypes.c_longlong) for n in ("a_stride0", "a_stride1", "b_stride0", "b_stride1", "sa_stride0", "sa_stride1", "sb_stride0", "sb_stride1",
-                                                 "out_stride0", "out_stride1", "ldo")] + \
-               [(n, ctypes.c_int) for n in ("lda", "ldb", "M", "N", "K", "batch0", "batch1", "dtype")] + [("alpha", ctypes.c_float)]
+# struct bflow_i8_gemm_desc, bflow_i8_pad (include/bflow_hip.h), packed by the caller: these calls are short, and a ctypes structure of 25 fields costs
+# as much as the launch
+I8_GEMM = struct.Struct("5Q11q8if4x")       # a b scale_a scale_b out | strides 0, 1 of a, b, sa, sb, out; ldo | lda ldb M N K batch0 batch1 dtype | alpha
+I8_PAD = struct.Struct("2Q2q2i")            # src dst | ld rows | K ldd
 
 
 # struct bflow_ns_matrix (include/bflow_hip.h), as rows of a host table
@@ -203,7 +203,8 @@ def lib() -> ctypes.CDLL:
         "bflow_cvx_upsample_bwd": [vp, vp, vp, vp, vp, vp, i, i, i, i, vp],
         "bflow_l1_masked_accumulate": [vp, vp, vp, i, i, ll, vp, vp],
         "bflow_l1_masked_grad": [vp, vp, vp, i, i, ll, vp, vp, f, vp, vp],
-        "bflow_i8_gemm": [ctypes.POINTER(I8GemmDesc), vp],
+        "bflow_i8_gemm": [ctypes.c_char_p, vp],
+        "bflow_i8_pad_rows": [ctypes.c_char_p, i, vp],
         "bflow_i8_quantize_rows": [vp, i, ll, ll, i, vp, i, vp, vp],
         "bflow_i8_quantize_pixels": [vp, vp, vp, i, i, i, i, i, i, vp, vp, vp],
         "bflow_ns_workspace_bytes": [vp, i],
@@ -227,7 +228,15 @@ def _check(rc: int, what: str):
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())      # torch.cuda.current_stream().cuda_stream without the Stream object
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """The context in which launches go to `device` (nothing to do where it is the current one)."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _dev(t: torch.Tensor, dtype=torch.float32, name: str = "tensor", contiguous: bool = True) -> int:
@@ -893,7 +902,7 @@ def _ns_workspace(table: np.ndarray, device: torch.device) -> torch.Tensor:
 def ns_orthogonalize(table: np.ndarray, dtype: torch.dtype, device: torch.device, steps: int, coefficients: Sequence[float], eps: float):
     """table: NS_MATRIX rows (src, dst, leading dimensions, rows, cols) of matrices of one dtype on `device`."""
     a, b, c = coefficients
-    with torch.cuda.device(device):
+    with _on(device):
         ws = _ns_workspace(table, device)
         _check(lib().bflow_ns_orthogonalize(table.ctypes.data, len(table), FLOAT_CODES[dtype], steps, a, b, c, eps, ws.data_ptr(), ws.numel(), _stream()),
                "bflow_ns_orthogonalize")
@@ -905,7 +914,7 @@ def muon_step(table: np.ndarray, device: torch.device, steps: int, coefficients:
     kernels when they run."""
     a, b, c = coefficients
     on_device = isinstance(lr, torch.Tensor)
-    with torch.cuda.device(device):
+    with _on(device):
         ws = _ns_workspace(table, device)
         _check(lib().bflow_muon_step(table.ctypes.data, len(table), steps, a, b, c, eps, momentum, int(nesterov), 0.0 if on_device else lr,
                                      _dev(lr, name="lr") if on_device else None, weight_decay, ws.data_ptr(), ws.numel(), _stream()), "bflow_muon_step")

@@ -10,7 +10,6 @@ The correlation volume runs on it with `correlation.precision: i8` (corr.py).
 """
 from __future__ import annotations
 
-import ctypes
 from typing import Optional, Tuple
 
 import torch
@@ -35,7 +34,7 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     if rows:
         flat = x.reshape(rows, K)                          # a view where the rows are evenly spaced
         flat = flat if flat.stride(1) == 1 or K == 1 else flat.contiguous()
-        with torch.cuda.device(x.device):
+        with hip._on(x.device):
             hip._check(hip.lib().bflow_i8_quantize_rows(flat.data_ptr(), hip.FLOAT_CODES[x.dtype], flat.stride(0), rows, K, q.data_ptr(), _padded(K), scale.data_ptr(),
                                                         hip._stream()), "bflow_i8_quantize_rows")
     return q[..., :K], scale
@@ -68,34 +67,78 @@ def _quantize_pixels(x, hi, lo, np_rows, device, lead, D, h, w, tiled):
     if D < 16 or D % 16:
         raise hip.BflowHipError(f"quantize_pixels: {D} channels, a multiple of 16 is needed")
     if B:
-        with torch.cuda.device(device):
+        with hip._on(device):
             hip._check(hip.lib().bflow_i8_quantize_pixels(x, hi, lo, np_rows, B, D, h, w, int(tiled), q.data_ptr(), scale.data_ptr(), hip._stream()),
                        "bflow_i8_quantize_pixels")
     return q, scale
 
 
-def _operand(t: torch.Tensor, what: str) -> torch.Tensor:
+def _ready(t: torch.Tensor, K: int) -> bool:
     """(..., rows, K) as the kernel reads it: K contiguous, everything else at multiples of 16 bytes, every row readable up to K rounded up to 16."""
-    hip._dev(t, torch.int8, what, contiguous=False)
-    rows, K = t.shape[-2:]
-    steps = [s for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n > 1]
-    last = t.storage_offset() + sum((n - 1) * s for n, s in zip(t.shape[:-1], t.stride()[:-1])) + _padded(K)
-    if (t.stride(-1) == 1 or K == 1) and t.data_ptr() % 16 == 0 and all(s % 16 == 0 for s in steps) and last <= t.untyped_storage().nbytes() \
-            and (rows == 1 or _padded(K) <= t.stride(-2) <= 1 << 22):
-        return t
-    room = torch.empty(t.shape[:-1] + (_padded(K),), dtype=torch.int8, device=t.device)
-    room[..., :K].copy_(t)
-    return room[..., :K]
+    shape, strides = t.shape, t.stride()
+    if (strides[-1] != 1 and K > 1) or t.data_ptr() % 16:
+        return False
+    need = (K + 15) & ~15
+    if shape[-2] > 1 and not need <= strides[-2] <= 1 << 22:
+        return False
+    for n, s in zip(shape[:-1], strides[:-1]):
+        if s % 16 and n > 1:
+            return False
+    if need == K:
+        return True
+    last = t.storage_offset() + sum((n - 1) * s for n, s in zip(shape[:-1], strides[:-1])) + need
+    return last <= t.untyped_storage().nbytes()
 
 
-def _two(t: torch.Tensor, batch: Tuple[int, ...], tail: int) -> torch.Tensor:
-    """t (..., tail dimensions) spread over `batch`, as (n0, n1, tail dimensions); repeated dimensions keep stride 0."""
-    t = t.expand(tuple(batch) + tuple(t.shape[-tail:]))
-    if len(batch) > 2:
-        t = t.flatten(0, len(batch) - 2)
-    while t.dim() < tail + 2:
-        t = t.unsqueeze(0)
-    return t
+def _operands(ts, K: int, device):
+    """The operands as the kernel reads them: those that are not are copied, rows 16 bytes apart or a multiple, in one launch where they are rows of
+    bytes at even distances."""
+    out, items = list(ts), []
+    ldd = _padded(K)
+    for i, t in enumerate(ts):
+        if _ready(t, K):
+            continue
+        room = torch.empty(t.shape[:-1] + (ldd,), dtype=torch.int8, device=device)
+        shape, strides = t.shape, t.stride()
+        even = (strides[-1] == 1 or K == 1) and (t.dim() == 2 or (t.dim() == 3 and strides[0] == shape[1] * strides[1]))
+        if even:
+            items.append(hip.I8_PAD.pack(t.data_ptr(), room.data_ptr(), strides[-2], room.numel() // ldd, K, ldd))
+        else:
+            room[..., :K].copy_(t)
+        out[i] = room[..., :K]
+    if items:
+        hip._check(hip.lib().bflow_i8_pad_rows(b"".join(items), len(items), hip._stream()), "bflow_i8_pad_rows")
+    return out
+
+
+def _broadcast(a: Tuple[int, ...], b: Tuple[int, ...]) -> Tuple[int, ...]:
+    n = max(len(a), len(b))
+    a, b = (1,) * (n - len(a)) + tuple(a), (1,) * (n - len(b)) + tuple(b)
+    for x, y in zip(a, b):
+        if x != y and x != 1 and y != 1:
+            raise hip.BflowHipError(f"matmul: leading dimensions {a} and {b} do not broadcast")
+    return tuple(y if x == 1 else x for x, y in zip(a, b))
+
+
+def _lead_strides(t: torch.Tensor, lead: int, batch: Tuple[int, ...]):
+    """Strides of t's first `lead` dimensions over `batch`; 0 where an element is repeated or there is only one."""
+    miss = len(batch) - lead
+    return [0] * miss + [s if n > 1 else 0 for n, s in zip(t.shape[:lead], t.stride()[:lead])]
+
+
+def _fold(batch, strides):
+    """The batch dimensions as two, with each operand's strides: neighbours become one where every operand steps evenly over them.  None where more than
+    two are left."""
+    dims = [(n, [s[i] for s in strides]) for i, n in enumerate(batch) if n > 1]
+    i = len(dims) - 2
+    while i >= 0 and len(dims) > 2:
+        (n0, s0), (n1, s1) = dims[i], dims[i + 1]
+        if all(x == n1 * y for x, y in zip(s0, s1)):
+            dims[i:i + 2] = [(n0 * n1, s1)]
+        i -= 1
+    if len(dims) > 2:
+        return None
+    return [(1, [0] * len(strides))] * (2 - len(dims)) + dims
 
 
 def matmul(a: torch.Tensor, scale_a: torch.Tensor, b: torch.Tensor, scale_b: torch.Tensor, out_dtype: torch.dtype = torch.float32, alpha: float = 1.0,
@@ -103,45 +146,50 @@ def matmul(a: torch.Tensor, scale_a: torch.Tensor, b: torch.Tensor, scale_b: tor
     """a (..., M, K) int8 with scales (..., M), b (..., N, K) int8 with scales (..., N) -> (..., M, N) of out_dtype (float32, float16, bfloat16):
     alpha * scale_a * scale_b * (a @ b^T), rounded once.  Leading dimensions broadcast.  Operands whose rows are not spaced by multiples of 16 bytes
     are copied first (quantize_rows spaces them).  out: where the result goes, dense in its last dimension.  Not differentiable."""
-    if a.dim() < 2 or b.dim() < 2 or a.shape[-1] != b.shape[-1]:
-        raise hip.BflowHipError(f"matmul: rows of the same length, got {tuple(a.shape)} and {tuple(b.shape)}")
-    if tuple(scale_a.shape) != tuple(a.shape[:-1]) or tuple(scale_b.shape) != tuple(b.shape[:-1]):
-        raise hip.BflowHipError(f"matmul: a scale for each row, got {tuple(scale_a.shape)}, {tuple(scale_b.shape)} for {tuple(a.shape)}, {tuple(b.shape)}")
-    for t, name in ((scale_a, "scale_a"), (scale_b, "scale_b")):
-        hip._dev(t, torch.float32, name, contiguous=False)
-    if out_dtype not in hip.FLOAT_CODES:
+    ashape, bshape = a.shape, b.shape
+    if len(ashape) < 2 or len(bshape) < 2 or ashape[-1] != bshape[-1]:
+        raise hip.BflowHipError(f"matmul: rows of the same length, got {tuple(ashape)} and {tuple(bshape)}")
+    if scale_a.shape != ashape[:-1] or scale_b.shape != bshape[:-1]:
+        raise hip.BflowHipError(f"matmul: a scale for each row, got {tuple(scale_a.shape)}, {tuple(scale_b.shape)} for {tuple(ashape)}, {tuple(bshape)}")
+    for t, kind, name in ((a, torch.int8, "a"), (b, torch.int8, "b"), (scale_a, torch.float32, "scale_a"), (scale_b, torch.float32, "scale_b")):
+        hip._dev(t, kind, name, contiguous=False)
+    code = hip.FLOAT_CODES.get(out_dtype)
+    if code is None:
         raise hip.BflowHipError(f"matmul: out_dtype {out_dtype}, expected one of {sorted(str(d) for d in hip.FLOAT_CODES)}")
-    M, N, K = a.shape[-2], b.shape[-2], a.shape[-1]
-    try:
-        batch = torch.broadcast_shapes(a.shape[:-2], b.shape[:-2])
-    except RuntimeError:
-        raise hip.BflowHipError(f"matmul: leading dimensions {tuple(a.shape[:-2])} and {tuple(b.shape[:-2])} do not broadcast") from None
-    shape = tuple(batch) + (M, N)
+    M, N, K = ashape[-2], bshape[-2], ashape[-1]
+    batch: Tuple[int, ...] = ()
+    if len(ashape) > 2 or len(bshape) > 2:
+        batch = _broadcast(ashape[:-2], bshape[:-2])
+    shape, device = batch + (M, N), a.device
     if out is None:
-        hip._dev(a, torch.int8, "a", contiguous=False)
-        out = torch.empty(shape, dtype=out_dtype, device=a.device)
-    elif tuple(out.shape) != shape or out.dtype != out_dtype or not out.is_cuda or (N > 1 and out.stride(-1) != 1) or (M > 1 and out.stride(-2) < N):
+        out = torch.empty(shape, dtype=out_dtype, device=device)
+    elif tuple(out.shape) != shape or out.dtype != out_dtype or not out.is_cuda or (N > 1 and out.stride(-1) != 1) or (M > 1 and out.stride(-2) < N) \
+            or any(n > 1 and not s for n, s in zip(shape, out.stride())):
         raise hip.BflowHipError(f"matmul: out {tuple(out.shape)} {out.dtype}, strides {out.stride()}: expected {shape} {out_dtype}, rows dense")
-    if not (a.device == b.device == scale_a.device == scale_b.device == out.device):
+    if not (device == b.device == scale_a.device == scale_b.device == out.device):
         raise hip.BflowHipError("matmul: all tensors on one device")
-    if not out.numel():
+    if not (M and N and out.numel()):
         return out
     if not K:
         return out.zero_()
-    keep = (_operand(a, "a"), _operand(b, "b"), scale_a if scale_a.stride(-1) == 1 else scale_a.contiguous(), scale_b if scale_b.stride(-1) == 1 else scale_b.contiguous())
-    # (_operand again: folding three or more leading dimensions may have made a dense copy)
-    pa, pb, sa, sb = _operand(_two(keep[0], batch, 2), "a"), _operand(_two(keep[1], batch, 2), "b"), _two(keep[2], batch, 1), _two(keep[3], batch, 1)
-    to = _two(out, batch, 2)
-    if to.data_ptr() != out.data_ptr():
-        raise hip.BflowHipError(f"matmul: out with strides {out.stride()}: its leading dimensions have to fold into two")
-    d = hip.I8GemmDesc(a=pa.data_ptr(), b=pb.data_ptr(), scale_a=sa.data_ptr(), scale_b=sb.data_ptr(), out=to.data_ptr(), a_stride0=pa.stride(0), a_stride1=pa.stride(1),
-                       b_stride0=pb.stride(0), b_stride1=pb.stride(1), sa_stride0=sa.stride(0), sa_stride1=sa.stride(1), sb_stride0=sb.stride(0), sb_stride1=sb.stride(1),
-                       out_stride0=to.stride(0), out_stride1=to.stride(1), ldo=to.stride(2) if M > 1 else N, lda=pa.stride(2) if M > 1 else _padded(K),
-                       ldb=pb.stride(2) if N > 1 else _padded(K), M=M, N=N, K=K, batch0=to.shape[0], batch1=to.shape[1], dtype=hip.FLOAT_CODES[out_dtype], alpha=alpha)
-    for name in ("a", "b"):                                # a dimension of one element may carry any stride: it is never taken
-        for k, n in ((0, d.batch0), (1, d.batch1)):
-            if n == 1:
-                setattr(d, f"{name}_stride{k}", 0)
-    with torch.cuda.device(out.device):
-        hip._check(hip.lib().bflow_i8_gemm(ctypes.byref(d), hip._stream()), "bflow_i8_gemm")
+    with hip._on(device):
+        pa, pb = _operands((a, b), K, device)
+        sa, sb = scale_a if scale_a.stride(-1) == 1 else scale_a.contiguous(), scale_b if scale_b.stride(-1) == 1 else scale_b.contiguous()
+        strides, n0, n1 = (0,) * 10, 1, 1
+        if batch:
+            la, lb = len(ashape) - 2, len(bshape) - 2
+            two = _fold(batch, [_lead_strides(pa, la, batch), _lead_strides(pb, lb, batch), _lead_strides(sa, la, batch), _lead_strides(sb, lb, batch),
+                                _lead_strides(out, len(batch), batch)])
+            if two is None:                                # dense copies of what is spread over more than two dimensions
+                whole = torch.empty(shape, dtype=out_dtype, device=device)
+                spread = lambda t, tail: t.expand(batch + tuple(t.shape[-tail:])).contiguous()
+                matmul(spread(a, 2).flatten(0, -3), spread(scale_a, 1).flatten(0, -2), spread(b, 2).flatten(0, -3), spread(scale_b, 1).flatten(0, -2), out_dtype, alpha,
+                       out=whole.view((-1, M, N)))
+                return out.copy_(whole)
+            (n0, s0), (n1, s1) = two
+            strides = tuple(v for pair in zip(s0, s1) for v in pair)
+        ld = _padded(K)
+        d = hip.I8_GEMM.pack(pa.data_ptr(), pb.data_ptr(), sa.data_ptr(), sb.data_ptr(), out.data_ptr(), *strides, out.stride(-2) if M > 1 else N,
+                             pa.stride(-2) if M > 1 else ld, pb.stride(-2) if N > 1 else ld, M, N, K, n0, n1, code, alpha)
+        hip._check(hip.lib().bflow_i8_gemm(d, hip._stream()), "bflow_i8_gemm")
     return out

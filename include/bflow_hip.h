@@ -618,6 +618,8 @@ int bflow_muon_step(const bflow_ns_matrix_t* m, int count, int steps, float a, f
  *                            the two (elements; 0 repeats it).  a: M rows of K bytes, lda apart; b: N rows, ldb apart; addresses, lda, ldb and
  *                            the strides of a and b are multiples of 16 bytes, and a row is READ up to K rounded up to 16 (what stands behind
  *                            K does not count).  out: ldo elements from row to row; not a, b or a scale.
+ *   bflow_i8_pad_rows      : rows of K bytes at any address, ld apart -> rows ldd apart (a multiple of 16), zeros behind K: one or two operands (a
+ *                            HOST table) in a launch
  *   bflow_i8_quantize_rows : x (rows, K) of dtype, ld elements apart -> q (rows, ldq), zeros behind K, scale (rows)
  *   bflow_i8_quantize_pixels: feature maps -> one row of D channels for each pixel: q (B, rows, D), scale (B, rows).  x (B, D, h, w) fp32, or
  *                            (x NULL) the fp16-pair operand x_hi, x_lo (B, D/32, np, 32) of bflow_split_pack.  tiled 0: rows = h w, pixels in
@@ -636,6 +638,13 @@ typedef struct bflow_i8_gemm_desc {
     float alpha;
 } bflow_i8_gemm_t;
 int bflow_i8_gemm(const bflow_i8_gemm_t* desc, bflow_stream_t stream);
+typedef struct bflow_i8_pad {
+    const void* src;
+    void*       dst;
+    long long   ld, rows;
+    int         K, ldd;
+} bflow_i8_pad_t;
+int bflow_i8_pad_rows(const bflow_i8_pad_t* items, int count, bflow_stream_t stream);
 int bflow_i8_quantize_rows(const void* x, int dtype, long long ld, long long rows, int K, signed char* q, int ldq, float* scale,
                            bflow_stream_t stream);
 int bflow_i8_quantize_pixels(const float* x, const void* x_hi, const void* x_lo, int np, int B, int D, int h, int w, int tiled, signed char* q,

@@ -63,15 +63,20 @@ def test_refuses_what_it_cannot_take():
 
 def test_c_entries_refuse_bad_arguments():
     """The C entries' own checks, before any launch: no GPU is touched."""
-    import ctypes
     lib = hip.lib()
-    fine = dict(a=256, b=256, scale_a=256, scale_b=256, out=256, ldo=8, lda=16, ldb=16, M=4, N=8, K=16, batch0=1, batch1=1, dtype=0, alpha=1.0)
+    names = ("a b scale_a scale_b out a_stride0 a_stride1 b_stride0 b_stride1 sa_stride0 sa_stride1 sb_stride0 sb_stride1 out_stride0 out_stride1 ldo "
+             "lda ldb M N K batch0 batch1 dtype alpha").split()
+    fine = dict(dict.fromkeys(names, 0), a=256, b=256, scale_a=256, scale_b=256, out=256, ldo=8, lda=16, ldb=16, M=4, N=8, K=16, batch0=1, batch1=1, alpha=1.0)
     for kw in (dict(a=0), dict(b=0), dict(scale_a=0), dict(scale_b=0), dict(out=0), dict(M=0), dict(N=-1), dict(K=0), dict(batch0=0), dict(batch1=0), dict(dtype=3), dict(lda=15), dict(ldb=0),
                dict(lda=24), dict(a=264), dict(b=257), dict(a_stride0=8), dict(b_stride1=4), dict(ldo=7), dict(K=131072, lda=131072, ldb=131072), dict(lda=(1 << 22) + 16),
                dict(batch0=256, batch1=256)):
-        assert lib.bflow_i8_gemm(ctypes.byref(hip.I8GemmDesc(**{**fine, **kw})), None) < 0, kw
+        v = {**fine, **kw}
+        assert lib.bflow_i8_gemm(hip.I8_GEMM.pack(*(v[n] for n in names)), None) < 0, kw
         assert b"i8_gemm" in lib.bflow_last_error_string()
     assert lib.bflow_i8_gemm(None, None) < 0
+    for item in ((0, 256, 8, 4, 8, 16), (256, 0, 8, 4, 8, 16), (256, 260, 8, 4, 8, 16), (256, 256, 8, 0, 8, 16), (256, 256, 8, 4, 0, 16), (256, 256, 8, 4, 8, 8), (256, 256, 8, 4, 20, 16)):
+        assert lib.bflow_i8_pad_rows(hip.I8_PAD.pack(*item), 1, None) == -1, item
+    assert lib.bflow_i8_pad_rows(None, 1, None) == -1 and lib.bflow_i8_pad_rows(hip.I8_PAD.pack(256, 256, 8, 4, 8, 16), 3, None) == -1
     for kw in (dict(x=0), dict(q=0), dict(s=0), dict(rows=0), dict(K=0), dict(ldq=8), dict(ldq=24), dict(q=260), dict(dtype=5), dict(ld=-1)):
         v = {**dict(x=256, dtype=0, ld=16, rows=4, K=16, q=256, ldq=16, s=256), **kw}
         assert lib.bflow_i8_quantize_rows(v["x"], v["dtype"], v["ld"], v["rows"], v["K"], v["q"], v["ldq"], v["s"], None) == -1, kw
@@ -362,3 +367,10 @@ def test_model_forward_in_8_bits(name):
             graphed = m(voxel_grid=vox, iters=3, test_mode=True)[1].get_params().clone()
             assert torch.equal(eager, graphed)
     assert bool(torch.isfinite(eager).all())
+
+
+@gpu
+def test_out_that_repeats_itself_is_refused():
+    a, sa = (t.to(DEV) for t in rows(5, 32))
+    with pytest.raises(hip.BflowHipError, match="out"):
+        int8.matmul(a.expand(3, 5, 32), sa.expand(3, 5), a, sa, out=torch.zeros(5, 5, device=DEV).expand(3, 5, 5))

@@ -45,18 +45,17 @@ __device__ __forceinline__ i32x4 cut(i32x4 v, int k, int K) {
 template <int BM, int BN, int WM, int WN>
 struct ByteTile {
     static constexpr int M = BM, N = BN, ACROSS = BN / WN, WAVES = (BM / WM) * ACROSS, THREADS = 64 * WAVES, MT = WM / 32, NT = WN / 32;
-    static constexpr int STAGE = (BM + BN) * CHUNK, LDS = 2 * STAGE, PIECES = (BM + BN) / 8;
+    static constexpr int STAGE = (BM + BN) * CHUNK, LDS = 2 * STAGE;
     static_assert(BM / 8 % WAVES == 0 && BN / 8 % WAVES == 0, "whole pieces of either operand for every wave");
     // B is the instruction's first operand: lane l then holds row l % 32 of a 32 x 32 block, four neighbouring columns in neighbouring registers
     i32x16 acc[MT][NT];
 
-    __device__ __forceinline__ void issue(rsrc_t a, int lda, int va, rsrc_t b, int ldb, int vb, int chunk, char* stage, int wave) {
+    static constexpr int PA = BM / 8 / WAVES, PB = BN / 8 / WAVES;
+    __device__ __forceinline__ void issue(rsrc_t a, const int (&va)[PA], rsrc_t b, const int (&vb)[PB], int chunk, char* stage, int wave) {
 #pragma unroll
-        for (int i = 0; i < PIECES / WAVES; ++i) {
-            const int p = wave + i * WAVES;
-            if (i * WAVES < BM / 8) dma_piece(a, stage + p * 1024, va, p * 8 * lda + chunk * CHUNK);
-            else dma_piece(b, stage + p * 1024, vb, (p - BM / 8) * 8 * ldb + chunk * CHUNK);
-        }
+        for (int i = 0; i < PA; ++i) dma_piece(a, stage + (wave + i * WAVES) * 1024, va[i], chunk * CHUNK);
+#pragma unroll
+        for (int i = 0; i < PB; ++i) dma_piece(b, stage + BM * CHUNK + (wave + i * WAVES) * 1024, vb[i], chunk * CHUNK);
     }
     template <bool CUT> __device__ __forceinline__ void multiply(const char* as, const char* bs, int lane, int k, int K) {
 #pragma unroll
@@ -78,20 +77,25 @@ struct ByteTile {
     __device__ __forceinline__ void run(rsrc_t a, int lda, rsrc_t b, int ldb, int K, char* lds) {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const int wm = wave / ACROSS, wn = wave % ACROSS;
-        const int va = lane_offset(lane, lda), vb = lane_offset(lane, ldb), chunks = (K + CHUNK - 1) / CHUNK;
+        const int chunks = (K + CHUNK - 1) / CHUNK;
+        int va[PA], vb[PB];
+#pragma unroll
+        for (int i = 0; i < PA; ++i) va[i] = lane_offset(lane, lda) + (wave + i * WAVES) * 8 * lda;
+#pragma unroll
+        for (int i = 0; i < PB; ++i) vb[i] = lane_offset(lane, ldb) + (wave + i * WAVES) * 8 * ldb;
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
                 for (int k = 0; k < 16; ++k) acc[i][j][k] = 0;
-        issue(a, lda, va, b, ldb, vb, 0, lds, wave);
+        issue(a, va, b, vb, 0, lds, wave);
         wait_chunk();
         __builtin_amdgcn_s_barrier();
         const char *as = lds + wm * WM * CHUNK, *bs = lds + (BM + wn * WN) * CHUNK;
         const int whole = K / CHUNK;
         for (int c = 0; c < whole; ++c) {
-            if (c + 1 < chunks) issue(a, lda, va, b, ldb, vb, c + 1, lds + ((c + 1) & 1) * STAGE, wave);
+            if (c + 1 < chunks) issue(a, va, b, vb, c + 1, lds + ((c + 1) & 1) * STAGE, wave);
             multiply<false>(as + (c & 1) * STAGE, bs + (c & 1) * STAGE, lane, 0, 0);
             wait_chunk();
             __builtin_amdgcn_s_barrier();
@@ -228,7 +232,7 @@ __global__ __launch_bounds__(256, 3) void i8_stream_kernel(StreamArgs s) {
     auto issue = [&](int c, int slot) {
 #pragma unroll
         for (int i = 0; i < PW; ++i)
-            dma_piece(ra, ring + slot * SLOT + i * 32 * CHUNK + wave * 1024, va, (c * 32 + wave * 8) * g.lda + i * CHUNK);
+            dma_piece(ra, ring + slot * SLOT + i * 32 * CHUNK + wave * 1024, va + (c * 32 + wave * 8) * g.lda, i * CHUNK);
     };
     __syncthreads();                    // the scales
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");

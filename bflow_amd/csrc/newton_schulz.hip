@@ -27,13 +27,13 @@ using namespace bflow::nt;
 
 constexpr int MOST = BFLOW_NS_MAX_MATRICES;
 constexpr float SA = 4096.f, SB = 1024.f;
-constexpr int NORM_MIN = 16384, NORM_PARTS = 1024;   // elements of one partial sum of squares at least; partials of a matrix at most
+constexpr int NORM_MIN = 4096, NORM_PARTS = 1024;   // elements of one partial sum of squares at least; partials of a matrix at most
+constexpr int LARGE_BLOCKS = 512;                   // 64 x 64 blocks of the Gram matrices from which the large tiles are taken
 
 struct Work {          // one matrix inside the products
     long long off;     // bytes from the workspace
     int r, s;          // rows <= columns
     int tile0;         // first workgroup of this launch
-    int split;         // Gram: k chunks of one workgroup
 };
 struct Entry {         // one matrix where it enters
     const void* src;   // the matrix, or the gradient (step)
@@ -95,34 +95,48 @@ template <int DT> __device__ __forceinline__ void store1(void* p, long long i, f
 // position of (row, col) in an operand of `cols` padded columns, in halves; the lo half is 32 further
 __device__ __forceinline__ long long at(int row, int col, int cols) { return (long long)row * (2 * cols) + (col >> 5) * 64 + (col & 31); }
 __device__ __forceinline__ float pair_value(_Float16 h, _Float16 l) { return fmaf((float)l, SPLIT_LO_INV, (float)h); }
-__device__ __forceinline__ void put1(_Float16* m, long long i, float v) {
-    _Float16 h, l;
-    split1(v, h, l);
-    m[i] = h;
-    m[i + 32] = l;
-}
-__device__ __forceinline__ void put4(_Float16* m, long long i, const float v[4]) {
-    half4 h, l;
+__device__ __forceinline__ void put8(_Float16* m, long long i, const float v[8]) {
+    half8 h, l;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) { _Float16 a, b; split1(v[k], a, b); h[k] = a; l[k] = b; }
-    *reinterpret_cast<half4*>(m + i) = h;
-    *reinterpret_cast<half4*>(m + i + 32) = l;
+    for (int k = 0; k < 8; ++k) { _Float16 a, b; split1(v[k], a, b); h[k] = a; l[k] = b; }
+    *reinterpret_cast<half8*>(m + i) = h;
+    *reinterpret_cast<half8*>(m + i + 32) = l;
 }
-__device__ __forceinline__ void get4(const _Float16* m, long long i, float v[4]) {
-    const half4 h = *reinterpret_cast<const half4*>(m + i), l = *reinterpret_cast<const half4*>(m + i + 32);
+__device__ __forceinline__ void get8(const _Float16* m, long long i, float v[8]) {
+    const half8 h = *reinterpret_cast<const half8*>(m + i), l = *reinterpret_cast<const half8*>(m + i + 32);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = pair_value(h[k], l[k]);
+    for (int k = 0; k < 8; ++k) v[k] = pair_value(h[k], l[k]);
 }
 
+// A BM x BN tile of 32-bit numbers in LDS, to be written by columns of four rows, read by rows of eight and by columns of eight: the groups of four
+// columns are permuted by the row's eighth, so that none of the three meets itself in a bank more than twice.
+template <int BN> struct Turn {
+    __device__ static __forceinline__ int at(int row, int col) { return row * BN + ((((col >> 2) ^ ((row >> 3) & 7)) << 2) | (col & 3)); }
+    __device__ static __forceinline__ void row8(const float* t, int row, int col, float v[8]) {      // col a multiple of 8
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float4 x = *reinterpret_cast<const float4*>(t + at(row, col + 4 * h));
+            v[4 * h] = x.x; v[4 * h + 1] = x.y; v[4 * h + 2] = x.z; v[4 * h + 3] = x.w;
+        }
+    }
+    __device__ static __forceinline__ void put_row8(float* t, int row, int col, const float v[8]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) *reinterpret_cast<float4*>(t + at(row, col + 4 * h)) = make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
+    }
+    __device__ static __forceinline__ void col8(const float* t, int row, int col, float v[8]) {      // row a multiple of 8
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = t[at(row + k, col)];
+    }
+};
+
 // ------------------------------------------------------------------------------------------------------------------------------ entry
-// Element e of the source in its own order (row-major over the m x n of the user).
+// What enters the iteration at element (i, j) of the user's matrix; `update`: the step's momentum is brought up to date.
 template <int DT, bool STEP>
-__device__ __forceinline__ float entering(const Entry& m, int i, int j, float mu, bool nesterov, bool update) {
-    const float g = load1<DT>(m.src, (long long)i * m.ld + j);
+__device__ __forceinline__ float entering(const Entry& m, long long from, long long dense, float mu, bool nesterov, bool update) {
+    const float g = load1<DT>(m.src, from);
     if constexpr (!STEP) return g;
-    const long long e = (long long)i * (m.tall ? m.r : m.s) + j;          // momentum is dense
-    float v = m.momentum[e];
-    if (update) { v = fmaf(mu, v, g); m.momentum[e] = v; }
+    float v = m.momentum[dense];
+    if (update) { v = fmaf(mu, v, g); m.momentum[dense] = v; }
     return nesterov ? fmaf(mu, v, g) : v;
 }
 
@@ -132,13 +146,14 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(Entries t, char* ws, float
     __shared__ double part[4];
     const int k = find(t.m, t.count, blockIdx.x);
     const Entry m = t.m[k];
-    const int cols = m.tall ? m.r : m.s;
-    const long long n = (long long)m.r * m.s, first = (long long)(blockIdx.x - m.tile0) * m.per;
-    const long long last = first + m.per < n ? first + m.per : n;
+    const unsigned cols = m.tall ? m.r : m.s;
+    const bool dense = m.ld == cols;
+    const unsigned n = (unsigned)m.r * (unsigned)m.s, first = (blockIdx.x - m.tile0) * (unsigned)m.per, last = min(first + (unsigned)m.per, n);   // n <= 2^30
     double sum = 0;
-    for (long long e = first + threadIdx.x; e < last; e += 256) {
-        const int i = (int)(e / cols), j = (int)(e - (long long)i * cols);
-        const float u = entering<DT, STEP>(m, i, j, mu, nesterov, true);
+#pragma unroll 8
+    for (unsigned e = first + threadIdx.x; e < last; e += 256) {
+        const long long from = dense ? (long long)e : (long long)(e / cols) * m.ld + e % cols;
+        const float u = entering<DT, STEP>(m, from, e, mu, nesterov, true);
         sum += (double)u * (double)u;
     }
     sum = wave_sum(sum);
@@ -151,13 +166,21 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(Entries t, char* ws, float
 template <int DT, bool STEP>
 __global__ __launch_bounds__(256) void ns_pack_kernel(Entries t, char* ws, float mu, int nesterov, float eps) {
     __shared__ double part[4];
-    __shared__ float tile[64][65];
+    __shared__ __attribute__((aligned(16))) float tile[64 * 64];
     const int k = find(t.m, t.count, blockIdx.x);
     const Entry m = t.m[k];
     const int R = up64(m.r), S = up64(m.s), across = S / 64;
     const int w = blockIdx.x - m.tile0, r0 = (w / across) * 64, s0 = (w - (w / across) * across) * 64;
-    const long long n = (long long)m.r * m.s;
-    const int parts = (int)((n + m.per - 1) / m.per);
+    const int fast = threadIdx.x & 63, slow = threadIdx.x >> 6;
+    const int i0 = m.tall ? s0 : r0, j0 = m.tall ? r0 : s0;               // of the user's matrix
+    const int rows = m.tall ? m.s : m.r, cols = m.tall ? m.r : m.s;
+    float v[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const int i = i0 + slow + 4 * e, j = j0 + fast;
+        v[e] = i < rows && j < cols ? entering<DT, STEP>(m, (long long)i * m.ld + j, (long long)i * cols + j, mu, nesterov, false) : 0.f;
+    }
+    const int parts = (int)(((long long)m.r * m.s + m.per - 1) / m.per);
     double sum = 0;
     for (int i = threadIdx.x; i < parts; i += 256) sum += ((const double*)(ws + m.off))[i];
     sum = wave_sum(sum);
@@ -169,21 +192,20 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(Entries t, char* ws, float
     const int g = norm > 0. && norm < (double)eps ? (int)log2((norm + (double)eps) / norm) : 0;
     if (w == 0 && threadIdx.x == 0) *(int*)(ws + g_at(m.off)) = g;
     const double scale = ldexp(1.0, x_exponent(m.r, m.s) + g) / (norm + (double)eps);
-    const int fast = threadIdx.x & 63, slow = threadIdx.x >> 6;
-    const int i0 = m.tall ? s0 : r0, j0 = m.tall ? r0 : s0;               // of the user's matrix
-    const int rows = m.tall ? m.s : m.r, cols = m.tall ? m.r : m.s;
-    for (int i = slow; i < 64; i += 4) {
-        float v = 0.f;
-        if (i0 + i < rows && j0 + fast < cols) v = (float)((double)entering<DT, STEP>(m, i0 + i, j0 + fast, mu, nesterov, false) * scale);
-        tile[i][fast] = v;
-    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) tile[Turn<64>::at(slow + 4 * e, fast)] = (float)((double)v[e] * scale);
     __syncthreads();
+    // rows of the user's tile are rows of X, or (tall) of Xt
     _Float16* x = (_Float16*)(ws + x_at(m.off));
     _Float16* xt = (_Float16*)(ws + xt_at(m.off, m.r, m.s, 0));
-    for (int i = slow; i < 64; i += 4) {
-        const float across_v = tile[i][fast], down_v = tile[fast][i];     // (i, fast) and (fast, i) of the user's tile
-        put1(x, at(r0 + i, s0 + fast, S), m.tall ? down_v : across_v);
-        put1(xt, at(s0 + i, r0 + fast, R), m.tall ? across_v : down_v);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int it = threadIdx.x + i * 256, line = it >> 3, eight = (it & 7) * 8;
+        float a[8], d[8];
+        Turn<64>::row8(tile, line, eight, a);
+        Turn<64>::col8(tile, eight, line, d);
+        put8(x, at(r0 + line, s0 + eight, S), m.tall ? d : a);
+        put8(xt, at(s0 + line, r0 + eight, R), m.tall ? a : d);
     }
 }
 
@@ -191,40 +213,53 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(Entries t, char* ws, float
 __device__ __forceinline__ int g_of(const char* ws, long long off, int drop) { return max(*(const int*)(ws + g_at(off)) - drop, 0); }
 
 // --------------------------------------------------------------------------------------------------------------------------- products
-// BM x BN tile of A B^T on pairs; wave (wm, wn) keeps WM x WN of it.
-template <int BM, int BN, int WM, int WN>
-struct PairTile {
-    static constexpr int ACROSS = BN / WN, WAVES = (BM / WM) * ACROSS, THREADS = 64 * WAVES, MT = WM / 32, NT = WN / 32;
-    static constexpr int STAGE = (BM + BN) * CHUNK, LDS = 2 * STAGE, PIECES = (BM + BN) / 8;
-    static_assert(PIECES % WAVES == 0, "whole pieces for every wave");
-    f32x16 hh[MT][NT], xx[MT][NT];
+// BM x BN tile of A B^T on pairs.  A group of waves has WM x WN of it each; KG groups share the contraction (a stage holds a chunk for each) and
+// are summed in LDS, in a fixed order.
+template <int BM_, int BN_, int WM, int WN, int KG_, int STAGES>
+struct Product {
+    static constexpr int BM = BM_, BN = BN_, KG = KG_;
+    static constexpr int ACROSS = BN / WN, WAVES = (BM / WM) * ACROSS, THREADS = 64 * WAVES * KG, MT = WM / 32, NT = WN / 32;
+    static constexpr int CHUNK_BYTES = (BM + BN) * CHUNK, STAGE = KG * CHUNK_BYTES, TILE = BM * BN * 4;
+    static constexpr int LDS = STAGES * STAGE > KG * TILE ? STAGES * STAGE : KG * TILE;
+    static_assert(BM / 8 % WAVES == 0 && BN / 8 % WAVES == 0, "whole pieces of either operand for every wave");
+    typedef Turn<BN> T;
 
-    __device__ __forceinline__ void issue(rsrc_t a, int lda, int va, rsrc_t b, int ldb, int vb, int chunk, char* stage, int wave) {
-#pragma unroll
-        for (int i = 0; i < PIECES / WAVES; ++i) {
-            const int p = wave + i * WAVES;
-            if (p < BM / 8) dma_piece(a, stage + p * 1024, va, p * 8 * lda + chunk * CHUNK);
-            else dma_piece(b, stage + p * 1024, vb, (p - BM / 8) * 8 * ldb + chunk * CHUNK);
-        }
-    }
-
-    __device__ __forceinline__ void run(rsrc_t a, int lda, rsrc_t b, int ldb, int chunk0, int chunks, char* lds) {
-        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // Leaves KG tiles in LDS (Turn order); the workgroup is synchronised.  a, b: descriptors of the tile's rows, at least `chunks` chunks long.
+    __device__ static __forceinline__ void run(rsrc_t a, int lda, rsrc_t b, int ldb, int chunks, char* lds) {
+        const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = w / WAVES, wave = w % WAVES;
         const int wm = wave / ACROSS, wn = wave % ACROSS;
         const int va = lane_offset(lane, lda), vb = lane_offset(lane, ldb);
+        f32x16 hh[MT][NT], xx[MT][NT];
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
                 for (int k = 0; k < 16; ++k) { hh[i][j][k] = 0.f; xx[i][j][k] = 0.f; }
-        issue(a, lda, va, b, ldb, vb, chunk0, lds, wave);
-        wait_chunk();
-        __builtin_amdgcn_s_barrier();
-        for (int c = 0; c < chunks; ++c) {
-            if (c + 1 < chunks) issue(a, lda, va, b, ldb, vb, chunk0 + c + 1, lds + ((c + 1) & 1) * STAGE, wave);
-            const char* as = lds + (c & 1) * STAGE + wm * WM * CHUNK;
-            const char* bs = lds + (c & 1) * STAGE + (BM + wn * WN) * CHUNK;
+        const int rounds = (chunks + KG - 1) / KG;
+        auto issue = [&](int round) {
+            char* stage = lds + (round % STAGES) * STAGE + group * CHUNK_BYTES;
+            const int c = round * KG + group;
+            const bool there = c < chunks;                           // behind the last chunk: zeros
+            const int at = there ? c * CHUNK : 0;
+#pragma unroll
+            for (int i = 0; i < BM / 8 / WAVES; ++i)
+                dma_piece(a, stage + (wave + i * WAVES) * 1024, there ? va + (wave + i * WAVES) * 8 * lda : OUTSIDE, at);
+#pragma unroll
+            for (int i = 0; i < BN / 8 / WAVES; ++i)
+                dma_piece(b, stage + BM * CHUNK + (wave + i * WAVES) * 1024, there ? vb + (wave + i * WAVES) * 8 * ldb : OUTSIDE, at);
+        };
+        constexpr int PIECES = (BM + BN) / 8 / WAVES;
+#pragma unroll
+        for (int r = 0; r < STAGES - 1; ++r) issue(r);
+        for (int r = 0; r < rounds; ++r) {
+            // this wave's part of round r has landed (STAGES - 2 rounds may be in flight behind it), its reads of round r - 1 have returned; behind the
+            // barrier that holds for every wave, and the stage of round r - 1 may be filled again
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * PIECES) : "memory");
+            __builtin_amdgcn_s_barrier();
+            issue(r + STAGES - 1);
+            const char* as = lds + (r % STAGES) * STAGE + group * CHUNK_BYTES + wm * WM * CHUNK;
+            const char* bs = lds + (r % STAGES) * STAGE + group * CHUNK_BYTES + (BM + wn * WN) * CHUNK;
 #pragma unroll
             for (int sub = 0; sub < 2; ++sub) {
                 half8 ah[MT], al[MT], bh[NT], bl[NT];
@@ -247,212 +282,246 @@ struct PairTile {
                         xx[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], xx[i][j], 0, 0, 0);
                     }
             }
-            wait_chunk();
-            __builtin_amdgcn_s_barrier();
         }
-    }
-
-    // f(row, col, v[4]): 4 consecutive rows of column `col` of the tile; the 32 lanes of a half wave hold 32 neighbouring columns
-    template <class F> __device__ __forceinline__ void each4(F f) const {
-        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        const int wm = wave / ACROSS, wn = wave % ACROSS;
+        wait_chunk();                          // also the pieces behind the last round: the tiles take their place
+        __builtin_amdgcn_s_barrier();
+        float* t = (float*)(lds + group * TILE);
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    float v[4];
+                for (int k = 0; k < 16; ++k)
+                    t[T::at(wm * WM + i * 32 + (k >> 2) * 8 + (lane >> 5) * 4 + (k & 3), wn * WN + j * 32 + (lane & 31))] = fmaf(xx[i][j][k], SPLIT_LO_INV, hh[i][j][k]);
+        __syncthreads();
+    }
+
+    __device__ static __forceinline__ void sum8(const char* lds, int row, int col, float v[8]) {
+        T::row8((const float*)lds, row, col, v);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) v[k] = fmaf(xx[i][j][q * 4 + k], SPLIT_LO_INV, hh[i][j][q * 4 + k]);
-                    f(wm * WM + i * 32 + q * 8 + (lane >> 5) * 4, wn * WN + j * 32 + (lane & 31), v);
-                }
+        for (int g = 1; g < KG; ++g) {
+            float u[8];
+            T::row8((const float*)(lds + g * TILE), row, col, u);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] += u[k];
+        }
+    }
+    // f(row, col, v): eight columns of a row, every one of the tile once; what f leaves in v goes back to LDS
+    template <class F> __device__ static __forceinline__ void rows(char* lds, F f) {
+        for (int i = threadIdx.x; i < BM * BN / 8; i += THREADS) {
+            const int row = i / (BN / 8), col = i % (BN / 8) * 8;
+            float v[8];
+            sum8(lds, row, col, v);
+            f(row, col, v);
+            T::put_row8((float*)lds, row, col, v);
+        }
+    }
+    // f(row, col, v): eight rows of a column of what `rows` left
+    template <class F> __device__ static __forceinline__ void columns(const char* lds, F f) {
+        for (int i = threadIdx.x; i < BM * BN / 8; i += THREADS) {
+            const int col = i / (BM / 8), row = i % (BM / 8) * 8;
+            float v[8];
+            T::col8((const float*)lds, row, col, v);
+            f(row, col, v);
+        }
     }
 };
 
-typedef PairTile<64, 64, 32, 32> Small;
-
-// tile t of the lower triangle (diagonal included), row by row
-__device__ __forceinline__ void lower(int t, int& i, int& j) {
-    i = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
-    while ((i + 1) * (i + 2) / 2 <= t) ++i;
-    while (i * (i + 1) / 2 > t) --i;
-    j = t - i * (i + 1) / 2;
+// Tile t of those that touch the lower triangle, band of BM rows by band; `down` = bands.
+template <class P> __host__ __device__ inline int tiles_of_band(int i, int R) { const int n = ((i + 1) * P::BM + P::BN - 1) / P::BN, all = (R + P::BN - 1) / P::BN; return n < all ? n : all; }
+template <class P> __host__ inline int lower_tiles(int R) {
+    int n = 0;
+    for (int i = 0; i * P::BM < R; ++i) n += tiles_of_band<P>(i, R);
+    return n;
 }
+template <class P> __device__ __forceinline__ void lower(int t, int R, int& r0, int& c0) {
+    int i = 0;
+    for (int n; t >= (n = tiles_of_band<P>(i, R)); ++i) t -= n;
+    r0 = i * P::BM;
+    c0 = t * P::BN;
+}
+// What of a symmetric matrix a tile writes: 64 x 64 blocks on the diagonal once, those below it to both sides, those above not at all (another tile's
+// mirror; the two differ in the last bit, and one writer keeps the result the same from run to run).
+__device__ __forceinline__ bool mine(int row, int col) { return row >> 6 >= col >> 6; }
+__device__ __forceinline__ bool mirrored(int row, int col) { return row >> 6 > col >> 6; }
 
-// One stretch of the contraction of one 64 x 64 tile of X X^T, lower triangle; partials in the order of the registers.
-__global__ __launch_bounds__(256) void ns_gram_kernel(Works t, const char* ws, float* parts) {
-    __shared__ __attribute__((aligned(1024))) char lds[Small::LDS];
+// A = X X^T as pairs, both triangles.
+template <class P>
+__global__ __launch_bounds__(P::THREADS, 2) void ns_gram_kernel(Works t, char* ws) {
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int k = find(t.m, t.count, blockIdx.x);
     const Work m = t.m[k];
-    const int R = up64(m.r), S = up64(m.s), chunks = S / 32, splits = (chunks + m.split - 1) / m.split;
-    const int w = blockIdx.x - m.tile0, tile = w / splits, part = w - tile * splits;
-    int ti, tj;
-    lower(tile, ti, tj);
+    const int R = up64(m.r), S = up64(m.s), ld = S * 4;
+    int r0, c0;
+    lower<P>(blockIdx.x - m.tile0, R, r0, c0);
     const char* x = ws + x_at(m.off);
-    const int ld = S * 4;
-    Small p;
-    p.run(rows_rsrc(x + (long long)ti * 64 * ld, R - ti * 64, ld, ld), ld, rows_rsrc(x + (long long)tj * 64 * ld, R - tj * 64, ld, ld), ld, part * m.split,
-          min(m.split, chunks - part * m.split), lds);
-    float* out = parts + (long long)blockIdx.x * 4096 + threadIdx.x * 4;
-    int q = 0;
-    p.each4([&](int, int, const float v[4]) { *reinterpret_cast<float4*>(out + (q++) * 1024) = make_float4(v[0], v[1], v[2], v[3]); });
-}
-
-// A = the sum of the partials, as pairs, both triangles.  t.tile0: as in the Gram launch.
-__global__ __launch_bounds__(256) void ns_gram_sum_kernel(Works t, Works sums, char* ws, const float* parts) {
-    const int k = find(sums.m, sums.count, blockIdx.x);
-    const Work m = t.m[k];
-    const int R = up64(m.r), chunks = up64(m.s) / 32, splits = (chunks + m.split - 1) / m.split;
-    const int tile = blockIdx.x - sums.m[k].tile0;
-    int ti, tj;
-    lower(tile, ti, tj);
-    const float* in = parts + ((long long)m.tile0 + (long long)tile * splits) * 4096 + threadIdx.x * 4;
+    P::run(rows_rsrc(x + (long long)r0 * ld, min(P::BM, R - r0), ld, ld), ld, rows_rsrc(x + (long long)c0 * ld, min(P::BN, R - c0), ld, ld), ld, S / 32, lds);
     const float scale = ldexpf(SA, -2 * x_exponent(m.r, m.s));
     _Float16* a = (_Float16*)(ws + a_at(m.off, m.r, m.s));
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    P::rows(lds, [&](int row, int col, float v[8]) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int p = 0; p < splits; ++p) {
-            const float4 v = *reinterpret_cast<const float4*>(in + (long long)p * 4096 + q * 1024);
-            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
-        }
-        const float v[4] = {s.x * scale, s.y * scale, s.z * scale, s.w * scale};
-        const int row = ti * 64 + (wave >> 1) * 32 + q * 8 + (lane >> 5) * 4, col = tj * 64 + (wave & 1) * 32 + (lane & 31);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) put1(a, at(row + e, col, R), v[e]);
-        if (ti != tj) put4(a, at(col, row, R), v);
-    }
-}
-
-// B = b A + c A^2, lower tiles computed, both triangles written.
-__global__ __launch_bounds__(256) void ns_poly_kernel(Works t, char* ws, float b, float c, int drop) {
-    __shared__ __attribute__((aligned(1024))) char lds[Small::LDS];
-    const int k = find(t.m, t.count, blockIdx.x);
-    const Work m = t.m[k];
-    const int R = up64(m.r), ld = R * 4;
-    int ti, tj;
-    lower(blockIdx.x - m.tile0, ti, tj);
-    const char* a = ws + a_at(m.off, m.r, m.s);
-    Small p;
-    p.run(rows_rsrc(a + (long long)ti * 64 * ld, R - ti * 64, ld, ld), ld, rows_rsrc(a + (long long)tj * 64 * ld, R - tj * 64, ld, ld), ld, 0, R / 32, lds);
-    _Float16* out = (_Float16*)(ws + b_at(m.off, m.r, m.s));
-    const float fb = b * (SB / SA), fc = ldexpf(c * (SB / (SA * SA)), -2 * g_of(ws, m.off, drop));
-    p.each4([&](int r, int cc, const float d[4]) {
-        const int row = ti * 64 + r, col = tj * 64 + cc;
-        float av[4], v[4];
-        get4((const _Float16*)a, at(col, row, R), av);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) { v[e] = fmaf(fb, av[e], fc * d[e]); put1(out, at(row + e, col, R), v[e]); }
-        if (ti != tj) put4(out, at(col, row, R), v);
+        for (int e = 0; e < 8; ++e) v[e] *= scale;
+        if (r0 + row < R && c0 + col < R && mine(r0 + row, c0 + col)) put8(a, at(r0 + row, c0 + col, R), v);
+    });
+    __syncthreads();
+    P::columns(lds, [&](int row, int col, const float v[8]) {
+        if (r0 + row < R && c0 + col < R && mirrored(r0 + row, c0 + col)) put8(a, at(c0 + col, r0 + row, R), v);
     });
 }
 
-// X <- a X + B X.  Both orders of the new X.
-__global__ __launch_bounds__(256) void ns_apply_kernel(Works t, char* ws, int from, float a, int drop, int drop_next) {
-    __shared__ __attribute__((aligned(1024))) char lds[Small::LDS];
+// B = b A + c A^2, both triangles.
+template <class P>
+__global__ __launch_bounds__(P::THREADS, 2) void ns_poly_kernel(Works t, char* ws, float b, float c, int drop) {
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int k = find(t.m, t.count, blockIdx.x);
     const Work m = t.m[k];
-    const int R = up64(m.r), S = up64(m.s), ld = R * 4, down = R / 64;
-    const int w = blockIdx.x - m.tile0, r0 = (w % down) * 64, s0 = (w / down) * 64;
+    const int R = up64(m.r), ld = R * 4;
+    int r0, c0;
+    lower<P>(blockIdx.x - m.tile0, R, r0, c0);
+    const char* a = ws + a_at(m.off, m.r, m.s);
+    P::run(rows_rsrc(a + (long long)r0 * ld, min(P::BM, R - r0), ld, ld), ld, rows_rsrc(a + (long long)c0 * ld, min(P::BN, R - c0), ld, ld), ld, R / 32, lds);
+    _Float16* out = (_Float16*)(ws + b_at(m.off, m.r, m.s));
+    const float fb = b * (SB / SA), fc = ldexpf(c * (SB / (SA * SA)), -2 * g_of(ws, m.off, drop));
+    P::rows(lds, [&](int row, int col, float v[8]) {
+        if (r0 + row >= R || c0 + col >= R || !mine(r0 + row, c0 + col)) return;
+        float av[8];
+        get8((const _Float16*)a, at(r0 + row, c0 + col, R), av);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = fmaf(fb, av[e], fc * v[e]);
+        put8(out, at(r0 + row, c0 + col, R), v);
+    });
+    __syncthreads();
+    P::columns(lds, [&](int row, int col, const float v[8]) {
+        if (r0 + row < R && c0 + col < R && mirrored(r0 + row, c0 + col)) put8(out, at(c0 + col, r0 + row, R), v);
+    });
+}
+
+// X <- a X + B X, by rows (in place: a tile reads and writes its own part alone) and by columns (from one Xt to the other).
+template <class P>
+__global__ __launch_bounds__(P::THREADS, 2) void ns_apply_kernel(Works t, char* ws, int from, float a, int drop, int drop_next) {
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    const int k = find(t.m, t.count, blockIdx.x);
+    const Work m = t.m[k];
+    const int R = up64(m.r), S = up64(m.s), ld = R * 4, down = (R + P::BM - 1) / P::BM;
+    const int w = blockIdx.x - m.tile0, r0 = (w % down) * P::BM, s0 = (w / down) * P::BN;
     const char* b = ws + b_at(m.off, m.r, m.s);
     const char* xt = ws + xt_at(m.off, m.r, m.s, from);
-    Small p;
-    p.run(rows_rsrc(b + (long long)r0 * ld, R - r0, ld, ld), ld, rows_rsrc(xt + (long long)s0 * ld, S - s0, ld, ld), ld, 0, R / 32, lds);
+    P::run(rows_rsrc(b + (long long)r0 * ld, min(P::BM, R - r0), ld, ld), ld, rows_rsrc(xt + (long long)s0 * ld, min(P::BN, S - s0), ld, ld), ld, R / 32, lds);
     _Float16* x = (_Float16*)(ws + x_at(m.off));
     _Float16* to = (_Float16*)(ws + xt_at(m.off, m.r, m.s, 1 - from));
     const int g = g_of(ws, m.off, drop), down_g = g_of(ws, m.off, drop_next) - g;
     const float fx = ldexpf(a, down_g), fd = ldexpf(1.f / SB, down_g - 2 * g);
-    p.each4([&](int r, int c, const float d[4]) {
-        const int row = r0 + r, col = s0 + c;
-        float xv[4], v[4];
-        get4((const _Float16*)xt, at(col, row, R), xv);
+    P::rows(lds, [&](int row, int col, float v[8]) {
+        if (r0 + row >= R || s0 + col >= S) return;
+        float xv[8];
+        get8(x, at(r0 + row, s0 + col, S), xv);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { v[e] = fmaf(fx, xv[e], d[e] * fd); put1(x, at(row + e, col, S), v[e]); }
-        put4(to, at(col, row, R), v);
+        for (int e = 0; e < 8; ++e) v[e] = fmaf(fx, xv[e], v[e] * fd);
+        put8(x, at(r0 + row, s0 + col, S), v);
+    });
+    __syncthreads();
+    P::columns(lds, [&](int row, int col, const float v[8]) {
+        if (r0 + row < R && s0 + col < S) put8(to, at(s0 + col, r0 + row, R), v);
     });
 }
 
 // The last X <- a X + B X: to the user's matrix, or into the weights.
-template <int DT, bool STEP>
-__global__ __launch_bounds__(256) void ns_leave_kernel(Exits t, const char* ws, int from, float a, int drop, float lr, const float* lr_device, float decay) {
-    __shared__ __attribute__((aligned(1024))) char lds[Small::LDS];
+template <class P, int DT, bool STEP>
+__global__ __launch_bounds__(P::THREADS, 2) void ns_leave_kernel(Exits t, const char* ws, int from, float a, int drop, float lr, const float* lr_device, float decay) {
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int k = find(t.m, t.count, blockIdx.x);
     const Exit m = t.m[k];
-    const int R = up64(m.r), S = up64(m.s), ld = R * 4, down = R / 64;
-    const int w = blockIdx.x - m.tile0, r0 = (w % down) * 64, s0 = (w / down) * 64;
+    const int R = up64(m.r), S = up64(m.s), ld = R * 4, down = (R + P::BM - 1) / P::BM;
+    const int w = blockIdx.x - m.tile0, r0 = (w % down) * P::BM, s0 = (w / down) * P::BN;
     const char* b = ws + b_at(m.off, m.r, m.s);
     const char* xt = ws + xt_at(m.off, m.r, m.s, from);
-    Small p;
-    p.run(rows_rsrc(b + (long long)r0 * ld, R - r0, ld, ld), ld, rows_rsrc(xt + (long long)s0 * ld, S - s0, ld, ld), ld, 0, R / 32, lds);
+    P::run(rows_rsrc(b + (long long)r0 * ld, min(P::BM, R - r0), ld, ld), ld, rows_rsrc(xt + (long long)s0 * ld, min(P::BN, S - s0), ld, ld), ld, R / 32, lds);
+    const _Float16* x = (const _Float16*)(ws + x_at(m.off));
     const int g = g_of(ws, m.off, drop), unit = -x_exponent(m.r, m.s) - g;
     const float fd = ldexpf(1.f / SB, -2 * g);
     if constexpr (STEP) lr = lr_device ? *lr_device : lr;
     const float keep = 1.f - lr * decay, rate = lr * m.size;
-    p.each4([&](int r, int c, const float d[4]) {
-        const int row = r0 + r, col = s0 + c;
-        float xv[4];
-        get4((const _Float16*)xt, at(col, row, R), xv);
+    auto store = [&](long long i, float v) {
+        if constexpr (STEP) ((float*)m.dst)[i] = fmaf(-rate, v, ((const float*)m.dst)[i] * keep);
+        else store1<DT>(m.dst, i, v);
+    };
+    P::rows(lds, [&](int row, int col, float v[8]) {
+        if (r0 + row >= R || s0 + col >= S) return;
+        float xv[8];
+        get8(x, at(r0 + row, s0 + col, S), xv);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (row + e >= m.r || col >= m.s) continue;
-            const float v = ldexpf(fmaf(a, xv[e], d[e] * fd), unit);
-            const long long i = m.tall ? (long long)col * m.ld + row + e : (long long)(row + e) * m.ld + col;
-            if constexpr (STEP) ((float*)m.dst)[i] = fmaf(-rate, v, ((const float*)m.dst)[i] * keep);
-            else store1<DT>(m.dst, i, v);
-        }
+        for (int e = 0; e < 8; ++e) v[e] = ldexpf(fmaf(a, xv[e], v[e] * fd), unit);
     });
+    __syncthreads();
+    // element by element along the user's rows: any address, whole lines
+    if (!m.tall)
+        for (int i = threadIdx.x; i < P::BM * P::BN; i += P::THREADS) {
+            const int row = i / P::BN, col = i % P::BN;
+            if (r0 + row < m.r && s0 + col < m.s) store((long long)(r0 + row) * m.ld + s0 + col, ((const float*)lds)[P::T::at(row, col)]);
+        }
+    else
+        for (int i = threadIdx.x; i < P::BM * P::BN; i += P::THREADS) {
+            const int row = i % P::BM, col = i / P::BM;
+            if (r0 + row < m.r && s0 + col < m.s) store((long long)(s0 + col) * m.ld + r0 + row, ((const float*)lds)[P::T::at(row, col)]);
+        }
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------ host
-constexpr int GRAM_WGS = 1024, GRAM_MIN = 8;   // workgroups of the Gram launch aimed at; k chunks of one of them at least
-
-struct Plan {
-    Works gram, sum, poly, apply;
-    Entries norm, pack;
-    Exits leave;
-    long long tiles_gram, tiles_sum, tiles_poly, tiles_apply, tiles_norm, tiles_pack, parts_at, bytes;
+// Two sets of tiles.  Small: the filters of a network; few tiles, so four groups of waves share a contraction.  Large: many.
+struct SmallSet {
+    typedef Product<64, 64, 32, 32, 4, 2> Square;      // A and B
+    typedef Product<64, 128, 32, 64, 1, 3> Panel;      // X
+};
+struct LargeSet {
+    typedef Product<128, 128, 64, 64, 2, 2> Square;
+    typedef Product<128, 128, 64, 64, 1, 2> Panel;
 };
 
-// The launches of one group of matrices; returns false where a count passes what a grid or an int holds.
-bool lay_out(const bflow_ns_matrix_t* m, int count, Plan& p) {
-    long long off = 0, work = 0;
-    p.tiles_gram = p.tiles_sum = p.tiles_poly = p.tiles_apply = p.tiles_norm = p.tiles_pack = 0;
-    for (int i = 0; i < count; ++i) {
-        const int r = m[i].rows < m[i].cols ? m[i].rows : m[i].cols, s = m[i].rows < m[i].cols ? m[i].cols : m[i].rows;
-        const long long T = up64(r) / 64;
-        work += T * (T + 1) / 2 * (up64(s) / 32);
+struct Plan {
+    Works square, panel;
+    Entries norm, pack;
+    Exits leave;
+    long long tiles_square, tiles_panel, tiles_norm, tiles_pack, bytes;
+    bool large;
+};
+
+template <class Set> void lay_out_products(Plan& p) {
+    for (int i = 0; i < p.square.count; ++i) {
+        const int r = p.square.m[i].r, s = p.square.m[i].s, R = up64(r), S = up64(s);
+        p.square.m[i].tile0 = (int)p.tiles_square;
+        p.panel.m[i] = p.square.m[i];
+        p.panel.m[i].tile0 = p.leave.m[i].tile0 = (int)p.tiles_panel;
+        p.tiles_square += lower_tiles<typename Set::Square>(R);
+        p.tiles_panel += (long long)((R + Set::Panel::BM - 1) / Set::Panel::BM) * ((S + Set::Panel::BN - 1) / Set::Panel::BN);
     }
+}
+
+// The launches of one group of matrices; returns false where a count passes what a grid holds.
+bool lay_out(const bflow_ns_matrix_t* m, int count, Plan& p) {
+    long long off = 0, blocks = 0;
+    p.tiles_square = p.tiles_panel = p.tiles_norm = p.tiles_pack = 0;
+    p.square.count = p.panel.count = p.norm.count = p.pack.count = p.leave.count = count;
     for (int i = 0; i < count; ++i) {
         const int tall = m[i].rows > m[i].cols;
         const int r = tall ? m[i].cols : m[i].rows, s = tall ? m[i].rows : m[i].cols;
-        const long long T = up64(r) / 64, U = up64(s) / 64, n = (long long)r * s, chunks = 2 * U;
-        long long split = (work + GRAM_WGS - 1) / GRAM_WGS;
-        split = split < GRAM_MIN ? GRAM_MIN : split;
-        split = split > chunks ? chunks : split;
+        const long long T = up64(r) / 64, U = up64(s) / 64, n = (long long)r * s;
         long long per = (n + NORM_PARTS - 1) / NORM_PARTS;
         per = per < NORM_MIN ? NORM_MIN : per;
-        p.gram.m[i] = {off, r, s, (int)p.tiles_gram, (int)split};
-        p.sum.m[i] = {off, r, s, (int)p.tiles_sum, 0};
-        p.poly.m[i] = {off, r, s, (int)p.tiles_poly, 0};
-        p.apply.m[i] = {off, r, s, (int)p.tiles_apply, 0};
+        p.square.m[i] = {off, r, s, 0};
         p.norm.m[i] = {m[i].src, m[i].momentum, m[i].src_ld, off, r, s, (int)p.tiles_norm, (int)per, tall};
         p.pack.m[i] = p.norm.m[i];
         p.pack.m[i].tile0 = (int)p.tiles_pack;
-        p.leave.m[i] = {m[i].dst, m[i].dst_ld, off, r, s, (int)p.tiles_apply, tall, 0.2f * sqrtf((float)s)};
-        p.tiles_gram += T * (T + 1) / 2 * ((chunks + split - 1) / split);
-        p.tiles_sum += T * (T + 1) / 2;
-        p.tiles_poly += T * (T + 1) / 2;
-        p.tiles_apply += T * U;
+        p.leave.m[i] = {m[i].dst, m[i].dst_ld, off, r, s, 0, tall, 0.2f * sqrtf((float)s)};
+        blocks += T * (T + 1) / 2;
         p.tiles_norm += (n + per - 1) / per;
         p.tiles_pack += T * U;
         off = (end_at(off, r, s) + 255) & ~255LL;
     }
-    p.gram.count = p.sum.count = p.poly.count = p.apply.count = p.norm.count = p.pack.count = p.leave.count = count;
-    p.parts_at = off;
-    p.bytes = off + p.tiles_gram * 4096 * 4;
-    return p.tiles_gram < (1LL << 30) && p.tiles_apply < (1LL << 30);
+    p.large = blocks >= LARGE_BLOCKS;
+    if (p.large) lay_out_products<LargeSet>(p);
+    else lay_out_products<SmallSet>(p);
+    p.bytes = off;
+    return p.tiles_pack < (1LL << 30);
 }
 
 const char* bad(const bflow_ns_matrix_t* m, int count) {
@@ -482,22 +551,40 @@ double reach(int steps, double a, double b, double c, double* gain) {
     return most;
 }
 
-template <int DT, bool STEP>
-int launch_all(const Plan& p, int steps, float a, float b, float c, float eps, double gain, char* ws, float mu, int nesterov, float lr, const float* lr_device, float decay,
-               hipStream_t st) {
-    float* parts = (float*)(ws + p.parts_at);
-    hipLaunchKernelGGL((ns_norm_kernel<DT, STEP>), dim3(p.tiles_norm), dim3(256), 0, st, p.norm, ws, mu, nesterov);
-    hipLaunchKernelGGL((ns_pack_kernel<DT, STEP>), dim3(p.tiles_pack), dim3(256), 0, st, p.pack, ws, mu, nesterov, eps);
+template <class K> int allow_lds(K kernel, int bytes) {
+    if (bytes <= 65536) return 0;
+    const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    BFLOW_REQUIRE(e == hipSuccess, (int)e, "newton_schulz: %s", hipGetErrorString(e));
+    return 0;
+}
+
+template <class Set, int DT, bool STEP>
+int launch_products(const Plan& p, int steps, float a, float b, float c, double gain, char* ws, float lr, const float* lr_device, float decay, hipStream_t st) {
+    typedef typename Set::Square Q;
+    typedef typename Set::Panel P;
+    const auto gram = ns_gram_kernel<Q>;
+    const auto poly = ns_poly_kernel<Q>;
+    const auto apply = ns_apply_kernel<P>;
+    const auto leave = ns_leave_kernel<P, DT, STEP>;
+    for (const int rc : {allow_lds(gram, Q::LDS), allow_lds(poly, Q::LDS), allow_lds(apply, P::LDS), allow_lds(leave, P::LDS)})
+        if (rc) return rc;
     const double bits = log2(gain);
     for (int k = 0; k < steps; ++k) {
         const int drop = (int)std::ceil(k * bits), next = (int)std::ceil((k + 1) * bits);
-        hipLaunchKernelGGL(ns_gram_kernel, dim3(p.tiles_gram), dim3(256), 0, st, p.gram, ws, parts);
-        hipLaunchKernelGGL(ns_gram_sum_kernel, dim3(p.tiles_sum), dim3(256), 0, st, p.gram, p.sum, ws, parts);
-        hipLaunchKernelGGL(ns_poly_kernel, dim3(p.tiles_poly), dim3(256), 0, st, p.poly, ws, b, c, drop);
-        if (k + 1 < steps) hipLaunchKernelGGL(ns_apply_kernel, dim3(p.tiles_apply), dim3(256), 0, st, p.apply, ws, k & 1, a, drop, next);
-        else hipLaunchKernelGGL((ns_leave_kernel<DT, STEP>), dim3(p.tiles_apply), dim3(256), 0, st, p.leave, ws, k & 1, a, drop, lr, lr_device, decay);
+        hipLaunchKernelGGL(gram, dim3(p.tiles_square), dim3(Q::THREADS), Q::LDS, st, p.square, ws);
+        hipLaunchKernelGGL(poly, dim3(p.tiles_square), dim3(Q::THREADS), Q::LDS, st, p.square, ws, b, c, drop);
+        if (k + 1 < steps) hipLaunchKernelGGL(apply, dim3(p.tiles_panel), dim3(P::THREADS), P::LDS, st, p.panel, ws, k & 1, a, drop, next);
+        else hipLaunchKernelGGL(leave, dim3(p.tiles_panel), dim3(P::THREADS), P::LDS, st, p.leave, ws, k & 1, a, drop, lr, lr_device, decay);
     }
     return launch_status("newton_schulz");
+}
+
+template <int DT, bool STEP>
+int launch_all(const Plan& p, int steps, float a, float b, float c, float eps, double gain, char* ws, float mu, int nesterov, float lr, const float* lr_device, float decay,
+               hipStream_t st) {
+    hipLaunchKernelGGL((ns_norm_kernel<DT, STEP>), dim3(p.tiles_norm), dim3(256), 0, st, p.norm, ws, mu, nesterov);
+    hipLaunchKernelGGL((ns_pack_kernel<DT, STEP>), dim3(p.tiles_pack), dim3(256), 0, st, p.pack, ws, mu, nesterov, eps);
+    return (p.large ? launch_products<LargeSet, DT, STEP> : launch_products<SmallSet, DT, STEP>)(p, steps, a, b, c, gain, ws, lr, lr_device, decay, st);
 }
 
 int check(const bflow_ns_matrix_t* m, int count, int steps, float a, float b, float c, float eps, const void* ws, long long ws_bytes, bool step, double* gain) {

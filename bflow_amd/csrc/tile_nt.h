@@ -33,7 +33,10 @@ __device__ __forceinline__ rsrc_t rows_rsrc(const void* base, int rows, long lon
     return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)(n > 0x7fffffffLL ? 0x7fffffffLL : n), 0x00020000);
 }
 
-// One wave's share of `pieces` 8-row pieces of a stage.  voff: lane_offset(); the rows start at the descriptor's base.
+// A wave's 8-row piece of a stage: lane_offset() + the piece's first row * ld in `voff`, the bytes along the row in `soff`.  The bounds check takes
+// soff off the descriptor's size before it compares voff, so what may lie outside (rows behind the last one, OUTSIDE for a whole piece) goes into
+// voff, and soff stays below the length of a row.
+constexpr int OUTSIDE = (int)0x80000000u;
 __device__ __forceinline__ int lane_offset(int lane, int ld) { return (lane >> 3) * ld + (((lane & 7) ^ (lane >> 3)) << 4); }
 __device__ __forceinline__ void dma_piece(rsrc_t r, char* lds_piece, int voff, int soff) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr_t)lds_piece, 16, voff, soff, 0, 0);

@@ -17,6 +17,7 @@
 // Layouts (workspace): an operand row is a row of 128-byte chunks of 32 columns, [32 hi | 32 lo] (tile_nt.h), rows and columns padded to 64
 // with zeros.  X is held twice, by rows (X, for the Gram product) and by columns (Xt, the right operand of B X): both products then read
 // both operands along the contraction.
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 #include "common.h"
@@ -182,9 +183,9 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(Entries t, char* ws, float
     if (threadIdx.x == 0) ((double*)(ws + m.off))[blockIdx.x - m.tile0] = part[0] + part[1] + part[2] + part[3];
 }
 
-// X and Xt of a 64 x 64 tile, scaled to sx / (|X| + eps), zeros in the padding.
+// X and (`both`) Xt of a 64 x 64 tile, scaled to sx / (|X| + eps), zeros in the padding.
 template <int DT, bool STEP>
-__global__ __launch_bounds__(256) void ns_pack_kernel(Entries t, char* ws, float mu, int nesterov, float eps) {
+__global__ __launch_bounds__(256) void ns_pack_kernel(Entries t, char* ws, float mu, int nesterov, float eps, int both) {
     __shared__ double part[4];
     __shared__ __attribute__((aligned(16))) float tile[64 * 64];
     const int k = find(t.m, t.count, blockIdx.x);
@@ -228,9 +229,16 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(Entries t, char* ws, float
         half8 ah, al, dh, dl;
         Turn<64>::pairs8(tile, line, eight, ah, al);
         Turn<64>::col8(tile, eight, line, dh, dl);
-        put8(m.tall ? xt : x, m.tall ? at(s0 + line, r0 + eight, R) : at(r0 + line, s0 + eight, S), ah, al);
-        put8(m.tall ? x : xt, m.tall ? at(r0 + line, s0 + eight, S) : at(s0 + line, r0 + eight, R), dh, dl);
+        if (both || !m.tall) put8(m.tall ? xt : x, m.tall ? at(s0 + line, r0 + eight, R) : at(r0 + line, s0 + eight, S), ah, al);
+        if (both || m.tall) put8(m.tall ? x : xt, m.tall ? at(r0 + line, s0 + eight, S) : at(s0 + line, r0 + eight, R), dh, dl);
     }
+}
+
+// Tile t of a lower triangle, diagonal included, row by row: (0, 0), (1, 0), (1, 1), (2, 0), ...
+__device__ __forceinline__ void lower32(int t, int& i, int& j) {
+    i = 0;
+    while ((i + 1) * (i + 2) / 2 <= t) ++i;
+    j = t - i * (i + 1) / 2;
 }
 
 // g of a step: what the start had, less `drop` for the growth since
@@ -555,6 +563,405 @@ __global__ __launch_bounds__(P::THREADS, 2) void ns_leave_kernel(Exits t, const 
     }
 }
 
+// ----------------------------------------------------------------------------------------------------------------------------- panels
+// Matrices of at most 256 rows (the filters of a network): what bounds the products above is memory, X by rows and by columns to and fro.  Here a
+// workgroup takes PANELS of X, all R rows by 64 columns, held by rows alone.  Once a panel is in LDS it is multiplied by B, updated in place,
+// written back, and multiplied by its own transpose, all from LDS; X crosses the chip once each way a step.  The Gram parts of a matrix' workgroups
+// are added, in order, where B is made of them.  A step is two launches instead of three.
+//   apply   D[s][r'] = sum_r X[r][s] B[r'][r]: the left operand needs eight rows of one column in a lane, which the transposing LDS read gives;
+//           four neighbouring columns of a row leave a lane together, so a panel is updated by 8-byte reads and writes.
+//   Gram    lower 32 x 32 tiles dealt over the waves; a panel's product is added to sums that stay in registers (16 a tile) from panel to panel.
+// B stays in LDS up to 128 rows and is streamed by chunks of 32 columns above (three or four in flight).
+constexpr int PANEL_ROWS = 256, PANEL_THREADS = 512;
+
+struct PanelWork {     // one matrix
+    long long off;
+    int r, s;
+    int wg0, square0, sum0;  // first workgroup of the panel launches, of those that make B, of those that add the parts
+    int per;           // panels of a workgroup
+};
+struct PanelWorks { PanelWork m[MOST]; int count; };
+struct PanelExit {     // where a matrix leaves
+    void* dst;
+    long long ld;
+    float size;
+    int tall;
+};
+struct PanelExits { PanelExit m[MOST]; };
+static_assert(sizeof(PanelWorks) + sizeof(PanelExits) <= 4000, "the tables are kernel arguments");
+// regions: norm partials, g, X, B, A, the Gram parts (32 bits, R x R each)
+__host__ __device__ inline long long pb_at(long long off, int r, int s) { return x_at(off) + mat_bytes(r, s); }
+__host__ __device__ inline long long pa_at(long long off, int r, int s) { return pb_at(off, r, s) + mat_bytes(r, r); }
+__host__ __device__ inline long long parts_at(long long off, int r, int s) { return pa_at(off, r, s) + mat_bytes(r, r); }
+__host__ __device__ inline int panels_of(int s) { return up64(s) / 64; }
+
+template <class F> __device__ __forceinline__ int find_by(int count, int wg, F first) {
+    const int lane = threadIdx.x & 63;
+    const bool before = lane < count && first(lane < count ? lane : 0) <= wg;
+    return __builtin_amdgcn_readfirstlane(__builtin_popcountll(__ballot(before)) - 1);
+}
+
+typedef short short4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) short4_t* tr_t;
+__device__ __forceinline__ half4 tr_read(const char* p) {
+    return __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_t)p));
+}
+__device__ __forceinline__ half8 join(half4 a, half4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+
+enum { FIRST = 0, MIDDLE = 1, LAST = 2 };     // Gram alone; update and Gram; update alone, to the user
+
+template <int RT> struct PanelSize {
+    static constexpr int R = 64 * RT, IMAGE = 2 * R * CHUNK, STAGE = R * CHUNK;
+    static constexpr bool RESIDENT = RT <= 2;
+    static constexpr int STAGES = RESIDENT ? 2 * RT : RT == 3 ? 4 : 3;
+    static constexpr int IMAGES = RESIDENT ? 2 : 1;        // room for the next panel beside the current one
+    static constexpr int LDS = IMAGES * IMAGE + STAGES * STAGE;
+};
+
+struct Numbers {       // of a step
+    int drop, drop_next;
+    float a, lr;
+    const float* lr_device;
+    float decay;
+};
+
+template <int RT, int MODE, int DT, bool STEP>
+__device__ __forceinline__ void panel_body(const PanelWork& m, const PanelExit& o, char* ws, int slice, const Numbers& nu, char* lds) {
+    typedef PanelSize<RT> P;
+    constexpr int R = P::R, STAGES = P::STAGES, AT = (RT + 1) / 2, GRAM = RT * (2 * RT + 1), GT = (GRAM + 7) / 8;
+    const int lane = threadIdx.x & 63, l31 = lane & 31, h = lane >> 5, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int S = up64(m.s), ldx = S * 4, ldb = R * 4, panels = S / 64;
+    char* x = ws + x_at(m.off);
+    char* stages = lds + P::IMAGES * P::IMAGE;
+    const rsrc_t rx = rows_rsrc(x, R, ldx, ldx), rb = rows_rsrc(ws + pb_at(m.off, m.r, m.s), R, ldb, ldb);
+    const int vx = lane_offset(lane, ldx), vb = lane_offset(lane, ldb);
+    const int g = MODE == FIRST ? 0 : g_of(ws, m.off, nu.drop), down_g = MODE == MIDDLE ? g_of(ws, m.off, nu.drop_next) - g : 0;
+    const float fx = ldexpf(nu.a, down_g), fd = ldexpf(1.f / SB, down_g - 2 * g);
+    const int unit = MODE == LAST ? -x_exponent(m.r, m.s) - g : 0;
+
+    auto load_panel = [&](int p, char* image) {   // 2 chunks x R rows, 8 rows a piece
+#pragma unroll
+        for (int i = 0; i < 2 * RT; ++i) {
+            const int q = w + i * 8, j = q / (8 * RT), piece = q - j * 8 * RT;
+            dma_piece(rx, image + j * R * CHUNK + piece * 1024, vx + piece * 8 * ldx, (p * 2 + j) * CHUNK);
+        }
+    };
+    auto load_b = [&](int c, int stage) {         // chunk c of B, all its rows; behind the last one zeros
+        const bool there = c < 2 * RT;
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+            dma_piece(rb, stages + stage * P::STAGE + (w + i * 8) * 1024, there ? vb + (w + i * 8) * 8 * ldb : OUTSIDE, there ? c * CHUNK : 0);
+    };
+
+    // apply: column block sb, row tiles t0, t0 + 4
+    const int sb = w & 1, t0 = w >> 1;
+    // transposing read u (rows + 4 u), half l (hi, lo): lane 16 k + i fetches row i / 4, four columns at 16 (k & 1) + 4 (i % 4), eight rows further for k >= 2
+    int tr[2][2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int l = 0; l < 2; ++l) {
+            const int row = h * 8 + u * 4 + ((lane & 15) >> 2), seg = ((lane & 16) >> 3) + ((lane & 3) >> 1) + 4 * l;
+            tr[u][l] = sb * R * CHUNK + row * CHUNK + ((seg ^ (row & 7)) << 4) + (lane & 1) * 8;
+        }
+    f32x16 sums[GT];
+    if (MODE != LAST)
+#pragma unroll
+        for (int t = 0; t < GT; ++t)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) sums[t][k] = 0.f;
+
+    const int first = slice * m.per, last = min(first + m.per, panels);
+    if (P::RESIDENT) {
+        load_panel(first, lds);
+        if (MODE != FIRST)
+#pragma unroll
+            for (int c = 0; c < 2 * RT; ++c) load_b(c, c);
+    }
+    for (int p = first; p < last; ++p) {
+        char* image = lds + (P::RESIDENT ? (p - first) & 1 : 0) * P::IMAGE;
+        if (P::RESIDENT) {
+            // this panel has landed: loads and stores leave vmcnt in order, and behind its pieces stand the 2 RT stores of the panel before it at most
+            if (MODE == MIDDLE && p > first) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * RT) : "memory");
+            else wait_chunk();
+            __builtin_amdgcn_s_barrier();         // for every wave; and the other image is free
+            if (p + 1 < last) load_panel(p + 1, lds + ((p + 1 - first) & 1) * P::IMAGE);
+        } else {
+            load_panel(p, image);
+            if (MODE == FIRST) {
+                wait_chunk();
+                __builtin_amdgcn_s_barrier();
+            } else {
+#pragma unroll
+                for (int c = 0; c < STAGES - 1; ++c) load_b(c, c);
+            }
+        }
+        if (MODE != FIRST) {
+            f32x16 hh[AT], xx[AT];
+#pragma unroll
+            for (int n = 0; n < AT; ++n)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) { hh[n][k] = 0.f; xx[n][k] = 0.f; }
+            int stage = 0;
+#pragma unroll 1
+            for (int c = 0; c < 2 * RT; ++c) {
+                if (!P::RESIDENT) {               // chunk c (and, before it, the panel) has landed; the stage of chunk c - 1 is free
+                    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * RT) : "memory");
+                    __builtin_amdgcn_s_barrier();
+                    load_b(c + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
+                }
+                const char* bs = stages + stage * P::STAGE;
+                stage = stage == STAGES - 1 ? 0 : stage + 1;
+#pragma unroll
+                for (int sub = 0; sub < 2; ++sub) {
+                    const char* at = image + (c * 32 + sub * 16) * CHUNK;
+                    const half8 xh = join(tr_read(at + tr[0][0]), tr_read(at + tr[1][0])), xl = join(tr_read(at + tr[0][1]), tr_read(at + tr[1][1]));
+#pragma unroll
+                    for (int n = 0; n < AT; ++n)
+                        if (t0 + 4 * n < 2 * RT) {
+                            const char* rows = bs + (t0 + 4 * n) * 32 * CHUNK;
+                            const half8 bh = __builtin_bit_cast(half8, frag(rows, lane, sub)), bl = __builtin_bit_cast(half8, frag(rows, lane, 2 + sub));
+                            hh[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xh, bh, hh[n], 0, 0, 0);
+                            xx[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xh, bl, xx[n], 0, 0, 0);
+                            xx[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xl, bh, xx[n], 0, 0, 0);
+                        }
+                }
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();         // every wave has read the old panel
+#pragma unroll
+            for (int n = 0; n < AT; ++n)
+                if (t0 + 4 * n < 2 * RT) {
+                    const int row = (t0 + 4 * n) * 32 + l31;
+                    char* mine = image + sb * R * CHUNK + row * CHUNK + h * 8;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        char *ph = mine + ((q ^ (row & 7)) << 4), *pl = mine + (((q + 4) ^ (row & 7)) << 4);
+                        half4 xh = *reinterpret_cast<const half4*>(ph), xl = *reinterpret_cast<const half4*>(pl);
+                        float v[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float d = fmaf(xx[n][q * 4 + e], SPLIT_LO_INV, hh[n][q * 4 + e]);
+                            v[e] = fmaf(fx, pair_value(xh[e], xl[e]), d * fd);
+                        }
+                        if (MODE == LAST) {       // the result itself, in the place of the pairs
+                            *reinterpret_cast<float2*>(ph) = make_float2(ldexpf(v[0], unit), ldexpf(v[1], unit));
+                            *reinterpret_cast<float2*>(pl) = make_float2(ldexpf(v[2], unit), ldexpf(v[3], unit));
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) { _Float16 a, b; pair_of(v[e], a, b); xh[e] = a; xl[e] = b; }
+                            *reinterpret_cast<half4*>(ph) = xh;
+                            *reinterpret_cast<half4*>(pl) = xl;
+                        }
+                    }
+                }
+            __syncthreads();
+        }
+        if (MODE == MIDDLE) {                     // back to memory: 256 bytes of a row together
+#pragma unroll
+            for (int n = 0; n < 2 * RT; ++n) {
+                const int i = threadIdx.x + n * PANEL_THREADS, seg = i & 7, j = (i >> 3) & 1, row = i >> 4;
+                *reinterpret_cast<i32x4*>(x + (long long)row * ldx + (p * 2 + j) * CHUNK + seg * 16) =
+                    *reinterpret_cast<const i32x4*>(image + j * R * CHUNK + row * CHUNK + ((seg ^ (row & 7)) << 4));
+            }
+        }
+        if (MODE == LAST) {
+            const float lr = STEP ? (nu.lr_device ? *nu.lr_device : nu.lr) : 0.f, keep = 1.f - lr * nu.decay, rate = lr * o.size;
+            // element by element along the user's rows, eight of a thread together
+            constexpr int AT_ONCE = 8;
+#pragma unroll 1
+            for (int n0 = 0; n0 < 8 * RT; n0 += AT_ONCE) {
+                long long to[AT_ONCE];
+                float v[AT_ONCE], old[AT_ONCE];
+#pragma unroll
+                for (int n = 0; n < AT_ONCE; ++n) {
+                    const int i = threadIdx.x + (n0 + n) * PANEL_THREADS, row = o.tall ? i % R : i >> 6, col = o.tall ? i / R : i & 63, s = p * 64 + col;
+                    const bool in = row < m.r && s < m.s;
+                    to[n] = !in ? -1 : o.tall ? (long long)s * o.ld + row : (long long)row * o.ld + s;
+                    const int seg = ((col & 31) >> 3) + ((col & 2) << 1);
+                    v[n] = *reinterpret_cast<const float*>(image + (col >> 5) * R * CHUNK + row * CHUNK + ((seg ^ (row & 7)) << 4) + ((col >> 2) & 1) * 8 + (col & 1) * 4);
+                    if constexpr (STEP) old[n] = in ? ((const float*)o.dst)[to[n]] : 0.f;
+                }
+#pragma unroll
+                for (int n = 0; n < AT_ONCE; ++n)
+                    if (to[n] >= 0) {
+                        if constexpr (STEP) ((float*)o.dst)[to[n]] = fmaf(-rate, v[n], old[n] * keep);
+                        else store1<DT>(o.dst, to[n], v[n]);
+                    }
+            }
+        }
+        if (MODE != LAST) {
+#pragma unroll
+            for (int t = 0; t < GT; ++t) {
+                const int tile = w + t * 8;
+                if (tile >= GRAM) continue;
+                int i, j;
+                lower32(tile, i, j);
+                f32x16 gh, gx;
+#pragma unroll
+                for (int k = 0; k < 16; ++k) { gh[k] = 0.f; gx[k] = 0.f; }
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int sub = 0; sub < 2; ++sub) {
+                        const char *ai = image + c * R * CHUNK + i * 32 * CHUNK, *aj = image + c * R * CHUNK + j * 32 * CHUNK;
+                        const half8 ih = __builtin_bit_cast(half8, frag(ai, lane, sub)), il = __builtin_bit_cast(half8, frag(ai, lane, 2 + sub));
+                        const half8 jh = __builtin_bit_cast(half8, frag(aj, lane, sub)), jl = __builtin_bit_cast(half8, frag(aj, lane, 2 + sub));
+                        gh = __builtin_amdgcn_mfma_f32_32x32x16_f16(ih, jh, gh, 0, 0, 0);
+                        gx = __builtin_amdgcn_mfma_f32_32x32x16_f16(ih, jl, gx, 0, 0, 0);
+                        gx = __builtin_amdgcn_mfma_f32_32x32x16_f16(il, jh, gx, 0, 0, 0);
+                    }
+#pragma unroll
+                for (int k = 0; k < 16; ++k) sums[t][k] += fmaf(gx[k], SPLIT_LO_INV, gh[k]);
+            }
+        }
+        if (!P::RESIDENT) {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();         // every wave is done with the panel and the stages
+        }
+    }
+    if (MODE != LAST) {
+        float* part = (float*)(ws + parts_at(m.off, m.r, m.s)) + (long long)slice * R * R;
+#pragma unroll
+        for (int t = 0; t < GT; ++t) {
+            const int tile = w + t * 8;
+            if (tile >= GRAM) continue;
+            int i, j;
+            lower32(tile, i, j);
+            const int col = j * 32 + l31, row0 = i * 32 + h * 4;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) part[(row0 + (k >> 2) * 8 + (k & 3)) * R + col] = sums[t][k];
+            if (i != j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *reinterpret_cast<float4*>(part + (long long)col * R + row0 + q * 8) = make_float4(sums[t][q * 4], sums[t][q * 4 + 1], sums[t][q * 4 + 2], sums[t][q * 4 + 3]);
+        }
+    }
+}
+
+template <int MODE, int DT, bool STEP>
+__device__ __forceinline__ void panel_switch(const PanelWork& m, const PanelExit& o, char* ws, const Numbers& nu, char* lds) {
+    const int slice = blockIdx.x - m.wg0;
+    switch (up64(m.r) / 64) {
+        case 1: panel_body<1, MODE, DT, STEP>(m, o, ws, slice, nu, lds); break;
+        case 2: panel_body<2, MODE, DT, STEP>(m, o, ws, slice, nu, lds); break;
+        case 3: panel_body<3, MODE, DT, STEP>(m, o, ws, slice, nu, lds); break;
+        default: panel_body<4, MODE, DT, STEP>(m, o, ws, slice, nu, lds); break;
+    }
+}
+__global__ __launch_bounds__(PANEL_THREADS, 2) void ns_panel_first_kernel(PanelWorks t, char* ws) {
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    panel_switch<FIRST, F32, false>(t.m[find_by(t.count, blockIdx.x, [&](int i) { return t.m[i].wg0; })], PanelExit{}, ws, Numbers{}, lds);
+}
+__global__ __launch_bounds__(PANEL_THREADS, 2) void ns_panel_middle_kernel(PanelWorks t, char* ws, Numbers nu) {
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    panel_switch<MIDDLE, F32, false>(t.m[find_by(t.count, blockIdx.x, [&](int i) { return t.m[i].wg0; })], PanelExit{}, ws, nu, lds);
+}
+template <int DT, bool STEP>
+__global__ __launch_bounds__(PANEL_THREADS, 2) void ns_panel_last_kernel(PanelWorks t, PanelExits leave, char* ws, Numbers nu) {
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    const int k = find_by(t.count, blockIdx.x, [&](int i) { return t.m[i].wg0; });
+    panel_switch<LAST, DT, STEP>(t.m[k], leave.m[k], ws, nu, lds);
+}
+
+// Four neighbouring numbers of A: the sum of the Gram parts, as pairs.
+__device__ __forceinline__ void summed(const float* f, long long one, int slices, float scale, half4& hi, half4& lo) {
+    float4 s = *reinterpret_cast<const float4*>(f);
+#pragma unroll 8
+    for (int n = 1; n < slices; ++n) {
+        const float4 v = *reinterpret_cast<const float4*>(f + n * one);
+        s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+    const float v[4] = {s.x * scale, s.y * scale, s.z * scale, s.w * scale};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { _Float16 a, l; pair_of(v[e], a, l); hi[e] = a; lo[e] = l; }
+}
+__device__ __forceinline__ int slices_of(const PanelWork& m) { return (panels_of(m.s) + m.per - 1) / m.per; }
+
+// A = the sum of the Gram parts, on its own launch: where there are many parts, adding them where B is made would have every tile's workgroup read
+// half of them or more.
+__global__ __launch_bounds__(256) void ns_panel_sum_kernel(PanelWorks t, char* ws) {
+    const PanelWork m = t.m[find_by(t.count, blockIdx.x, [&](int i) { return t.m[i].sum0; })];
+    const int R = up64(m.r), i = (blockIdx.x - m.sum0) * 256 + threadIdx.x, row = i / (R / 4), col = i % (R / 4) * 4;      // R * R / 4 is a multiple of 256
+    half4 hi, lo;
+    summed((const float*)(ws + parts_at(m.off, m.r, m.s)) + (long long)row * R + col, (long long)R * R, slices_of(m), ldexpf(SA, -2 * x_exponent(m.r, m.s)), hi, lo);
+    _Float16* a = (_Float16*)(ws + pa_at(m.off, m.r, m.s)) + at(row, col, R);
+    *reinterpret_cast<half4*>(a) = hi;
+    *reinterpret_cast<half4*>(a + 32) = lo;
+}
+
+// B = b A + c A^2 of matrices of at most 256 rows: a 64 x 64 tile of the lower triangle a workgroup; the two blocks of 64 rows of A that it needs stand
+// whole in LDS.  SUMMED: A is in memory; otherwise the parts are added on the way.
+typedef Product<64, 64, 32, 32, 2, 2> PanelSquare;     // (its way of writing a tile; two groups of waves share the contraction)
+constexpr int panel_square_lds(int R) { return 2 * (R / 32) * 64 * CHUNK + PanelSquare::KG * PanelSquare::TILE; }
+
+template <bool SUMMED>
+__global__ __launch_bounds__(PANEL_THREADS, 2) void ns_panel_square_kernel(PanelWorks t, char* ws, float b, float c, int drop) {
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    const PanelWork m = t.m[find_by(t.count, blockIdx.x, [&](int i) { return t.m[i].square0; })];
+    const int R = up64(m.r), chunks = R / 32;
+    int ti, tj;
+    lower32(blockIdx.x - m.square0, ti, tj);
+    char *tiles = lds, *image = lds + PanelSquare::KG * PanelSquare::TILE;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (int blk = 0; blk < (ti == tj ? 1 : 2); ++blk) {
+        const int row0 = (blk ? tj : ti) * 64;
+        char* to = image + blk * chunks * 64 * CHUNK;
+        if constexpr (SUMMED) {
+            const int ld = R * 4;
+            const rsrc_t ra = rows_rsrc(ws + pa_at(m.off, m.r, m.s) + (long long)row0 * ld, 64, ld, ld);
+            const int va = lane_offset(lane, ld) + w * 8 * ld;
+            for (int cc = 0; cc < chunks; ++cc) dma_piece(ra, to + cc * 64 * CHUNK + w * 1024, va, cc * CHUNK);
+        } else {
+            const float* from = (const float*)(ws + parts_at(m.off, m.r, m.s)) + (long long)row0 * R;
+            const float scale = ldexpf(SA, -2 * x_exponent(m.r, m.s));
+            const int slices = slices_of(m);
+            for (int i = threadIdx.x; i < 16 * R; i += PANEL_THREADS) {      // four columns of a row
+                const int col = i % (R / 4) * 4, row = i / (R / 4), seg = (col & 31) >> 3;
+                half4 hi, lo;
+                summed(from + row * R + col, (long long)R * R, slices, scale, hi, lo);
+                char* at = to + ((col >> 5) * 64 + row) * CHUNK + (col & 4) * 2;
+                *reinterpret_cast<half4*>(at + ((seg ^ (row & 7)) << 4)) = hi;
+                *reinterpret_cast<half4*>(at + (((seg + 4) ^ (row & 7)) << 4)) = lo;
+            }
+        }
+    }
+    if constexpr (SUMMED) wait_chunk();
+    __syncthreads();
+    const char *rows_i = image, *rows_j = image + (ti == tj ? 0 : chunks * 64 * CHUNK);
+    const int group = w >> 2, wm = (w >> 1) & 1, wn = w & 1;
+    f32x16 hh, xx;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) { hh[e] = 0.f; xx[e] = 0.f; }
+    for (int cc = group; cc < chunks; cc += 2)
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
+            const char *ai = rows_i + (cc * 64 + wm * 32) * CHUNK, *aj = rows_j + (cc * 64 + wn * 32) * CHUNK;
+            const half8 ih = __builtin_bit_cast(half8, frag(ai, lane, sub)), il = __builtin_bit_cast(half8, frag(ai, lane, 2 + sub));
+            const half8 jh = __builtin_bit_cast(half8, frag(aj, lane, sub)), jl = __builtin_bit_cast(half8, frag(aj, lane, 2 + sub));
+            hh = __builtin_amdgcn_mfma_f32_32x32x16_f16(ih, jh, hh, 0, 0, 0);
+            xx = __builtin_amdgcn_mfma_f32_32x32x16_f16(ih, jl, xx, 0, 0, 0);
+            xx = __builtin_amdgcn_mfma_f32_32x32x16_f16(il, jh, xx, 0, 0, 0);
+        }
+    float* mine_t = (float*)(tiles + group * PanelSquare::TILE);
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+        mine_t[PanelSquare::T::at(wm * 32 + (e >> 2) * 8 + (lane >> 5) * 4 + (e & 3), wn * 32 + (lane & 31))] = fmaf(xx[e], SPLIT_LO_INV, hh[e]);
+    __syncthreads();
+    _Float16* out = (_Float16*)(ws + pb_at(m.off, m.r, m.s));
+    const float fb = b * (SB / SA), fc = ldexpf(c * (SB / (SA * SA)), -2 * g_of(ws, m.off, drop));
+    PanelSquare::rows(tiles, [&](int, int row, int col, float v[8]) {
+        const char* at = rows_i + ((tj * 2 + (col >> 5)) * 64 + row) * CHUNK;
+        const int seg = (col & 31) >> 3;
+        const half8 ah = *reinterpret_cast<const half8*>(at + ((seg ^ (row & 7)) << 4)), al = *reinterpret_cast<const half8*>(at + (((seg + 4) ^ (row & 7)) << 4));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = fmaf(fb, pair_value(ah[e], al[e]), fc * v[e]);
+    }, [&](int row, int col, half8 h, half8 l) { put8(out, at(ti * 64 + row, tj * 64 + col, R), h, l); });
+    if (ti == tj) return;
+    __syncthreads();
+    PanelSquare::columns(tiles, [&](int row, int col, half8 h, half8 l) { put8(out, at(tj * 64 + col, ti * 64 + row, R), h, l); });
+}
+
 // ------------------------------------------------------------------------------------------------------------------------------ host
 // Two sets of tiles.  Small: the filters of a network; few tiles, so four groups of waves share a contraction.  Large: many.
 struct SmallSet {
@@ -570,8 +977,11 @@ struct Plan {
     Works square, panel;
     Entries norm, pack;
     Exits leave;
-    long long tiles_square, tiles_panel, tiles_norm, tiles_pack, bytes;
+    long long tiles_square, tiles_panel, tiles_sum, tiles_norm, tiles_pack, bytes;
     bool large;
+    bool panels;           // every matrix of at most PANEL_ROWS rows: `works` instead of `square` and `panel`
+    PanelWorks works;
+    int lds_panel, lds_square;
 };
 
 template <class Set> void lay_out_products(Plan& p) {
@@ -583,6 +993,55 @@ template <class Set> void lay_out_products(Plan& p) {
         p.tiles_square += lower_tiles<typename Set::Square>(R);
         p.tiles_panel += (long long)((R + Set::Panel::BM - 1) / Set::Panel::BM) * ((S + Set::Panel::BN - 1) / Set::Panel::BN);
     }
+}
+
+// Panels of a workgroup.  A panel takes COST microseconds by its rows; the workgroups of a list (one for each CU at most, where that can be) should take
+// the same time, the least that does it.
+constexpr int PANEL_WGS = 256;
+constexpr double PANEL_COST[5] = {0, 2, 3.5, 7, 14};
+constexpr double PART_COST = 0.35;     // of adding a part where B is made, for each 64 rows; a launch that adds them costs 4 us
+void lay_out_panels(Plan& p) {
+    const int count = p.works.count;
+    auto per_of = [&](int i, double time) {
+        const double n = time / PANEL_COST[up64(p.works.m[i].r) / 64];
+        const int panels = panels_of(p.works.m[i].s);
+        return n < 1 ? 1 : n > panels ? panels : (int)n;
+    };
+    double time = 2;
+    for (;; time *= 1.1) {
+        long long wgs = 0;
+        bool one = true;                 // a matrix in one piece each: no fewer workgroups to be had
+        for (int i = 0; i < count; ++i) {
+            const int panels = panels_of(p.works.m[i].s), per = per_of(i, time);
+            wgs += (panels + per - 1) / per;
+            one = one && per == panels;
+        }
+        if (wgs <= PANEL_WGS || one) break;
+    }
+    long long wgs = 0, squares = 0, sums = 0, off = 0;
+    double adding = 0;
+    p.lds_panel = p.lds_square = 0;
+    for (int i = 0; i < count; ++i) {
+        PanelWork& m = p.works.m[i];
+        const int R = up64(m.r), panels = panels_of(m.s), lds = R == 64 ? PanelSize<1>::LDS : R == 128 ? PanelSize<2>::LDS : R == 192 ? PanelSize<3>::LDS : PanelSize<4>::LDS;
+        m.per = per_of(i, time);
+        const long long slices = (panels + m.per - 1) / m.per;
+        m.off = p.norm.m[i].off = p.pack.m[i].off = p.leave.m[i].off = off;
+        m.wg0 = (int)wgs;
+        m.square0 = (int)squares;
+        m.sum0 = (int)sums;
+        wgs += slices;
+        squares += (long long)(R / 64) * (R / 64 + 1) / 2;
+        sums += (long long)R * R / 1024;
+        adding = std::max(adding, PART_COST * slices * R / 64);
+        off = (parts_at(off, m.r, m.s) + slices * R * R * 4 + 255) & ~255LL;
+        p.lds_panel = lds > p.lds_panel ? lds : p.lds_panel;
+        p.lds_square = panel_square_lds(R) > p.lds_square ? panel_square_lds(R) : p.lds_square;
+    }
+    p.tiles_panel = wgs;
+    p.tiles_square = squares;
+    p.tiles_sum = adding > 4 ? sums : 0;
+    p.bytes = off;
 }
 
 // The launches of one group of matrices; returns false where a count passes what a grid holds.
@@ -605,6 +1064,16 @@ bool lay_out(const bflow_ns_matrix_t* m, int count, Plan& p) {
         p.tiles_norm += (n + per - 1) / per;
         p.tiles_pack += T * U;
         off = (end_at(off, r, s) + 255) & ~255LL;
+    }
+    p.panels = true;
+    p.works.count = count;
+    for (int i = 0; i < count; ++i) {
+        p.panels = p.panels && p.square.m[i].r <= PANEL_ROWS;
+        p.works.m[i] = {0, p.square.m[i].r, p.square.m[i].s, 0, 0, 0, 1};
+    }
+    if (p.panels) {
+        lay_out_panels(p);
+        return p.tiles_pack < (1LL << 30);
     }
     // One 1024 x 1024 (136 blocks): 261 us in small tiles, 452 in large ones; 8 of 512 x 512 (288): 304 / 329; 2048 x 2048 (528): 958 / 800;
     // 12 of 640 x 640 (660): 615 / 504; 8192 x 8192: 47.5 / 33.3 ms.
@@ -674,10 +1143,33 @@ int launch_products(const Plan& p, int steps, float a, float b, float c, double 
 }
 
 template <int DT, bool STEP>
+int launch_panels(const Plan& p, int steps, float a, float b, float c, double gain, char* ws, float lr, const float* lr_device, float decay, hipStream_t st) {
+    const auto last = ns_panel_last_kernel<DT, STEP>;
+    for (const int rc : {allow_lds(ns_panel_first_kernel, p.lds_panel), allow_lds(ns_panel_middle_kernel, p.lds_panel), allow_lds(last, p.lds_panel), allow_lds(ns_panel_square_kernel<true>, p.lds_square),
+                         allow_lds(ns_panel_square_kernel<false>, p.lds_square)})
+        if (rc) return rc;
+    const double bits = log2(gain);
+    PanelExits exits;
+    for (int i = 0; i < p.works.count; ++i) exits.m[i] = {p.leave.m[i].dst, p.leave.m[i].ld, p.leave.m[i].size, p.leave.m[i].tall};
+    const dim3 grid(p.tiles_panel), block(PANEL_THREADS);
+    hipLaunchKernelGGL(ns_panel_first_kernel, grid, block, p.lds_panel, st, p.works, ws);
+    for (int k = 0; k < steps; ++k) {
+        const Numbers nu = {(int)std::ceil(k * bits), (int)std::ceil((k + 1) * bits), a, lr, lr_device, decay};
+        if (p.tiles_sum) hipLaunchKernelGGL(ns_panel_sum_kernel, dim3(p.tiles_sum), dim3(256), 0, st, p.works, ws);
+        const auto square = p.tiles_sum ? ns_panel_square_kernel<true> : ns_panel_square_kernel<false>;
+        hipLaunchKernelGGL(square, dim3(p.tiles_square), block, p.lds_square, st, p.works, ws, b, c, nu.drop);
+        if (k + 1 < steps) hipLaunchKernelGGL(ns_panel_middle_kernel, grid, block, p.lds_panel, st, p.works, ws, nu);
+        else hipLaunchKernelGGL(last, grid, block, p.lds_panel, st, p.works, exits, ws, nu);
+    }
+    return launch_status("newton_schulz");
+}
+
+template <int DT, bool STEP>
 int launch_all(const Plan& p, int steps, float a, float b, float c, float eps, double gain, char* ws, float mu, int nesterov, float lr, const float* lr_device, float decay,
                hipStream_t st) {
     hipLaunchKernelGGL((ns_norm_kernel<DT, STEP>), dim3(p.tiles_norm), dim3(256), 0, st, p.norm, ws, mu, nesterov);
-    hipLaunchKernelGGL((ns_pack_kernel<DT, STEP>), dim3(p.tiles_pack), dim3(256), 0, st, p.pack, ws, mu, nesterov, eps);
+    hipLaunchKernelGGL((ns_pack_kernel<DT, STEP>), dim3(p.tiles_pack), dim3(256), 0, st, p.pack, ws, mu, nesterov, eps, (int)!p.panels);
+    if (p.panels) return launch_panels<DT, STEP>(p, steps, a, b, c, gain, ws, lr, lr_device, decay, st);
     return (p.large ? launch_products<LargeSet, DT, STEP> : launch_products<SmallSet, DT, STEP>)(p, steps, a, b, c, gain, ws, lr, lr_device, decay, st);
 }
 

@@ -46,7 +46,7 @@ template <int BM, int BN, int WM, int WN>
 struct ByteTile {
     static constexpr int M = BM, N = BN, ACROSS = BN / WN, WAVES = (BM / WM) * ACROSS, THREADS = 64 * WAVES, MT = WM / 32, NT = WN / 32;
     static constexpr int STAGE = (BM + BN) * CHUNK, LDS = 2 * STAGE;
-    static_assert(BM / 8 % WAVES == 0 && BN / 8 % WAVES == 0, "whole pieces of either operand for every wave");
+    static_assert(BM / 8 % WAVES == 0 && BN / 8 % WAVES == 0 && WAVES % 2 == 0, "whole pieces of either operand for every wave, all odd or all even");
     // B is the instruction's first operand: lane l then holds row l % 32 of a 32 x 32 block, four neighbouring columns in neighbouring registers
     i32x16 acc[MT][NT];
 
@@ -80,9 +80,9 @@ struct ByteTile {
         const int chunks = (K + CHUNK - 1) / CHUNK;
         int va[PA], vb[PB];
 #pragma unroll
-        for (int i = 0; i < PA; ++i) va[i] = lane_offset(lane, lda) + (wave + i * WAVES) * 8 * lda;
+        for (int i = 0; i < PA; ++i) va[i] = lane_offset(lane, lda, wave) + (wave + i * WAVES) * 8 * lda;
 #pragma unroll
-        for (int i = 0; i < PB; ++i) vb[i] = lane_offset(lane, ldb) + (wave + i * WAVES) * 8 * ldb;
+        for (int i = 0; i < PB; ++i) vb[i] = lane_offset(lane, ldb, wave) + (wave + i * WAVES) * 8 * ldb;
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -227,7 +227,7 @@ __global__ __launch_bounds__(256, 3) void i8_stream_kernel(StreamArgs s) {
         }
     const rsrc_t ra = rows_rsrc(g.a + z0 * g.a0 + z1 * g.a1 + (long long)m0 * g.lda, rows, g.lda, row_bytes);
     const rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc((void*)((T*)g.out + z0 * g.o0 + z1 * g.o1 + (long long)m0 * g.ldo), 0, 0x7fffffff, 0x00020000);
-    const int va = lane_offset(lane, g.lda);
+    const int va = lane_offset(lane, g.lda, wave);
     // a chunk lies as KC columns of 32 rows x 128 bytes; a wave moves eight rows of each
     auto issue = [&](int c, int slot) {
 #pragma unroll

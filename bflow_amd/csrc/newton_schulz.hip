@@ -256,12 +256,12 @@ struct Product {
     typedef Product<BM_, BN_, WM, WN, KG_, STAGES, false> Halves;
     static constexpr int CHUNK_BYTES = (BM + BN) * CHUNK, STAGE = KG * CHUNK_BYTES, TILE = BM * BN * 4;
     static constexpr int LDS = STAGES * STAGE > KG * TILE ? STAGES * STAGE : KG * TILE;
-    static_assert(BM / 8 % WAVES == 0 && BN / 8 % WAVES == 0, "whole pieces of either operand for every wave");
+    static_assert(BM / 8 % WAVES == 0 && BN / 8 % WAVES == 0 && WAVES % 2 == 0, "whole pieces of either operand for every wave, all odd or all even");
     typedef Turn<BN> T;
 
-    __device__ static __forceinline__ int source(int lane, int ld) {
-        if constexpr (PAIRS) return lane_offset(lane, ld);
-        const int seg = (lane & 7) ^ (lane >> 3);
+    __device__ static __forceinline__ int source(int lane, int ld, int wave) {
+        if constexpr (PAIRS) return lane_offset(lane, ld, wave);
+        const int seg = lane_segment(lane, wave);
         return (lane >> 3) * ld + (seg >> 2) * CHUNK + (seg & 3) * 16;
     }
 
@@ -270,7 +270,7 @@ struct Product {
         const int chunks = columns / COLUMNS;
         const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = w / WAVES, wave = w % WAVES;
         const int wm = wave / ACROSS, wn = wave % ACROSS;
-        const int va = source(lane, lda), vb = source(lane, ldb);
+        const int va = source(lane, lda, wave), vb = source(lane, ldb, wave);
         f32x16 hh[MT][NT], xx[MT][NT];
 #pragma unroll
         for (int i = 0; i < MT; ++i)
@@ -634,7 +634,7 @@ __device__ __forceinline__ void panel_body(const PanelWork& m, const PanelExit& 
     char* x = ws + x_at(m.off);
     char* stages = lds + P::IMAGES * P::IMAGE;
     const rsrc_t rx = rows_rsrc(x, R, ldx, ldx), rb = rows_rsrc(ws + pb_at(m.off, m.r, m.s), R, ldb, ldb);
-    const int vx = lane_offset(lane, ldx), vb = lane_offset(lane, ldb);
+    const int vx = lane_offset(lane, ldx, w), vb = lane_offset(lane, ldb, w);
     const int g = MODE == FIRST ? 0 : g_of(ws, m.off, nu.drop), down_g = MODE == MIDDLE ? g_of(ws, m.off, nu.drop_next) - g : 0;
     const float fx = ldexpf(nu.a, down_g), fd = ldexpf(1.f / SB, down_g - 2 * g);
     const int unit = MODE == LAST ? -x_exponent(m.r, m.s) - g : 0;
@@ -662,7 +662,7 @@ __device__ __forceinline__ void panel_body(const PanelWork& m, const PanelExit& 
 #pragma unroll
         for (int l = 0; l < 2; ++l) {
             const int row = h * 8 + u * 4 + ((lane & 15) >> 2), seg = ((lane & 16) >> 3) + ((lane & 3) >> 1) + 4 * l;
-            tr[u][l] = sb * R * CHUNK + row * CHUNK + ((seg ^ (row & 7)) << 4) + (lane & 1) * 8;
+            tr[u][l] = sb * R * CHUNK + row * CHUNK + ((seg ^ swizzle(row)) << 4) + (lane & 1) * 8;
         }
     f32x16 sums[GT];
     if (MODE != LAST)
@@ -736,7 +736,7 @@ __device__ __forceinline__ void panel_body(const PanelWork& m, const PanelExit& 
                     char* mine = image + sb * R * CHUNK + row * CHUNK + h * 8;
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        char *ph = mine + ((q ^ (row & 7)) << 4), *pl = mine + (((q + 4) ^ (row & 7)) << 4);
+                        char *ph = mine + ((q ^ swizzle(row)) << 4), *pl = mine + (((q + 4) ^ swizzle(row)) << 4);
                         half4 xh = *reinterpret_cast<const half4*>(ph), xl = *reinterpret_cast<const half4*>(pl);
                         float v[4];
 #pragma unroll
@@ -762,7 +762,7 @@ __device__ __forceinline__ void panel_body(const PanelWork& m, const PanelExit& 
             for (int n = 0; n < 2 * RT; ++n) {
                 const int i = threadIdx.x + n * PANEL_THREADS, seg = i & 7, j = (i >> 3) & 1, row = i >> 4;
                 *reinterpret_cast<i32x4*>(x + (long long)row * ldx + (p * 2 + j) * CHUNK + seg * 16) =
-                    *reinterpret_cast<const i32x4*>(image + j * R * CHUNK + row * CHUNK + ((seg ^ (row & 7)) << 4));
+                    *reinterpret_cast<const i32x4*>(image + j * R * CHUNK + row * CHUNK + ((seg ^ swizzle(row)) << 4));
             }
         }
         if (MODE == LAST) {
@@ -779,7 +779,7 @@ __device__ __forceinline__ void panel_body(const PanelWork& m, const PanelExit& 
                     const bool in = row < m.r && s < m.s;
                     to[n] = !in ? -1 : o.tall ? (long long)s * o.ld + row : (long long)row * o.ld + s;
                     const int seg = ((col & 31) >> 3) + ((col & 2) << 1);
-                    v[n] = *reinterpret_cast<const float*>(image + (col >> 5) * R * CHUNK + row * CHUNK + ((seg ^ (row & 7)) << 4) + ((col >> 2) & 1) * 8 + (col & 1) * 4);
+                    v[n] = *reinterpret_cast<const float*>(image + (col >> 5) * R * CHUNK + row * CHUNK + ((seg ^ swizzle(row)) << 4) + ((col >> 2) & 1) * 8 + (col & 1) * 4);
                     if constexpr (STEP) old[n] = in ? ((const float*)o.dst)[to[n]] : 0.f;
                 }
 #pragma unroll
@@ -910,7 +910,7 @@ __global__ __launch_bounds__(PANEL_THREADS, 2) void ns_panel_square_kernel(Panel
         if constexpr (SUMMED) {
             const int ld = R * 4;
             const rsrc_t ra = rows_rsrc(ws + pa_at(m.off, m.r, m.s) + (long long)row0 * ld, 64, ld, ld);
-            const int va = lane_offset(lane, ld) + w * 8 * ld;
+            const int va = lane_offset(lane, ld, w) + w * 8 * ld;
             for (int cc = 0; cc < chunks; ++cc) dma_piece(ra, to + cc * 64 * CHUNK + w * 1024, va, cc * CHUNK);
         } else {
             const float* from = (const float*)(ws + parts_at(m.off, m.r, m.s)) + (long long)row0 * R;
@@ -921,8 +921,8 @@ __global__ __launch_bounds__(PANEL_THREADS, 2) void ns_panel_square_kernel(Panel
                 half4 hi, lo;
                 summed(from + row * R + col, (long long)R * R, slices, scale, hi, lo);
                 char* at = to + ((col >> 5) * 64 + row) * CHUNK + (col & 4) * 2;
-                *reinterpret_cast<half4*>(at + ((seg ^ (row & 7)) << 4)) = hi;
-                *reinterpret_cast<half4*>(at + (((seg + 4) ^ (row & 7)) << 4)) = lo;
+                *reinterpret_cast<half4*>(at + ((seg ^ swizzle(row)) << 4)) = hi;
+                *reinterpret_cast<half4*>(at + (((seg + 4) ^ swizzle(row)) << 4)) = lo;
             }
         }
     }
@@ -953,7 +953,7 @@ __global__ __launch_bounds__(PANEL_THREADS, 2) void ns_panel_square_kernel(Panel
     PanelSquare::rows(tiles, [&](int, int row, int col, float v[8]) {
         const char* at = rows_i + ((tj * 2 + (col >> 5)) * 64 + row) * CHUNK;
         const int seg = (col & 31) >> 3;
-        const half8 ah = *reinterpret_cast<const half8*>(at + ((seg ^ (row & 7)) << 4)), al = *reinterpret_cast<const half8*>(at + (((seg + 4) ^ (row & 7)) << 4));
+        const half8 ah = *reinterpret_cast<const half8*>(at + ((seg ^ swizzle(row)) << 4)), al = *reinterpret_cast<const half8*>(at + (((seg + 4) ^ swizzle(row)) << 4));
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = fmaf(fb, pair_value(ah[e], al[e]), fc * v[e]);
     }, [&](int row, int col, half8 h, half8 l) { put8(out, at(ti * 64 + row, tj * 64 + col, R), h, l); });

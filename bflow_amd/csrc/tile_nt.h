@@ -6,8 +6,8 @@
 //   fp16 pairs       32 consecutive k of a row: 32 hi halves, then 32 lo halves (value = hi + lo * 2^-11, common.h)
 // so one loader and one LDS image serve both.  A stage holds one chunk of BM rows of A and BN rows of B; it is filled by LDS-DMA, 16 bytes a
 // lane: a wave instruction moves 8 rows of 128 bytes.  The DMA writes LDS linearly, so the bank swizzle is applied to the SOURCE address:
-// the 16-byte segment s of row r lands at segment s ^ (r & 7).  A fragment read (ds_read_b128, 32 rows by 2 neighbouring segments) then
-// touches every bank group equally.
+// the 16-byte segment s of row r lands at segment s ^ ((r >> 1) & 7).  LDS has 64 banks, two rows; 16 rows of a fragment read (ds_read_b128) then
+// take each bank once.  (With r & 7, rows r and r + 8 met: half of all LDS cycles were conflicts.)
 // Two stages alternate; the next chunk is in flight while the current one is multiplied, one barrier per chunk.
 #pragma once
 #include "common.h"
@@ -37,14 +37,17 @@ __device__ __forceinline__ rsrc_t rows_rsrc(const void* base, int rows, long lon
 // soff off the descriptor's size before it compares voff, so what may lie outside (rows behind the last one, OUTSIDE for a whole piece) goes into
 // voff, and soff stays below the length of a row.
 constexpr int OUTSIDE = (int)0x80000000u;
-__device__ __forceinline__ int lane_offset(int lane, int ld) { return (lane >> 3) * ld + (((lane & 7) ^ (lane >> 3)) << 4); }
+__device__ __forceinline__ int swizzle(int row) { return (row >> 1) & 7; }
+// `piece`: the piece's number in the LDS image (its parity counts: eight rows are half a period of the swizzle)
+__device__ __forceinline__ int lane_segment(int lane, int piece) { return (lane & 7) ^ swizzle((piece & 1) * 8 + (lane >> 3)); }
+__device__ __forceinline__ int lane_offset(int lane, int ld, int piece) { return (lane >> 3) * ld + (lane_segment(lane, piece) << 4); }
 __device__ __forceinline__ void dma_piece(rsrc_t r, char* lds_piece, int voff, int soff) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lptr_t)lds_piece, 16, voff, soff, 0, 0);
 }
 
 // 16 bytes of the fragment of row block `rows` (32 rows, LDS image): lane l reads row l % 32, segment 2 * sub + l / 32.
 __device__ __forceinline__ i32x4 frag(const char* rows, int lane, int sub) {
-    const int seg = (2 * sub + (lane >> 5)) ^ (lane & 7);
+    const int seg = (2 * sub + (lane >> 5)) ^ swizzle(lane & 31);
     return *reinterpret_cast<const i32x4*>(rows + (lane & 31) * CHUNK + seg * 16);
 }
 

@@ -36,6 +36,7 @@ struct Work {          // one matrix inside the products
     long long off;     // bytes from the workspace
     int r, s;          // rows <= columns
     int tile0;         // first workgroup of this launch
+    int ex;            // log2 sx
 };
 struct Entry {         // one matrix where it enters
     const void* src;   // the matrix, or the gradient (step)
@@ -43,7 +44,7 @@ struct Entry {         // one matrix where it enters
     long long ld, off;
     int r, s;
     int tile0, per;    // first workgroup; elements of one partial (norm)
-    int tall;
+    int tall, ex;
 };
 struct Exit {          // one matrix where it leaves
     void* dst;         // the result, or the weights (step)
@@ -51,6 +52,7 @@ struct Exit {          // one matrix where it leaves
     int r, s;
     int tile0, tall;
     float size;        // step: 0.2 sqrt(max(m, n))
+    int ex;
 };
 struct Works { Work m[MOST]; int count; };
 struct Entries { Entry m[MOST]; int count; };
@@ -68,7 +70,7 @@ __host__ __device__ inline long long b_at(long long off, int r, int s) { return 
 __host__ inline long long end_at(long long off, int r, int s) { return b_at(off, r, s) + mat_bytes(r, r); }
 
 // sx: the power of two next to sqrt(r s), at most 2^14 (|X| <= 2 then stays below the largest fp16)
-__host__ __device__ inline int x_exponent(int r, int s) {
+inline int x_exponent(int r, int s) {
     const double e = 0.5 * log2((double)r * (double)s);
     const int k = (int)(e + 0.5);
     return k > 14 ? 14 : k;
@@ -212,7 +214,7 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(Entries t, char* ws, float
     // (NaN and infinite norms: the comparison is false, g = 0)
     const int g = norm > 0. && norm < (double)eps ? (int)log2((norm + (double)eps) / norm) : 0;
     if (w == 0 && threadIdx.x == 0) *(int*)(ws + g_at(m.off)) = g;
-    const double scale = ldexp(1.0, x_exponent(m.r, m.s) + g) / (norm + (double)eps);
+    const double scale = ldexp(1.0, m.ex + g) / (norm + (double)eps);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
         _Float16 h, l;
@@ -444,7 +446,7 @@ __global__ __launch_bounds__(P::THREADS, 2) void ns_gram_kernel(Works t, char* w
     lower<P>(blockIdx.x - m.tile0, R, r0, c0);
     const char* x = ws + x_at(m.off);
     P::run(rows_rsrc(x + (long long)r0 * ld, min(P::BM, R - r0), ld, ld), ld, rows_rsrc(x + (long long)c0 * ld, min(P::BN, R - c0), ld, ld), ld, S, lds);
-    const float scale = ldexpf(SA, -2 * x_exponent(m.r, m.s));
+    const float scale = ldexpf(SA, -2 * m.ex);
     _Float16* a = (_Float16*)(ws + a_at(m.off, m.r, m.s));
     P::rows(lds, [&](int, int, int, float v[8]) {
 #pragma unroll
@@ -529,7 +531,7 @@ __global__ __launch_bounds__(P::THREADS, 2) void ns_leave_kernel(Exits t, const 
     typename P::Ahead xv;
     xv.load((const _Float16*)(ws + x_at(m.off)), r0, s0, R, S);
     P::run(rows_rsrc(b + (long long)r0 * ld, min(P::BM, R - r0), ld, ld), ld, rows_rsrc(xt + (long long)s0 * ld, min(P::BN, S - s0), ld, ld), ld, R, lds);
-    const int g = g_of(ws, m.off, drop), unit = -x_exponent(m.r, m.s) - g;
+    const int g = g_of(ws, m.off, drop), unit = -m.ex - g;
     const float fd = ldexpf(1.f / SB, -2 * g);
     if constexpr (STEP) lr = lr_device ? *lr_device : lr;
     const float keep = 1.f - lr * decay, rate = lr * m.size;
@@ -576,7 +578,8 @@ constexpr int PANEL_ROWS = 256, PANEL_THREADS = 512;
 
 struct PanelWork {     // one matrix
     long long off;
-    int r, s;
+    short r, ex;       // rows; log2 sx
+    int s;
     int wg0, square0, sum0;  // first workgroup of the panel launches, of those that make B, of those that add the parts
     int per;           // panels of a workgroup
 };
@@ -588,12 +591,13 @@ struct PanelExit {     // where a matrix leaves
     int tall;
 };
 struct PanelExits { PanelExit m[MOST]; };
-static_assert(sizeof(PanelWorks) + sizeof(PanelExits) <= 4000, "the tables are kernel arguments");
-// regions: norm partials, g, X, B, A, the Gram parts (32 bits, R x R each)
+static_assert(sizeof(PanelWorks) + sizeof(PanelExits) <= 4096, "the tables are kernel arguments");
+// regions: norm partials, g, X, B, A, the Gram parts (32 bits, lower tiles)
 __host__ __device__ inline long long pb_at(long long off, int r, int s) { return x_at(off) + mat_bytes(r, s); }
 __host__ __device__ inline long long pa_at(long long off, int r, int s) { return pb_at(off, r, s) + mat_bytes(r, r); }
 __host__ __device__ inline long long parts_at(long long off, int r, int s) { return pa_at(off, r, s) + mat_bytes(r, r); }
 __host__ __device__ inline int panels_of(int s) { return up64(s) / 64; }
+__host__ __device__ inline long long part_size(int R) { return (long long)(R / 32) * (R / 32 + 1) / 2 * 1024; }      // lower 32 x 32 tiles, in numbers
 
 template <class F> __device__ __forceinline__ int find_by(int count, int wg, F first) {
     const int lane = threadIdx.x & 63;
@@ -637,7 +641,7 @@ __device__ __forceinline__ void panel_body(const PanelWork& m, const PanelExit& 
     const int vx = lane_offset(lane, ldx, w), vb = lane_offset(lane, ldb, w);
     const int g = MODE == FIRST ? 0 : g_of(ws, m.off, nu.drop), down_g = MODE == MIDDLE ? g_of(ws, m.off, nu.drop_next) - g : 0;
     const float fx = ldexpf(nu.a, down_g), fd = ldexpf(1.f / SB, down_g - 2 * g);
-    const int unit = MODE == LAST ? -x_exponent(m.r, m.s) - g : 0;
+    const int unit = MODE == LAST ? -m.ex - g : 0;
 
     auto load_panel = [&](int p, char* image) {   // 2 chunks x R rows, 8 rows a piece
 #pragma unroll
@@ -820,21 +824,15 @@ __device__ __forceinline__ void panel_body(const PanelWork& m, const PanelExit& 
             __builtin_amdgcn_s_barrier();         // every wave is done with the panel and the stages
         }
     }
-    if (MODE != LAST) {
-        float* part = (float*)(ws + parts_at(m.off, m.r, m.s)) + (long long)slice * R * R;
+    if (MODE != LAST) {                           // the lower tiles, each in the order of the registers: whole lines
+        float* part = (float*)(ws + parts_at(m.off, m.r, m.s)) + (long long)slice * part_size(R) + lane * 4;
 #pragma unroll
         for (int t = 0; t < GT; ++t) {
             const int tile = w + t * 8;
             if (tile >= GRAM) continue;
-            int i, j;
-            lower32(tile, i, j);
-            const int col = j * 32 + l31, row0 = i * 32 + h * 4;
 #pragma unroll
-            for (int k = 0; k < 16; ++k) part[(row0 + (k >> 2) * 8 + (k & 3)) * R + col] = sums[t][k];
-            if (i != j)
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    *reinterpret_cast<float4*>(part + (long long)col * R + row0 + q * 8) = make_float4(sums[t][q * 4], sums[t][q * 4 + 1], sums[t][q * 4 + 2], sums[t][q * 4 + 3]);
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<float4*>(part + tile * 1024 + q * 256) = make_float4(sums[t][q * 4], sums[t][q * 4 + 1], sums[t][q * 4 + 2], sums[t][q * 4 + 3]);
         }
     }
 }
@@ -864,7 +862,7 @@ __global__ __launch_bounds__(PANEL_THREADS, 2) void ns_panel_last_kernel(PanelWo
     panel_switch<LAST, DT, STEP>(t.m[k], leave.m[k], ws, nu, lds);
 }
 
-// Four neighbouring numbers of A: the sum of the Gram parts, as pairs.
+// Four numbers of A, rows 8 q + 4 h .. + 3 of column `lane % 32` of a tile: the sum of the Gram parts, as pairs.
 __device__ __forceinline__ void summed(const float* f, long long one, int slices, float scale, half4& hi, half4& lo) {
     float4 s = *reinterpret_cast<const float4*>(f);
 #pragma unroll 8
@@ -879,15 +877,28 @@ __device__ __forceinline__ void summed(const float* f, long long one, int slices
 __device__ __forceinline__ int slices_of(const PanelWork& m) { return (panels_of(m.s) + m.per - 1) / m.per; }
 
 // A = the sum of the Gram parts, on its own launch: where there are many parts, adding them where B is made would have every tile's workgroup read
-// half of them or more.
+// half of them or more.  A workgroup adds one 32 x 32 tile and writes it to both sides.
 __global__ __launch_bounds__(256) void ns_panel_sum_kernel(PanelWorks t, char* ws) {
+    __shared__ half2_t tile[32][33];
     const PanelWork m = t.m[find_by(t.count, blockIdx.x, [&](int i) { return t.m[i].sum0; })];
-    const int R = up64(m.r), i = (blockIdx.x - m.sum0) * 256 + threadIdx.x, row = i / (R / 4), col = i % (R / 4) * 4;      // R * R / 4 is a multiple of 256
+    const int R = up64(m.r), n = blockIdx.x - m.sum0, lane = threadIdx.x & 63, q = threadIdx.x >> 6, col = lane & 31, row = q * 8 + (lane >> 5) * 4;
+    int i, j;
+    lower32(n, i, j);
     half4 hi, lo;
-    summed((const float*)(ws + parts_at(m.off, m.r, m.s)) + (long long)row * R + col, (long long)R * R, slices_of(m), ldexpf(SA, -2 * x_exponent(m.r, m.s)), hi, lo);
-    _Float16* a = (_Float16*)(ws + pa_at(m.off, m.r, m.s)) + at(row, col, R);
-    *reinterpret_cast<half4*>(a) = hi;
-    *reinterpret_cast<half4*>(a + 32) = lo;
+    summed((const float*)(ws + parts_at(m.off, m.r, m.s)) + n * 1024 + threadIdx.x * 4, part_size(R), slices_of(m), ldexpf(SA, -2 * m.ex), hi, lo);
+    _Float16* a = (_Float16*)(ws + pa_at(m.off, m.r, m.s));
+    if (i != j) {                                 // column by column: the tile on the other side of the diagonal
+        *reinterpret_cast<half4*>(a + at(j * 32 + col, i * 32 + row, R)) = hi;
+        *reinterpret_cast<half4*>(a + at(j * 32 + col, i * 32 + row, R) + 32) = lo;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) tile[row + e][col] = half2_t{hi[e], lo[e]};
+    __syncthreads();
+    const int r = threadIdx.x >> 3, c = (threadIdx.x & 7) * 4;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { hi[e] = tile[r][c + e][0]; lo[e] = tile[r][c + e][1]; }
+    *reinterpret_cast<half4*>(a + at(i * 32 + r, j * 32 + c, R)) = hi;
+    *reinterpret_cast<half4*>(a + at(i * 32 + r, j * 32 + c, R) + 32) = lo;
 }
 
 // B = b A + c A^2 of matrices of at most 256 rows: a 64 x 64 tile of the lower triangle a workgroup; the two blocks of 64 rows of A that it needs stand
@@ -913,16 +924,26 @@ __global__ __launch_bounds__(PANEL_THREADS, 2) void ns_panel_square_kernel(Panel
             const int va = lane_offset(lane, ld, w) + w * 8 * ld;
             for (int cc = 0; cc < chunks; ++cc) dma_piece(ra, to + cc * 64 * CHUNK + w * 1024, va, cc * CHUNK);
         } else {
-            const float* from = (const float*)(ws + parts_at(m.off, m.r, m.s)) + (long long)row0 * R;
-            const float scale = ldexpf(SA, -2 * x_exponent(m.r, m.s));
-            const int slices = slices_of(m);
-            for (int i = threadIdx.x; i < 16 * R; i += PANEL_THREADS) {      // four columns of a row
-                const int col = i % (R / 4) * 4, row = i / (R / 4), seg = (col & 31) >> 3;
+            const float* parts = (const float*)(ws + parts_at(m.off, m.r, m.s));
+            const float scale = ldexpf(SA, -2 * m.ex);
+            const int slices = slices_of(m), col = lane & 31, row = (w & 3) * 8 + (lane >> 5) * 4;
+            for (int n = w >> 2; n < 2 * chunks; n += 2) {       // 32 x 32 tiles of the block, four waves each
+                const int half = n & 1, i = row0 / 32 + half, j = n >> 1, up = max(i, j), left = min(i, j);
                 half4 hi, lo;
-                summed(from + row * R + col, (long long)R * R, slices, scale, hi, lo);
-                char* at = to + ((col >> 5) * 64 + row) * CHUNK + (col & 4) * 2;
-                *reinterpret_cast<half4*>(at + ((seg ^ swizzle(row)) << 4)) = hi;
-                *reinterpret_cast<half4*>(at + (((seg + 4) ^ swizzle(row)) << 4)) = lo;
+                summed(parts + (up * (up + 1) / 2 + left) * 1024 + (w & 3) * 256 + lane * 4, part_size(R), slices, scale, hi, lo);
+                char* at = to + (j * 64 + half * 32) * CHUNK;
+                if (i >= j) {                                    // four rows of a column
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        char* r = at + (row + e) * CHUNK + (col & 7) * 2;
+                        *reinterpret_cast<_Float16*>(r + (((col >> 3) ^ swizzle(row + e)) << 4)) = hi[e];
+                        *reinterpret_cast<_Float16*>(r + ((((col >> 3) + 4) ^ swizzle(row + e)) << 4)) = lo[e];
+                    }
+                } else {                                         // from the other side of the diagonal: four columns of a row
+                    char* r = at + col * CHUNK + (row & 4) * 2;
+                    *reinterpret_cast<half4*>(r + (((row >> 3) ^ swizzle(col)) << 4)) = hi;
+                    *reinterpret_cast<half4*>(r + ((((row >> 3) + 4) ^ swizzle(col)) << 4)) = lo;
+                }
             }
         }
     }
@@ -1032,9 +1053,9 @@ void lay_out_panels(Plan& p) {
         m.sum0 = (int)sums;
         wgs += slices;
         squares += (long long)(R / 64) * (R / 64 + 1) / 2;
-        sums += (long long)R * R / 1024;
+        sums += part_size(R) / 1024;
         adding = std::max(adding, PART_COST * slices * R / 64);
-        off = (parts_at(off, m.r, m.s) + slices * R * R * 4 + 255) & ~255LL;
+        off = (parts_at(off, m.r, m.s) + slices * part_size(R) * 4 + 255) & ~255LL;
         p.lds_panel = lds > p.lds_panel ? lds : p.lds_panel;
         p.lds_square = panel_square_lds(R) > p.lds_square ? panel_square_lds(R) : p.lds_square;
     }
@@ -1055,11 +1076,11 @@ bool lay_out(const bflow_ns_matrix_t* m, int count, Plan& p) {
         const long long T = up64(r) / 64, U = up64(s) / 64, n = (long long)r * s;
         long long per = (n + NORM_PARTS - 1) / NORM_PARTS;
         per = per < NORM_MIN ? NORM_MIN : per;
-        p.square.m[i] = {off, r, s, 0};
-        p.norm.m[i] = {m[i].src, m[i].momentum, m[i].src_ld, off, r, s, (int)p.tiles_norm, (int)per, tall};
+        p.square.m[i] = {off, r, s, 0, x_exponent(r, s)};
+        p.norm.m[i] = {m[i].src, m[i].momentum, m[i].src_ld, off, r, s, (int)p.tiles_norm, (int)per, tall, x_exponent(r, s)};
         p.pack.m[i] = p.norm.m[i];
         p.pack.m[i].tile0 = (int)p.tiles_pack;
-        p.leave.m[i] = {m[i].dst, m[i].dst_ld, off, r, s, 0, tall, 0.2f * sqrtf((float)s)};
+        p.leave.m[i] = {m[i].dst, m[i].dst_ld, off, r, s, 0, tall, 0.2f * sqrtf((float)s), x_exponent(r, s)};
         blocks += T * (T + 1) / 2;
         p.tiles_norm += (n + per - 1) / per;
         p.tiles_pack += T * U;
@@ -1069,7 +1090,7 @@ bool lay_out(const bflow_ns_matrix_t* m, int count, Plan& p) {
     p.works.count = count;
     for (int i = 0; i < count; ++i) {
         p.panels = p.panels && p.square.m[i].r <= PANEL_ROWS;
-        p.works.m[i] = {0, p.square.m[i].r, p.square.m[i].s, 0, 0, 0, 1};
+        if (p.panels) p.works.m[i] = {0, (short)p.square.m[i].r, (short)p.square.m[i].ex, p.square.m[i].s, 0, 0, 0, 1};
     }
     if (p.panels) {
         lay_out_panels(p);
@@ -1096,6 +1117,11 @@ const char* bad(const bflow_ns_matrix_t* m, int count) {
 // Largest |x| that the steps make of any x in [0, 1] (the coefficients have to keep the iterates inside the pairs' range), and the largest
 // gain |x'| / |x| of one step there.
 double reach(int steps, double a, double b, double c, double* gain) {
+    static thread_local struct { int steps; double a, b, c, most, gain; } last = {0, 0, 0, 0, 0, 0};     // 20000 polynomials: once for a user's coefficients
+    if (last.steps == steps && last.a == a && last.b == b && last.c == c) {
+        *gain = last.gain;
+        return last.most;
+    }
     double most = 0;
     *gain = 1;
     for (int i = 0; i <= 4096; ++i) {
@@ -1108,6 +1134,7 @@ double reach(int steps, double a, double b, double c, double* gain) {
             if (std::fabs(f) > *gain) *gain = std::fabs(f);
         }
     }
+    last = {steps, a, b, c, most, *gain};
     return most;
 }
 

@@ -15,6 +15,7 @@ The reference trains with AdamW alone (modules/raft_spline.py:321-356).
 """
 from __future__ import annotations
 
+import math
 from typing import Dict, List, Sequence, Tuple
 
 import numpy as np
@@ -32,7 +33,9 @@ def _as_matrix(t: torch.Tensor, what: str) -> torch.Tensor:
         raise hip.BflowHipError(f"{what}: a matrix or a filter has two dimensions or more, got {tuple(t.shape)}")
     if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1]:
         return t
-    return t.contiguous().view(t.shape[0], -1)
+    if t.dim() == 2:
+        return t.contiguous()
+    return t.contiguous().view(t.shape[0], math.prod(t.shape[1:]))
 
 
 def _table(entries: Sequence[Tuple[int, int, int, int, int, int, int]]) -> np.ndarray:
@@ -53,27 +56,47 @@ def orthogonalize(matrices: Sequence[torch.Tensor], steps: int = STEPS, coeffici
     """Newton-Schulz steps on every matrix of a list: new tensors of the same shapes and types (float32, float16 or bfloat16, mixed as you like).
 
     Sums are held in 32 bits, products in fp16 pairs (fp32-class), whatever the type; the result is rounded once.  Tensors of more than two
-    dimensions are taken as (shape[0], everything else).  An empty matrix stays empty, a zero matrix zero; one with a NaN or an infinity
+    dimensions are taken as (shape[0], everything else).  The results of one type share a buffer.  An empty matrix stays empty, a zero matrix zero; one with a NaN or an infinity
     becomes all NaN.  Not differentiable: the results carry no graph."""
     _check_numbers(steps, coefficients, eps)
     if isinstance(matrices, torch.Tensor):
         raise hip.BflowHipError("orthogonalize takes a list of matrices")
-    results: List[torch.Tensor] = []
+    matrices = list(matrices)
     groups: Dict[Tuple[torch.dtype, torch.device], list] = {}
-    held = []                                             # contiguous copies live until the launches are enqueued
     for i, t in enumerate(matrices):
-        hip._dev(t, None, f"matrix {i}", contiguous=False)
-        if t.dtype not in hip.FLOAT_CODES:
-            raise hip.BflowHipError(f"matrix {i}: dtype {t.dtype}, expected one of {sorted(str(d) for d in hip.FLOAT_CODES)}")
-        x = _as_matrix(t, f"matrix {i}")
-        out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-        results.append(out)
-        if t.numel():
-            held.append(x)
-            rows, cols = x.shape
-            groups.setdefault((t.dtype, t.device), []).append((x.data_ptr(), out.data_ptr(), 0, x.stride(0) if rows > 1 else cols, cols, rows, cols))
-    for (dtype, device), entries in groups.items():
-        hip.ns_orthogonalize(_table(entries), dtype, device, int(steps), coefficients, eps)
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            hip._dev(t, None, f"matrix {i}", contiguous=False)                    # says why not
+        key = (t.dtype, t.device)
+        if key not in groups:
+            if t.dtype not in hip.FLOAT_CODES:
+                raise hip.BflowHipError(f"matrix {i}: dtype {t.dtype}, expected one of {sorted(str(d) for d in hip.FLOAT_CODES)}")
+            groups[key] = []
+        groups[key].append(i)
+    results: List[torch.Tensor] = [None] * len(matrices)
+    held = []                                             # contiguous copies live until the launches are enqueued
+    for (dtype, device), members in groups.items():
+        # one buffer for the results of a type, each on a boundary of 64 elements: an allocation each would cost as much as the launches
+        starts, total = [], 0
+        for i in members:
+            starts.append(total)
+            total += (matrices[i].numel() + 63) & ~63
+        room = torch.empty(total, dtype=dtype, device=device)
+        base, size, entries = room.data_ptr(), room.element_size(), []
+        for i, start in zip(members, starts):
+            t = matrices[i]
+            x = _as_matrix(t, f"matrix {i}")
+            shape, rows, cols = t.shape, x.shape[0], x.shape[1]
+            strides, n = [], 1
+            for d in reversed(shape):
+                strides.append(n)
+                n *= max(d, 1)
+            results[i] = room.as_strided(shape, strides[::-1], start)
+            if rows and cols:
+                if x is not t:
+                    held.append(x)
+                entries.append((x.data_ptr(), base + start * size, 0, x.stride(0) if rows > 1 else cols, cols, rows, cols))
+        if entries:
+            hip.ns_orthogonalize(_table(entries), dtype, device, int(steps), coefficients, eps)
     return results
 
 
@@ -124,21 +147,22 @@ class Muon(torch.optim.Optimizer):
         by_device: Dict[torch.device, list] = {}
         held = []
         for p in params:
-            g = p.grad
-            if g.is_sparse or g.dtype != torch.float32 or g.device != p.device:
+            g, state = p.grad, self.state[p]
+            if g.layout is not torch.strided or g.dtype is not torch.float32 or g.device != p.device:
                 raise hip.BflowHipError(f"Muon: gradients are dense float32 tensors on the parameter's device, got {g.dtype}, {g.layout}, {g.device}")
-            hip._dev(p, torch.float32, "parameter")
-            state = self.state[p]
             v = state.get("momentum_buffer")
             if v is None:
+                if not p.is_cuda:
+                    hip._dev(p, torch.float32, "parameter")
                 v = state["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
             if v.shape != p.shape:
                 raise hip.BflowHipError(f"Muon: momentum of shape {tuple(v.shape)} for a parameter of shape {tuple(p.shape)}")
-            g = _as_matrix(g, "gradient")
-            held.append(g)
-            rows, cols = g.shape
-            by_device.setdefault(p.device, []).append((g.data_ptr(), p.data_ptr(), hip._dev(v, torch.float32, "momentum"), g.stride(0) if rows > 1 else cols, cols,
-                                                       rows, cols))
+            x = _as_matrix(g, "gradient")
+            if x is not g:
+                held.append(x)
+            rows, cols = x.shape
+            by_device.setdefault(p.device, []).append((x.data_ptr(), hip._dev(p, torch.float32, "parameter"), hip._dev(v, torch.float32, "momentum"),
+                                                       x.stride(0) if rows > 1 else cols, cols, rows, cols))
         for device, entries in by_device.items():
             on_device = torch.is_tensor(lr) and lr.is_cuda
             hip.muon_step(_table(entries), device, int(group["steps"]), group["coefficients"], group["eps"], group["momentum"], group["nesterov"],

@@ -374,3 +374,29 @@ def test_out_that_repeats_itself_is_refused():
     a, sa = (t.to(DEV) for t in rows(5, 32))
     with pytest.raises(hip.BflowHipError, match="out"):
         int8.matmul(a.expand(3, 5, 32), sa.expand(3, 5), a, sa, out=torch.zeros(5, 5, device=DEV).expand(3, 5, 5))
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m,n,k", [(4090, 4080, 260), (2201, 2179, 300), (2176, 2178, 128), (1100, 2050, 129), (700, 772, 256), (513, 264, 1), (257, 256, 17), (8192, 33, 70), (40, 5000, 3000)])
+def test_matmul_of_every_form(m, n, k, kind):
+    """Tiles of each size, whole and odd, the streaming form at its limits (K = 1, 17, 128, 129, 256), against integers on the GPU's 64-bit floats: exact."""
+    a, sa = rows(m, k, 3)
+    b, sb = rows(n, k, 4)
+    sa, sb = sa / (200 * k), sb
+    y = int8.matmul(a.to(DEV), sa.to(DEV), b.to(DEV), sb.to(DEV), out_dtype=kind)
+    check(y, product(a, sa, b, sb), kind)
+
+
+@gpu
+def test_streaming_form_leaves_the_rest_alone():
+    """M, N and K that end inside a chunk, a panel and a segment; an `out` inside a larger buffer, several matrices, a repeated left side."""
+    for kind in KINDS:
+        a, sa = rows(555, 200, 1)
+        b, sb = rows(312, 200, 2, (3,))
+        room = torch.full((3, 570, 336), 7.0, dtype=kind, device=DEV)
+        view = room[:, 8:563, 8:320]
+        int8.matmul(a.to(DEV), (sa / 4096).to(DEV), b.to(DEV), sb.to(DEV), out_dtype=kind, out=view)
+        check(view.contiguous(), product(a, sa / 4096, b, sb), kind)
+        view.fill_(7.0)
+        assert bool((room == 7.0).all())

@@ -354,3 +354,51 @@ def test_training_steps_with_muon_eager_and_graphed():
     # the same kernels on the same numbers, but for the order of the look-up adjoint's sums (2^-24 each, through three updates)
     assert graphed == pytest.approx(eager, rel=1e-3)
     assert all(bool(torch.isfinite(p).all()) for p in m2.parameters())
+
+
+# ------------------------------------------------------------------------------------------------------------ the other sets of tiles
+@gpu
+@pytest.mark.parametrize("dtype", list(TOL))
+@pytest.mark.parametrize("shapes", [[(390 + k % 11, 385 + 3 * k % 40) for k in range(20)],         # 560 blocks of 64 x 64 in the Gram matrices: large tiles
+                                    [(257, 300), (40, 1000), (1, 5), (300, 257)],                   # one matrix over 256 rows: small tiles for all
+                                    [(256, 256), (193, 2000), (64, 64), (1, 3000), (2500, 65), (130, 129)]],     # at most 256 rows: panels
+                         ids=["large", "small", "panels"])
+def test_lists_of_every_set(shapes, dtype):
+    xs = [gradient(*s, seed=k).to(dtype) for k, s in enumerate(shapes)]
+    ys = muon.orthogonalize([x.to(DEV) for x in xs])
+    for x, y in zip(xs, ys):
+        assert off(y, plain(x)) < TOL[dtype]
+
+
+@gpu
+@pytest.mark.parametrize("shapes", [[(390, 385 + k) for k in range(20)], [(300, 280), (7, 9)], [(128, 1920), (192, 500), (256, 80), (9, 200)]], ids=["large", "small", "panels"])
+def test_step_of_every_set(shapes):
+    ps = [torch.nn.Parameter(gradient(*s, seed=k, size=1.0).to(DEV)) for k, s in enumerate(shapes)]
+    opt = muon.Muon(ps, lr=0.05, weight_decay=0.1)
+    before = [p.detach().clone() for p in ps]
+    for k, p in enumerate(ps):
+        p.grad = gradient(*shapes[k], seed=50 + k).to(DEV)
+    opt.step()
+    for p, old in zip(ps, before):
+        want, v = plain_step(old, p.grad, torch.zeros_like(old), 0.05, 0.1, 0.95, True)
+        moved, wanted = p.detach().cpu().double() - old.cpu().double(), want - old.cpu().double()
+        assert float((moved - wanted).norm()) < F32_TOL * float(wanted.norm()) + 2.0 ** -23 * float(want.norm())
+        assert off(opt.state[p]["momentum_buffer"], v) < 2.0 ** -23
+
+
+@gpu
+def test_long_matrices():
+    """Many panels of a workgroup, many parts of a Gram matrix; columns that end inside a panel."""
+    for shape in ((3, 70001), (64, 20033), (200, 9001), (70001, 2)):
+        x = gradient(*shape, seed=shape[0])
+        (y,) = muon.orthogonalize([x.to(DEV)])
+        assert off(y, plain(x)) < F32_TOL
+
+
+@gpu
+def test_results_of_one_type_share_a_buffer_and_stay_apart():
+    xs = [gradient(3, 5, seed=k).to(DEV) for k in range(4)]
+    ys = muon.orthogonalize(xs)
+    keep = [y.clone() for y in ys]
+    ys[1].fill_(7.0)
+    assert torch.equal(ys[0], keep[0]) and torch.equal(ys[2], keep[2]) and all(y.data_ptr() % 256 == 0 for y in ys)

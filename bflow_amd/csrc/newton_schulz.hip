@@ -983,6 +983,253 @@ __global__ __launch_bounds__(PANEL_THREADS, 2) void ns_panel_square_kernel(Panel
     PanelSquare::columns(tiles, [&](int row, int col, half8 h, half8 l) { put8(out, at(tj * 64 + col, ti * 64 + row, R), h, l); });
 }
 
+// ------------------------------------------------------------------------------------------------------------------------------ tiny
+// Matrices of at most 32 rows (heads, first layers, everything small in a list): one workgroup does all of it in one launch, in 64 bits.
+// All steps are polynomials of the starting Gram matrix S and commute with it: each multiplies by P = a + b S + c S^2 from the left and turns S into
+// P S P, so that the last X is the product of the P times the first X.  X is read twice, for S and for the end; the steps run on r x r matrices in
+// LDS.  In 32 bits that form loses what matters (an error of S in a weak direction grows with it, to 1e-4 in five steps); in 64 it costs little at
+// this size, products of 32-bit numbers are exact in it, and the result is off by its last rounding alone -- where the pairs above would do a little
+// worse than 32 bits (X is held to 2^-23, and few terms average).
+// v_mfma_f64_16x16x4: lane l holds row l % 16, k = l / 16 of the left operand, column l % 16 of the right one, and rows l / 16 + 4 e of the result.
+constexpr int TINY_ROWS = 32, TINY_THREADS = 512, TINY_LD = 33;
+// Numbers of a matrix: one workgroup reads them twice, in front of the panels of the list's other matrices (2 x 2: 9 us, 16 x 512 and 32 x 256: 13 and 17
+// us, 32 x 640 31 us -- the panels take 13 us a step and any number of matrices).  More of them with 8 rows and less, where pairs would be worse than
+// 32 bits (2 x 1152: by a quarter) and a thread a column is quick (4 x 2304: 13 us, 8 x 8000 37, 2 x 60000 86).
+constexpr int TINY_FEW = 8;
+constexpr long long TINY_NUMBERS = 1 << 13, TINY_NUMBERS_FEW = 1 << 17;
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+struct TinyTable { bflow_ns_matrix_t m[MOST]; };
+struct TinyNumbers {
+    double a, b, c, eps;
+    int steps, nesterov;
+    float mu, lr, decay;
+    const float* lr_device;
+};
+
+// tile (ti, tj) of X Y, R x R matrices in LDS
+template <int R> __device__ __forceinline__ f64x4 tiny_product(const double* x, const double* y, int ti, int tj, int lane) {
+    const double* xr = x + (ti * 16 + (lane & 15)) * TINY_LD + (lane >> 4);
+    const double* yc = y + (lane >> 4) * TINY_LD + tj * 16 + (lane & 15);
+    f64x4 d = {0., 0., 0., 0.}, d2 = {0., 0., 0., 0.};
+#pragma unroll
+    for (int k = 0; k < R; k += 8) {                    // two chains: the instruction's latency is its length
+        d = __builtin_amdgcn_mfma_f64_16x16x4f64(xr[k], yc[k * TINY_LD], d, 0, 0, 0);
+        d2 = __builtin_amdgcn_mfma_f64_16x16x4f64(xr[k + 4], yc[(k + 4) * TINY_LD], d2, 0, 0, 0);
+    }
+    return d + d2;
+}
+
+// NV > 0: at most NV rows (4 or 8), whose 16-row tiles would be mostly padding: S and the end by ordinary 64-bit arithmetic, a column a thread.
+template <int NT, int NV, int DT, bool STEP>
+__device__ __forceinline__ void tiny_body(const bflow_ns_matrix_t& m, const TinyNumbers& nu, double* S, double* room) {
+    constexpr int WAVES = TINY_THREADS / 64, SQUARE = TINY_ROWS * TINY_LD, R = NT * 16, AHEAD = 4 / NT;
+    double *P = room, *T = room + SQUARE, *Q = room + 2 * SQUARE;
+    const bool tall = m.rows > m.cols;
+    const int r = tall ? m.cols : m.rows, s = tall ? m.rows : m.cols;
+    const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // (i, j) of the r x s matrix, zero outside.  No branch around the loads: those outside read the last element inside, and all of a batch are in
+    // flight together.
+    auto number = [&](int i, int j, bool update) -> float {
+        const bool inside = i < r && j < s;
+        const int ic = min(i, r - 1), jc = min(j, s - 1), row = tall ? jc : ic, col = tall ? ic : jc;
+        const float x = load1<DT>(m.src, (long long)row * m.src_ld + col);
+        if constexpr (!STEP) return inside ? x : 0.f;
+        float* at = m.momentum + (long long)row * m.cols + col;
+        float v = *at;
+        if (update) {
+            v = fmaf(nu.mu, v, x);
+            if (inside) *at = v;
+        }
+        return !inside ? 0.f : nu.nesterov ? fmaf(nu.mu, v, x) : v;
+    };
+    if constexpr (NV > 0) {
+        constexpr int PAIRS = NV * (NV + 1) / 2, TOGETHER = 8 / NV;
+        double acc[PAIRS];
+#pragma unroll
+        for (int n = 0; n < PAIRS; ++n) acc[n] = 0;
+        for (int j = threadIdx.x; j < s; j += TOGETHER * TINY_THREADS) {
+            float x[TOGETHER][NV];
+#pragma unroll
+            for (int u = 0; u < TOGETHER; ++u)
+#pragma unroll
+                for (int i = 0; i < NV; ++i) x[u][i] = number(i, j + u * TINY_THREADS, true);
+#pragma unroll
+            for (int u = 0; u < TOGETHER; ++u)
+#pragma unroll
+                for (int i = 0, n = 0; i < NV; ++i)
+#pragma unroll
+                    for (int k = 0; k <= i; ++k, ++n) acc[n] = fma((double)x[u][i], (double)x[u][k], acc[n]);
+        }
+#pragma unroll
+        for (int n = 0; n < PAIRS; ++n) {
+            const double v = wave_sum(acc[n]);
+            if (lane == 0) room[w * PAIRS + n] = v;
+        }
+        for (int i = threadIdx.x; i < R * R; i += TINY_THREADS) S[(i / R) * TINY_LD + i % R] = 0;
+        __syncthreads();
+        if (threadIdx.x < PAIRS) {
+            int i = 0, n = threadIdx.x;
+            while (n > i) n -= ++i;                     // (0, 0), (1, 0), (1, 1), ...
+            double sum = 0;
+#pragma unroll
+            for (int k = 0; k < WAVES; ++k) sum += room[k * PAIRS + threadIdx.x];
+            S[i * TINY_LD + n] = sum;
+            S[n * TINY_LD + i] = sum;
+        }
+    } else {
+        // S = X X^T, before the norm is known; AHEAD blocks of 16 columns are read together
+        f64x4 acc[3] = {{0., 0., 0., 0.}, {0., 0., 0., 0.}, {0., 0., 0., 0.}};
+        for (int c0 = w * 16; c0 < s; c0 += AHEAD * WAVES * 16) {
+            float x[AHEAD][NT][4];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[u][n][e] = number(n * 16 + l15, c0 + u * WAVES * 16 + g * 4 + e, true);
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const double x0 = x[u][0][e], x1 = x[u][NT - 1][e];
+                    acc[0] = __builtin_amdgcn_mfma_f64_16x16x4f64(x0, x0, acc[0], 0, 0, 0);
+                    if (NT == 2) {
+                        acc[1] = __builtin_amdgcn_mfma_f64_16x16x4f64(x1, x0, acc[1], 0, 0, 0);
+                        acc[2] = __builtin_amdgcn_mfma_f64_16x16x4f64(x1, x1, acc[2], 0, 0, 0);
+                    }
+                }
+        }
+#pragma unroll
+        for (int n = 0; n < 2 * NT - 1; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) room[(w * 3 + n) * 256 + (g + 4 * e) * 16 + l15] = acc[n][e];
+        __syncthreads();
+        for (int i = threadIdx.x; i < (2 * NT - 1) * 256; i += TINY_THREADS) {
+            double sum = 0;
+#pragma unroll
+            for (int k = 0; k < WAVES; ++k) sum += room[k * 768 + i];
+            const int n = i >> 8, row = ((i >> 4) & 15) + (n > 0 ? 16 : 0), col = (i & 15) + (n == 2 ? 16 : 0);
+            S[row * TINY_LD + col] = sum;
+            if (n == 1) S[col * TINY_LD + row] = sum;
+        }
+    }
+    __syncthreads();
+    double trace = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) trace += S[i * TINY_LD + i];
+    const double scale = 1. / (sqrt(trace) + nu.eps);
+    __syncthreads();
+    for (int i = threadIdx.x; i < R * R; i += TINY_THREADS) S[(i / R) * TINY_LD + i % R] *= scale * scale;
+    __syncthreads();
+    // four waves make P Q, four P S and then P S P
+    const int tile = w & 3, ti = tile >> (NT - 1), tj = tile & (NT - 1);
+    const bool on = tile < NT * NT, left = w < 4;
+    const int at = (ti * 16 + g) * TINY_LD + tj * 16 + l15;     // of number e: 4 e rows further
+    for (int k = 0; k < nu.steps; ++k) {
+        if (left && on) {
+            const f64x4 d = tiny_product<R>(S, S, ti, tj, lane);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                P[at + 4 * e * TINY_LD] = (ti == tj && g + 4 * e == l15 ? nu.a : 0.) + nu.b * S[at + 4 * e * TINY_LD] + nu.c * d[e];
+        }
+        __syncthreads();
+        f64x4 d = {0., 0., 0., 0.};
+        if (on && !(left && k == 0)) d = tiny_product<R>(P, left ? Q : S, ti, tj, lane);
+        if (!left && on)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) T[at + 4 * e * TINY_LD] = d[e];
+        __syncthreads();
+        if (left && on)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) Q[at + 4 * e * TINY_LD] = k == 0 ? P[at + 4 * e * TINY_LD] : d[e];
+        if (!left && on) {
+            d = tiny_product<R>(T, P, ti, tj, lane);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) S[at + 4 * e * TINY_LD] = d[e];      // (S was last read in front of the barrier)
+        }
+        __syncthreads();
+    }
+    // the last X
+    const float lr = STEP ? (nu.lr_device ? *nu.lr_device : nu.lr) : 0.f, keep = 1.f - lr * nu.decay, rate = lr * 0.2f * sqrtf((float)s);
+    if constexpr (NV > 0) {
+        for (int j = threadIdx.x; j < s; j += TINY_THREADS) {
+            float x[NV], old[NV];
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                x[i] = number(i, j, false);
+                if constexpr (STEP) old[i] = ((const float*)m.dst)[tall ? (long long)j * m.dst_ld + min(i, r - 1) : (long long)min(i, r - 1) * m.dst_ld + j];
+            }
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                double d = 0;
+#pragma unroll
+                for (int k = 0; k < NV; ++k) d = fma(Q[i * TINY_LD + k], (double)x[k], d);
+                if (i >= r) continue;
+                const float v = (float)(d * scale);
+                const long long to = tall ? (long long)j * m.dst_ld + i : (long long)i * m.dst_ld + j;
+                if constexpr (STEP) ((float*)m.dst)[to] = fmaf(-rate, v, old[i] * keep);
+                else store1<DT>(m.dst, to, v);
+            }
+        }
+    } else {
+        double q[NT][R / 4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int k = 0; k < R / 4; ++k) q[n][k] = Q[(n * 16 + l15) * TINY_LD + 4 * k + g] * scale;
+        for (int c0 = w * 16; c0 < s; c0 += AHEAD * WAVES * 16) {
+            float x[AHEAD][R / 4];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+                for (int k = 0; k < R / 4; ++k) x[u][k] = number(4 * k + g, c0 + u * WAVES * 16 + l15, false);
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int j = c0 + u * WAVES * 16 + l15;
+                f64x4 d[NT];
+                float old[NT][4];
+                long long to[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    d[n] = f64x4{0., 0., 0., 0.};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int i = n * 16 + g + 4 * e;
+                        to[n][e] = i >= r || j >= s ? -1 : tall ? (long long)j * m.dst_ld + i : (long long)i * m.dst_ld + j;
+                        if constexpr (STEP) old[n][e] = ((const float*)m.dst)[max(to[n][e], 0LL)];
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < R / 4; ++k)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) d[n] = __builtin_amdgcn_mfma_f64_16x16x4f64(q[n][k], (double)x[u][k], d[n], 0, 0, 0);
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (to[n][e] >= 0) {
+                            const float v = (float)d[n][e];
+                            if constexpr (STEP) ((float*)m.dst)[to[n][e]] = fmaf(-rate, v, old[n][e] * keep);
+                            else store1<DT>(m.dst, to[n][e], v);
+                        }
+            }
+        }
+    }
+}
+
+template <int DT, bool STEP>
+__global__ __launch_bounds__(TINY_THREADS) void ns_tiny_kernel(TinyTable t, TinyNumbers nu) {
+    __shared__ double S[TINY_ROWS * TINY_LD];
+    __shared__ double room[TINY_THREADS / 64 * 3 * 256];      // the waves' parts of S; then P, T and Q
+    static_assert(3 * TINY_ROWS * TINY_LD <= TINY_THREADS / 64 * 3 * 256, "three matrices fit the parts");
+    const bflow_ns_matrix_t m = t.m[blockIdx.x];
+    const int r = min(m.rows, m.cols);
+    if (r <= 4) tiny_body<1, 4, DT, STEP>(m, nu, S, room);
+    else if (r <= 8) tiny_body<1, 8, DT, STEP>(m, nu, S, room);
+    else if (r <= 16) tiny_body<1, 0, DT, STEP>(m, nu, S, room);
+    else tiny_body<2, 0, DT, STEP>(m, nu, S, room);
+}
+
 // ------------------------------------------------------------------------------------------------------------------------------ host
 // Two sets of tiles.  Small: the filters of a network; few tiles, so four groups of waves share a contraction.  Large: many.
 struct SmallSet {
@@ -1200,22 +1447,56 @@ int launch_all(const Plan& p, int steps, float a, float b, float c, float eps, d
     return (p.large ? launch_products<LargeSet, DT, STEP> : launch_products<SmallSet, DT, STEP>)(p, steps, a, b, c, gain, ws, lr, lr_device, decay, st);
 }
 
-int check(const bflow_ns_matrix_t* m, int count, int steps, float a, float b, float c, float eps, const void* ws, long long ws_bytes, bool step, double* gain) {
+int check(const bflow_ns_matrix_t* m, int count, int steps, double a, double b, double c, double eps, const void* ws, long long ws_bytes, bool step, double* gain) {
     const char* why = bad(m, count);
     BFLOW_REQUIRE(!why, BFLOW_E_ARG, "newton_schulz: %s", why);
     BFLOW_REQUIRE(steps >= 1 && steps <= 32, BFLOW_E_ARG, "newton_schulz: %d steps (1 .. 32)", steps);
     BFLOW_REQUIRE(eps > 0.f && eps < 1.f, BFLOW_E_ARG, "newton_schulz: eps %g outside (0, 1)", (double)eps);
     const double most = reach(steps, a, b, c, gain);
     BFLOW_REQUIRE(most <= 1.9 && std::fabs(b) * 4 + std::fabs(c) * 16 < 63, BFLOW_E_ARG,
-                  "newton_schulz: coefficients (%g, %g, %g) take a singular value in [0, 1] to %g: the iterates must stay below 1.9", (double)a, (double)b,
-                  (double)c, most);
-    BFLOW_REQUIRE(!count || (ws && ((uintptr_t)ws & 255) == 0), BFLOW_E_ARG, "newton_schulz: workspace null or not aligned to 256 bytes");
+                  "newton_schulz: coefficients (%g, %g, %g) take a singular value in [0, 1] to %g: the iterates must stay below 1.9", a, b, c, most);
     const long long need = bflow_ns_workspace_bytes(m, count);
+    BFLOW_REQUIRE(need <= 0 || (ws && ((uintptr_t)ws & 255) == 0), BFLOW_E_ARG, "newton_schulz: workspace null or not aligned to 256 bytes");
     BFLOW_REQUIRE(need >= 0 && ws_bytes >= need, BFLOW_E_ARG, "newton_schulz: workspace of %lld bytes, %lld needed", ws_bytes, need);
     for (int i = 0; i < count; ++i)
         BFLOW_REQUIRE(m[i].src && m[i].dst && m[i].src_ld >= m[i].cols && m[i].dst_ld >= m[i].cols && (!step || m[i].momentum), BFLOW_E_ARG,
                       "newton_schulz: matrix %d: null pointer or a row shorter than its columns", i);
     return 0;
+}
+bool tiny(const bflow_ns_matrix_t& m) {
+    const int r = m.rows < m.cols ? m.rows : m.cols;
+    return r <= TINY_ROWS && (long long)m.rows * m.cols <= (r <= TINY_FEW ? TINY_NUMBERS_FEW : TINY_NUMBERS);
+}
+
+// f(group, n) for the matrices of a list that are tiny, or those that are not, MOST at a time.  f returns a status.
+template <class F> long long for_groups(const bflow_ns_matrix_t* m, int count, bool want_tiny, F f) {
+    bflow_ns_matrix_t group[MOST];
+    int n = 0;
+    for (int i = 0; i < count; ++i) {
+        if (tiny(m[i]) == want_tiny) group[n++] = m[i];
+        if (n == MOST || (i + 1 == count && n)) {
+            if (const long long rc = f(group, n)) return rc;
+            n = 0;
+        }
+    }
+    return 0;
+}
+
+template <int DT, bool STEP>
+int launch_list(const bflow_ns_matrix_t* m, int count, int steps, double a, double b, double c, double eps, double gain, char* ws, float mu, int nesterov, float lr,
+                const float* lr_device, float decay, hipStream_t st) {
+    long long rc = for_groups(m, count, true, [&](const bflow_ns_matrix_t* group, int n) -> long long {
+        TinyTable t = {};
+        for (int i = 0; i < n; ++i) t.m[i] = group[i];
+        hipLaunchKernelGGL((ns_tiny_kernel<DT, STEP>), dim3(n), dim3(TINY_THREADS), 0, st, t, TinyNumbers{a, b, c, eps, steps, nesterov, mu, lr, decay, lr_device});
+        return launch_status("newton_schulz");
+    });
+    if (rc) return (int)rc;
+    return (int)for_groups(m, count, false, [&](const bflow_ns_matrix_t* group, int n) -> long long {
+        static thread_local Plan p;
+        lay_out(group, n, p);
+        return launch_all<DT, STEP>(p, steps, (float)a, (float)b, (float)c, (float)eps, gain, ws, mu, nesterov, lr, lr_device, decay, st);
+    });
 }
 }  // namespace
 
@@ -1225,39 +1506,30 @@ extern "C" long long bflow_ns_workspace_bytes(const bflow_ns_matrix_t* m, int co
         return BFLOW_E_ARG;
     }
     long long most = 0;
-    for (int i = 0; i < count; i += MOST) {
+    const long long rc = for_groups(m, count, false, [&](const bflow_ns_matrix_t* group, int n) -> long long {
         static thread_local Plan p;
-        if (!lay_out(m + i, count - i < MOST ? count - i : MOST, p)) {
+        if (!lay_out(group, n, p)) {
             set_error("newton_schulz: too many tiles");
             return BFLOW_E_LIMIT;
         }
         most = p.bytes > most ? p.bytes : most;
-    }
-    return most;
+        return 0;
+    });
+    return rc ? rc : most;
 }
 
-extern "C" int bflow_ns_orthogonalize(const bflow_ns_matrix_t* m, int count, int dtype, int steps, float a, float b, float c, float eps, void* ws, long long ws_bytes,
-                                      bflow_stream_t stream) {
+extern "C" int bflow_ns_orthogonalize(const bflow_ns_matrix_t* m, int count, int dtype, int steps, double a, double b, double c, double eps, void* ws,
+                                      long long ws_bytes, bflow_stream_t stream) {
     BFLOW_REQUIRE(dtype >= F32 && dtype <= BF16, BFLOW_E_ARG, "ns_orthogonalize: dtype %d", dtype);
     double gain;
     if (const int rc = check(m, count, steps, a, b, c, eps, ws, ws_bytes, false, &gain)) return rc;
-    for (int i = 0; i < count; i += MOST) {
-        static thread_local Plan p;
-        lay_out(m + i, count - i < MOST ? count - i : MOST, p);
-        const auto go = dtype == F32 ? launch_all<F32, false> : dtype == F16 ? launch_all<F16, false> : launch_all<BF16, false>;
-        if (const int rc = go(p, steps, a, b, c, eps, gain, (char*)ws, 0.f, 0, 0.f, nullptr, 0.f, (hipStream_t)stream)) return rc;
-    }
-    return 0;
+    const auto go = dtype == F32 ? launch_list<F32, false> : dtype == F16 ? launch_list<F16, false> : launch_list<BF16, false>;
+    return go(m, count, steps, a, b, c, eps, gain, (char*)ws, 0.f, 0, 0.f, nullptr, 0.f, (hipStream_t)stream);
 }
 
-extern "C" int bflow_muon_step(const bflow_ns_matrix_t* m, int count, int steps, float a, float b, float c, float eps, float momentum, int nesterov, float lr,
-                               const float* lr_device, float weight_decay, void* ws, long long ws_bytes, bflow_stream_t stream) {
+extern "C" int bflow_muon_step(const bflow_ns_matrix_t* m, int count, int steps, double a, double b, double c, double eps, float momentum, int nesterov,
+                               float lr, const float* lr_device, float weight_decay, void* ws, long long ws_bytes, bflow_stream_t stream) {
     double gain;
     if (const int rc = check(m, count, steps, a, b, c, eps, ws, ws_bytes, true, &gain)) return rc;
-    for (int i = 0; i < count; i += MOST) {
-        static thread_local Plan p;
-        lay_out(m + i, count - i < MOST ? count - i : MOST, p);
-        if (const int rc = launch_all<F32, true>(p, steps, a, b, c, eps, gain, (char*)ws, momentum, nesterov, lr, lr_device, weight_decay, (hipStream_t)stream)) return rc;
-    }
-    return 0;
+    return launch_list<F32, true>(m, count, steps, a, b, c, eps, gain, (char*)ws, momentum, nesterov, lr, lr_device, weight_decay, (hipStream_t)stream);
 }

@@ -124,7 +124,7 @@ def lib() -> ctypes.CDLL:
         raise BflowHipError(f"{_LIB_PATH} is missing: build it with `python -m bflow_amd.build` "
                             "(hipcc --offload-arch=gfx950); there is no CPU fallback")
     L = ctypes.CDLL(_LIB_PATH)
-    vp, i, ll, f = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+    vp, i, ll, f, d = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_double
     L.bflow_version.restype = i
     L.bflow_version.argtypes = []
     L.bflow_last_error_string.restype = ctypes.c_char_p
@@ -208,8 +208,8 @@ def lib() -> ctypes.CDLL:
         "bflow_i8_quantize_rows": [vp, i, ll, ll, i, vp, i, vp, vp],
         "bflow_i8_quantize_pixels": [vp, vp, vp, i, i, i, i, i, i, vp, vp, vp],
         "bflow_ns_workspace_bytes": [vp, i],
-        "bflow_ns_orthogonalize": [vp, i, i, i, f, f, f, f, vp, ll, vp],
-        "bflow_muon_step": [vp, i, i, f, f, f, f, f, i, f, vp, f, vp, ll, vp],
+        "bflow_ns_orthogonalize": [vp, i, i, i, d, d, d, d, vp, ll, vp],
+        "bflow_muon_step": [vp, i, i, d, d, d, d, f, i, f, vp, f, vp, ll, vp],
     }
     for name, args in sig.items():
         if _ABI_ANY and not hasattr(L, name):

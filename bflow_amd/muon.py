@@ -55,9 +55,10 @@ def _check_numbers(steps: int, coefficients: Sequence[float], eps: float):
 def orthogonalize(matrices: Sequence[torch.Tensor], steps: int = STEPS, coefficients: Sequence[float] = COEFFICIENTS, eps: float = EPS) -> List[torch.Tensor]:
     """Newton-Schulz steps on every matrix of a list: new tensors of the same shapes and types (float32, float16 or bfloat16, mixed as you like).
 
-    Sums are held in 32 bits, products in fp16 pairs (fp32-class), whatever the type; the result is rounded once.  Tensors of more than two
-    dimensions are taken as (shape[0], everything else).  The results of one type share a buffer.  An empty matrix stays empty, a zero matrix zero; one with a NaN or an infinity
-    becomes all NaN.  Not differentiable: the results carry no graph."""
+    Sums are held in 32 bits, products in fp16 pairs (fp32-class; small matrices in 64 bits); a 16-bit result is rounded once, and its Gram matrices
+    come from the pairs' leading halves.  Tensors of more than two dimensions are taken as (shape[0], everything else).  The results of one type share
+    a buffer.  An empty matrix stays empty, a zero matrix zero; one with a NaN or an infinity becomes all NaN.  The same list gives the same bits; a
+    matrix in another list may be tiled another way and differ by roundings.  Not differentiable: the results carry no graph."""
     _check_numbers(steps, coefficients, eps)
     if isinstance(matrices, torch.Tensor):
         raise hip.BflowHipError("orthogonalize takes a list of matrices")
@@ -104,7 +105,8 @@ class Muon(torch.optim.Optimizer):
     """Muon for matrices and filters; AdamW for the groups marked `adamw=True` (biases, the scales and shifts of norms).
 
     lr may be a float32 scalar tensor on the parameters' device: the kernels read it when they run, so a captured graph follows a schedule.
-    Parameters, gradients and states are float32.  capturable: the AdamW step counters live on the device (torch.optim.AdamW)."""
+    Parameters, gradients and states are float32.  capturable: a step may be captured, after a first one that creates the states; the AdamW step
+    counters live on the device (torch.optim.AdamW)."""
 
     def __init__(self, params, lr=1e-3, momentum: float = 0.95, weight_decay: float = 0.0, nesterov: bool = True, steps: int = STEPS,
                  coefficients: Sequence[float] = COEFFICIENTS, eps: float = EPS, betas: Tuple[float, float] = (0.9, 0.999), adamw_eps: float = 1e-8,
@@ -138,22 +140,30 @@ class Muon(torch.optim.Optimizer):
                 loss = closure()
         for group in self.param_groups:
             params = [p for p in group["params"] if p.grad is not None and p.numel()]
+            if params and params[0].is_cuda and torch.cuda.is_current_stream_capturing():
+                # a captured first step would clear the state at every replay; counters and rates on the host would stay as they were
+                if not group["capturable"]:
+                    raise hip.BflowHipError("Muon: a step is captured into a graph with capturable=True only")
+                if any(not self.state.get(p) for p in params):
+                    raise hip.BflowHipError("Muon: take a first step outside the capture, it creates the states")
             if params:
                 (self._adamw if group["adamw"] else self._muon)(group, params)
         return loss
 
     def _muon(self, group, params):
         lr = group["lr"]
+        if torch.is_tensor(lr) and (lr.numel() != 1 or lr.dtype != torch.float32):
+            raise hip.BflowHipError(f"Muon: lr is a number or a float32 scalar, got {tuple(lr.shape)} {lr.dtype}")
         by_device: Dict[torch.device, list] = {}
         held = []
         for p in params:
-            g, state = p.grad, self.state[p]
+            g = p.grad
             if g.layout is not torch.strided or g.dtype is not torch.float32 or g.device != p.device:
                 raise hip.BflowHipError(f"Muon: gradients are dense float32 tensors on the parameter's device, got {g.dtype}, {g.layout}, {g.device}")
+            hip._dev(p, torch.float32, "parameter")
+            state = self.state[p]
             v = state.get("momentum_buffer")
             if v is None:
-                if not p.is_cuda:
-                    hip._dev(p, torch.float32, "parameter")
                 v = state["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
             if v.shape != p.shape:
                 raise hip.BflowHipError(f"Muon: momentum of shape {tuple(v.shape)} for a parameter of shape {tuple(p.shape)}")

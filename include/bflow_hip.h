@@ -590,11 +590,12 @@ int bflow_l1_masked_grad(const float* src, const float* tgt, const unsigned char
  *   bflow_muon_step       : per matrix, all fp32:  momentum = mu momentum + src (dense);  u = src + mu momentum (nesterov) or momentum;
  *                           dst = dst (1 - lr weight_decay) - lr 0.2 sqrt(max(rows, cols)) X(u).  lr: *lr_device (device float) when given.
  * `m` is a HOST table, read during the call (it travels in the launches' arguments; lists of any length, 64 matrices a round).  Matrices are
- * row-major, *_ld elements from row to row.  Arithmetic: fp16 pairs with fp32 sums (fp32-class accuracy), norms in fp64; a list gives the same
- * bits as its matrices one by one up to the order of partial sums, which depends on the sizes in the list alone, never on timing.  A matrix
- * with a NaN or an infinity becomes all NaN, a zero matrix stays zero.
- * ws: bflow_ns_workspace_bytes(m, count) bytes (rows and cols alone are read), aligned to 256, free for other use once the call's launches ran:
- * calls that may run at the same time need one each.
+ * row-major, *_ld elements from row to row, and none overlaps another but dst = src.  Arithmetic: fp16 pairs with fp32 sums (fp32-class accuracy;
+ * for 16-bit results A from the leading halves), small matrices in fp64, norms in fp64.  A list gives the same bits every time; its matrices one
+ * by one, or in another list, may be tiled another way and differ by roundings.  A matrix with a NaN or an infinity becomes all NaN, a zero matrix
+ * stays zero.
+ * ws: bflow_ns_workspace_bytes(m, count) bytes (rows and cols alone are read; 0 where all are small: ws may be NULL), aligned to 256, free for
+ * other use once the call's launches ran: calls that may run at the same time need one each.
  * steps 1 .. 32, eps in (0, 1), |a x + b x^3 + c x^5| iterated from [0, 1] has to stay below 1.9 and 4 |b| + 16 |c| below 63.                    */
 #define BFLOW_NS_MAX_MATRICES 64          /* of one round of launches  */
 #define BFLOW_NS_MAX_SIDE     (1 << 20)   /* rows or cols of one matrix; 2^30 elements at most */
@@ -606,9 +607,9 @@ typedef struct bflow_ns_matrix {
     int         rows, cols;
 } bflow_ns_matrix_t;
 long long bflow_ns_workspace_bytes(const bflow_ns_matrix_t* m, int count);
-int bflow_ns_orthogonalize(const bflow_ns_matrix_t* m, int count, int dtype, int steps, float a, float b, float c, float eps,
+int bflow_ns_orthogonalize(const bflow_ns_matrix_t* m, int count, int dtype, int steps, double a, double b, double c, double eps,
                            void* ws, long long ws_bytes, bflow_stream_t stream);
-int bflow_muon_step(const bflow_ns_matrix_t* m, int count, int steps, float a, float b, float c, float eps, float momentum, int nesterov,
+int bflow_muon_step(const bflow_ns_matrix_t* m, int count, int steps, double a, double b, double c, double eps, float momentum, int nesterov,
                     float lr, const float* lr_device, float weight_decay, void* ws, long long ws_bytes, bflow_stream_t stream);
 
 /* 8-bit integers with a scale for each row (csrc/int8_gemm.hip; host side bflow_amd/int8.py).  No counterpart in the reference; the

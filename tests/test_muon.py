@@ -75,17 +75,19 @@ def test_c_entry_refuses_bad_tables():
     """The C entry's own checks, before any launch: no GPU is touched."""
     lib = hip.lib()
 
-    def call(rows=4, cols=8, src=256, dst=256, src_ld=8, dst_ld=8, momentum=256, steps=5, abc=muon.COEFFICIENTS, eps=1e-7, dtype=0, ws=256, ws_bytes=1 << 30, step=False):
+    def call(rows=40, cols=80, src=256, dst=256, src_ld=80, dst_ld=80, momentum=256, steps=5, abc=muon.COEFFICIENTS, eps=1e-7, dtype=0, ws=256, ws_bytes=1 << 30, step=False):
         t = muon._table([(src, dst, momentum, src_ld, dst_ld, rows, cols)])
         if step:
             return lib.bflow_muon_step(t.ctypes.data, 1, steps, *abc, eps, 0.9, 1, 0.1, None, 0.0, ws, ws_bytes, None)
         return lib.bflow_ns_orthogonalize(t.ctypes.data, 1, dtype, steps, *abc, eps, ws, ws_bytes, None)
 
     for kw in (dict(rows=0), dict(cols=0), dict(cols=hip_limit() + 1), dict(rows=-1), dict(rows=1 << 16, cols=1 << 16, src_ld=1 << 16, dst_ld=1 << 16), dict(src=0), dict(dst=0),
-               dict(src_ld=7), dict(dst_ld=7), dict(steps=0), dict(steps=33), dict(eps=0.0), dict(eps=1.0), dict(dtype=3), dict(dtype=-1), dict(ws=0), dict(ws=128),
+               dict(src_ld=79), dict(dst_ld=79), dict(steps=0), dict(steps=33), dict(eps=0.0), dict(eps=1.0), dict(dtype=3), dict(dtype=-1), dict(ws=0), dict(ws=128),
                dict(ws_bytes=1024), dict(abc=(5.0, 0.0, 0.0)), dict(abc=(float("nan"), 0.0, 0.0)), dict(step=True, momentum=0)):
         assert call(**kw) == -1, kw
         assert b"newton_schulz" in lib.bflow_last_error_string() or b"ns_orthogonalize" in lib.bflow_last_error_string()
+    for kw in (dict(src=0), dict(dst_ld=3), dict(step=True, momentum=0), dict(steps=0)):       # a matrix that needs no workspace is checked all the same
+        assert call(rows=4, cols=8, **kw) == -1, kw
     assert lib.bflow_ns_workspace_bytes(None, 1) == -1
     empty = muon._table([])
     assert lib.bflow_ns_workspace_bytes(empty.ctypes.data, 0) == 0
@@ -200,6 +202,57 @@ def test_zero_tiny_huge_and_lost_values():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", list(TOL))
+def test_small_matrices_around_the_limits_of_their_kernel(dtype):
+    """Few rows, up to the sizes where the kernel in one workgroup ends and just beyond, wide and tall, alone and beside larger ones.  Held in 64 bits
+    below the limits: there fp32 results are off by their own rounding alone."""
+    shapes = [(r, c) for r in (1, 2, 4, 5, 8) for c in (1, 8, 513, 2049)] + [(r, c) for r in (9, 15, 16, 17, 31, 32) for c in (9, 33, 129, 256)]
+    shapes += [(8, 16384), (8, 16385), (1, 131072), (1, 131073), (32, 257), (33, 40), (16, 512), (16, 513), (9, 910), (9, 911), (3, 3), (2, 70001)]
+    shapes += [(c, r) for r, c in shapes if c != r]
+    xs = [gradient(*s, seed=k).to(dtype) for k, s in enumerate(shapes)]
+    dev = [x.to(DEV) for x in xs]
+    alone = muon.orthogonalize(dev)
+    beside = muon.orthogonalize([torch.ones(200, 300, device=DEV, dtype=dtype)] + dev)[1:]
+    for x, y, z in zip(xs, alone, beside):
+        r, numbers = min(x.shape), x.numel()
+        held = r <= 32 and numbers <= (1 << 17 if r <= 8 else 1 << 13)
+        # 64 bits: 2^-24 for the result's rounding; five steps of 2^-53 * sqrt(131072) each, at a growth of 485, stay far below it
+        limit = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11 + 2.0 ** -24, torch.bfloat16: 2.0 ** -8 + 2.0 ** -24}[dtype] * 1.001 if held else TOL[dtype]
+        if dtype is torch.float16:
+            limit += 2.0 ** -25 * math.sqrt(numbers) / float(plain(x).norm())           # below 2^-14 its step is 2^-24 whatever the value
+        assert off(y, plain(x)) < limit, (tuple(x.shape), limit)
+        assert not held or torch.equal(y, z)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", list(TOL))
+def test_result_over_the_matrix_itself(dtype):
+    """The C entry with dst = src: small matrices, panels and larger ones; the same bits as into another place."""
+    for shapes in ([(7, 90), (30, 100), (100, 20), (5, 3000), (64, 576)], [(300, 280), (12, 40)]):
+        xs = [gradient(*s, seed=k).to(dtype).to(DEV) for k, s in enumerate(shapes)]
+        want = muon.orthogonalize(xs)
+        table = muon._table([(x.data_ptr(), x.data_ptr(), 0, x.shape[1], x.shape[1], *x.shape) for x in xs])
+        hip.ns_orthogonalize(table, dtype, xs[0].device, 5, muon.COEFFICIENTS, 1e-7)
+        assert all(torch.equal(x, y) for x, y in zip(xs, want))
+
+
+@gpu
+def test_small_matrices_lost_values_and_steps():
+    x = gradient(12, 90, seed=4)
+    nan, inf, zero, small, large = x.clone(), x.clone(), torch.zeros(8, 3), x * 1e-37, x * 1e37
+    nan[11, 89], inf[0, 0] = float("nan"), float("inf")
+    ys = muon.orthogonalize([t.to(DEV) for t in (nan, inf, zero, small, large)])
+    assert torch.isnan(ys[0]).all() and torch.isnan(ys[1]).all() and not ys[2].any()
+    assert off(ys[3], plain(small)) < 2.0 ** -23 and off(ys[4], plain(large)) < 2.0 ** -23
+    for steps, eps in ((1, 1e-7), (2, 0.5), (9, 1e-7)):
+        for abc in (muon.COEFFICIENTS, (1.5, -0.5, 0.0)):
+            for shape in ((12, 90), (30, 31), (3, 1200)):
+                x = gradient(*shape, seed=steps)
+                (y,) = muon.orthogonalize([x.to(DEV)], steps=steps, coefficients=abc, eps=eps)
+                assert off(y, plain(x, steps, abc, eps)) < 2.0 ** -23, (steps, eps, abc, shape)
+
+
+@gpu
 def test_refuses_on_the_device():
     x = torch.zeros(4, 4, device=DEV)
     with pytest.raises(hip.BflowHipError, match="two dimensions"):
@@ -292,6 +345,59 @@ def test_optimizer_takes_strided_gradients_and_a_rate_on_the_device():
     assert torch.equal(p, q)
     b.load_state_dict(copy.deepcopy(a.state_dict()))
     assert torch.equal(b.state[q]["momentum_buffer"], a.state[p]["momentum_buffer"])
+
+
+@gpu
+def test_small_filters_step():
+    """Heads and first layers, as the step's kernel for small matrices takes them, with a rate on the device, eager and captured."""
+    shapes = [(2, 64, 3, 3), (2, 128, 1, 1), (8, 1, 1, 1), (20, 17), (32, 31), (1, 5), (70, 4, 2, 1), (40, 8, 3, 3)]
+    rate = torch.tensor(0.02, device=DEV)
+
+    def make():
+        return [torch.nn.Parameter(gradient(*s, seed=k, size=1.0).to(DEV)) for k, s in enumerate(shapes)]
+    ps, qs = make(), make()
+    a = muon.Muon(ps, lr=0.02, weight_decay=0.1)
+    b = muon.Muon(qs, lr=rate, weight_decay=0.1, capturable=True)
+    grads = [torch.empty(s, device=DEV) for s in shapes]
+    for p, q, g in zip(ps, qs, grads):
+        p.grad = q.grad = g
+    vs, graph = [torch.zeros(s, dtype=torch.float64) for s in shapes], torch.cuda.CUDAGraph()
+    for t in range(4):
+        for k, g in enumerate(grads):
+            g.copy_(gradient(*shapes[k], seed=10 * t + k))
+        before = [p.detach().cpu().clone() for p in ps]
+        a.step()
+        if t == 0:
+            b.step()
+            torch.cuda.synchronize()
+            with torch.cuda.graph(graph):
+                b.step()
+        else:
+            graph.replay()
+        for k, p in enumerate(ps):
+            want, vs[k] = plain_step(before[k], grads[k], vs[k], 0.02, 0.1, 0.95, True)
+            moved, wanted = p.detach().cpu().double() - before[k].double(), want - before[k].double()
+            assert float((moved - wanted).norm()) < F32_TOL * float(wanted.norm()) + 2.0 ** -23 * float(want.norm())
+            assert torch.equal(p, qs[k])
+            vs[k] = a.state[p]["momentum_buffer"].cpu().double()
+
+
+@gpu
+def test_a_capture_needs_states_and_says_so(monkeypatch):
+    w, x = torch.nn.Parameter(torch.ones(4, 4, device=DEV)), torch.nn.Parameter(torch.ones(4, device=DEV))
+    w.grad, x.grad = torch.ones(4, 4, device=DEV), torch.ones(4, device=DEV)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    groups = lambda: [{"params": [w]}, {"params": [x], "adamw": True}]
+    with pytest.raises(hip.BflowHipError, match="capturable"):
+        muon.Muon(groups()).step()
+    for group in groups():
+        with pytest.raises(hip.BflowHipError, match="first step"):
+            muon.Muon([group], capturable=True).step()
+    for lr in (torch.ones(2, device=DEV), torch.ones((), device=DEV, dtype=torch.float64), torch.ones(0, device=DEV)):
+        monkeypatch.undo()
+        with pytest.raises(hip.BflowHipError, match="float32 scalar"):
+            muon.Muon([w], lr=lr).step()
+    assert torch.equal(w, torch.ones_like(w)) and torch.equal(x, torch.ones_like(x))
 
 
 @gpu

@@ -228,7 +228,7 @@ def test_small_matrices_around_the_limits_of_their_kernel(dtype):
 @pytest.mark.parametrize("dtype", list(TOL))
 def test_result_over_the_matrix_itself(dtype):
     """The C entry with dst = src: small matrices, panels and larger ones; the same bits as into another place."""
-    for shapes in ([(7, 90), (30, 100), (100, 20), (5, 3000), (64, 576)], [(300, 280), (12, 40)]):
+    for shapes in ([(7, 90), (30, 100), (100, 20), (5, 3000), (64, 576)], [(300, 280), (12, 40)], [(32, 245), (500, 16), (33, 33), (20, 400), (2, 40000)]):
         xs = [gradient(*s, seed=k).to(dtype).to(DEV) for k, s in enumerate(shapes)]
         want = muon.orthogonalize(xs)
         table = muon._table([(x.data_ptr(), x.data_ptr(), 0, x.shape[1], x.shape[1], *x.shape) for x in xs])
@@ -348,9 +348,10 @@ def test_optimizer_takes_strided_gradients_and_a_rate_on_the_device():
 
 
 @gpu
-def test_small_filters_step():
+@pytest.mark.parametrize("shapes", [[(2, 64, 3, 3), (2, 128, 1, 1), (8, 1, 1, 1), (20, 17), (32, 31), (1, 5), (70, 4, 2, 1), (200, 16)],
+                                    [(2, 64, 3, 3), (20, 17), (64, 5, 7, 7), (40, 8, 3, 3), (96, 64, 1, 1)]], ids=["alone", "beside"])
+def test_small_filters_step(shapes):
     """Heads and first layers, as the step's kernel for small matrices takes them, with a rate on the device, eager and captured."""
-    shapes = [(2, 64, 3, 3), (2, 128, 1, 1), (8, 1, 1, 1), (20, 17), (32, 31), (1, 5), (70, 4, 2, 1), (40, 8, 3, 3)]
     rate = torch.tensor(0.02, device=DEV)
 
     def make():

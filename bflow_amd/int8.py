@@ -91,24 +91,35 @@ def _ready(t: torch.Tensor, K: int) -> bool:
 
 
 def _operands(ts, K: int, device):
-    """The operands as the kernel reads them: those that are not are copied, rows 16 bytes apart or a multiple, in one launch where they are rows of
-    bytes at even distances."""
-    out, items = list(ts), []
+    """(address, strides) of the operands as the kernel reads them, and what holds them: those that are not ready are copied into one buffer, rows 16
+    bytes apart or a multiple, in one launch where they are rows of bytes at even distances."""
+    out, items, wanting, room, total = [], [], [], None, 0
     ldd = _padded(K)
     for i, t in enumerate(ts):
         if _ready(t, K):
+            out.append((t.data_ptr(), t.stride()))
             continue
-        room = torch.empty(t.shape[:-1] + (ldd,), dtype=torch.int8, device=device)
-        shape, strides = t.shape, t.stride()
-        even = (strides[-1] == 1 or K == 1) and (t.dim() == 2 or (t.dim() == 3 and strides[0] == shape[1] * strides[1]))
-        if even:
-            items.append(hip.I8_PAD.pack(t.data_ptr(), room.data_ptr(), strides[-2], room.numel() // ldd, K, ldd))
-        else:
-            room[..., :K].copy_(t)
-        out[i] = room[..., :K]
-    if items:
-        hip._check(hip.lib().bflow_i8_pad_rows(b"".join(items), len(items), hip._stream()), "bflow_i8_pad_rows")
-    return out
+        rows, strides = 1, (1,)
+        for n in reversed(t.shape[:-1]):
+            strides = (rows * ldd,) + strides
+            rows *= n
+        out.append((total, strides))
+        wanting.append((i, t, rows))
+        total += rows * ldd
+    if wanting:
+        room = torch.empty(total, dtype=torch.int8, device=device)
+        base = room.data_ptr()
+        for i, t, rows in wanting:
+            at, strides = out[i]
+            out[i] = (base + at, strides)
+            shape, from_ = t.shape, t.stride()
+            if (from_[-1] == 1 or K == 1) and (len(shape) == 2 or (len(shape) == 3 and from_[0] == shape[1] * from_[1])):
+                items.append(hip.I8_PAD.pack(t.data_ptr(), base + at, from_[-2], rows, K, ldd))
+            else:
+                room.as_strided(shape, strides, at).copy_(t)
+        if items:
+            hip._check(hip.lib().bflow_i8_pad_rows(b"".join(items), len(items), hip._stream()), "bflow_i8_pad_rows")
+    return out, room
 
 
 def _broadcast(a: Tuple[int, ...], b: Tuple[int, ...]) -> Tuple[int, ...]:
@@ -120,10 +131,9 @@ def _broadcast(a: Tuple[int, ...], b: Tuple[int, ...]) -> Tuple[int, ...]:
     return tuple(y if x == 1 else x for x, y in zip(a, b))
 
 
-def _lead_strides(t: torch.Tensor, lead: int, batch: Tuple[int, ...]):
-    """Strides of t's first `lead` dimensions over `batch`; 0 where an element is repeated or there is only one."""
-    miss = len(batch) - lead
-    return [0] * miss + [s if n > 1 else 0 for n, s in zip(t.shape[:lead], t.stride()[:lead])]
+def _lead_strides(shape, strides, lead: int, batch: Tuple[int, ...]):
+    """Strides of an operand's first `lead` dimensions over `batch`; 0 where an element is repeated or there is only one."""
+    return [0] * (len(batch) - lead) + [s if n > 1 else 0 for n, s in zip(shape[:lead], strides[:lead])]
 
 
 def _fold(batch, strides):
@@ -173,13 +183,13 @@ def matmul(a: torch.Tensor, scale_a: torch.Tensor, b: torch.Tensor, scale_b: tor
     if not K:
         return out.zero_()
     with hip._on(device):
-        pa, pb = _operands((a, b), K, device)
+        ((pa, ra), (pb, rb)), held = _operands((a, b), K, device)         # (held: until the launches are enqueued)
         sa, sb = scale_a if scale_a.stride(-1) == 1 else scale_a.contiguous(), scale_b if scale_b.stride(-1) == 1 else scale_b.contiguous()
         strides, n0, n1 = (0,) * 10, 1, 1
         if batch:
             la, lb = len(ashape) - 2, len(bshape) - 2
-            two = _fold(batch, [_lead_strides(pa, la, batch), _lead_strides(pb, lb, batch), _lead_strides(sa, la, batch), _lead_strides(sb, lb, batch),
-                                _lead_strides(out, len(batch), batch)])
+            two = _fold(batch, [_lead_strides(ashape, ra, la, batch), _lead_strides(bshape, rb, lb, batch), _lead_strides(ashape, sa.stride(), la, batch),
+                                _lead_strides(bshape, sb.stride(), lb, batch), _lead_strides(shape, out.stride(), len(batch), batch)])
             if two is None:                                # dense copies of what is spread over more than two dimensions
                 whole = torch.empty(shape, dtype=out_dtype, device=device)
                 spread = lambda t, tail: t.expand(batch + tuple(t.shape[-tail:])).contiguous()
@@ -189,7 +199,7 @@ def matmul(a: torch.Tensor, scale_a: torch.Tensor, b: torch.Tensor, scale_b: tor
             (n0, s0), (n1, s1) = two
             strides = tuple(v for pair in zip(s0, s1) for v in pair)
         ld = _padded(K)
-        d = hip.I8_GEMM.pack(pa.data_ptr(), pb.data_ptr(), sa.data_ptr(), sb.data_ptr(), out.data_ptr(), *strides, out.stride(-2) if M > 1 else N,
-                             pa.stride(-2) if M > 1 else ld, pb.stride(-2) if N > 1 else ld, M, N, K, n0, n1, code, alpha)
+        d = hip.I8_GEMM.pack(pa, pb, sa.data_ptr(), sb.data_ptr(), out.data_ptr(), *strides, out.stride(-2) if M > 1 else N,
+                             ra[-2] if M > 1 else ld, rb[-2] if N > 1 else ld, M, N, K, n0, n1, code, alpha)
         hip._check(hip.lib().bflow_i8_gemm(d, hip._stream()), "bflow_i8_gemm")
     return out

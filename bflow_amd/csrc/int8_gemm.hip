@@ -1,7 +1,7 @@
 // Rows of 8-bit integers against rows of 8-bit integers, with a scale for each row of either side, and the quantisation in front of it
 // (gfx950 only).
 //
-//   out[i][j] = alpha * sa[i] * sb[j] * sum_k a[i][k] b[j][k]        sums exact in 32-bit integers (|k| < 2^17)
+//   out[i][j] = (alpha * sa[i]) * sb[j] * sum_k a[i][k] b[j][k]      sums exact in 32-bit integers (k < 2^17), then 32-bit floating point
 //   q[k] = nearest whole number to 127 x[k] / max|x| (halves to even, exactly), scale = max|x| / 127
 //
 // The integer matrix rate is twice the fp16 rate; at a feature dimension of 256 the correlation volume leaves the matrix cores' bound for the
@@ -30,6 +30,14 @@ struct GemmArgs {
     int tiles_m, tiles_n;
     int wide;               // the output's rows start at multiples of 16 bytes
 };
+
+// sum (alpha scale_a) scale_b, rounded to 32 bits before it is rounded to 16: left to itself the compiler joins the last product and the rounding to fp16
+// into one instruction in some kernels, and a row's bits would depend on which one takes it.
+template <class T> __device__ __forceinline__ T scaled(int sum, float sa, float sb) {
+    float v = (float)sum * sa * sb;
+    if constexpr (sizeof(T) == 2) asm("" : "+v"(v));
+    return (T)v;
+}
 
 // bytes k .. k + 15 of a fragment: those at or behind K become zero
 __device__ __forceinline__ i32x4 cut(i32x4 v, int k, int K) {
@@ -159,7 +167,7 @@ __global__ __launch_bounds__(Tile::THREADS, 2) void i8_gemm_kernel(GemmArgs g) {
                 const f32x4 c = *reinterpret_cast<const f32x4*>(scale_b + nw - n0 + j * 32 + q * 8 + (lane >> 5) * 4);
                 T4 v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = (T)((float)t.acc[i][j][q * 4 + e] * s * c[e]);
+                for (int e = 0; e < 4; ++e) v[e] = scaled<T>(t.acc[i][j][q * 4 + e], s, c[e]);
                 *reinterpret_cast<T4*>(turn + (lane & 31) * ROW + (j * 32 + q * 8 + (lane >> 5) * 4) * (int)sizeof(T)) = v;
             }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // the wave's own writes; no other wave touches this part
@@ -269,7 +277,7 @@ __global__ __launch_bounds__(256, 3) void i8_stream_kernel(StreamArgs s) {
                     const f32x4 sc = *reinterpret_cast<const f32x4*>(scale_b + wave * 64 + at);
                     T4 v;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = (T)((float)acc[j][q * 4 + e] * sr * sc[e]);
+                    for (int e = 0; e < 4; ++e) v[e] = scaled<T>(acc[j][q * 4 + e], sr, sc[e]);
                     *reinterpret_cast<T4*>(turn + (lane & 31) * ROW + (at - t * TURN) * (int)sizeof(T)) = v;
                 }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // the wave's own writes; no other wave touches this part
@@ -298,6 +306,7 @@ struct SkinnyArgs {
     long long of, om;      // strides of the output along the few and the many rows
     int F, M, K, n1;
     float alpha;
+    int few_is_a;          // alpha scale_a goes first, as in the other kernels: a row has the same bits however many stand beside it
 };
 constexpr int SKINNY_AHEAD = 8;    // steps of 64 k in flight
 
@@ -344,7 +353,7 @@ __global__ __launch_bounds__(256) void i8_skinny_kernel(SkinnyArgs g) {
             const int row = wave * 16 + (lane >> 4) * 4 + e;
             if (row < g.F) {
                 const float sf = g.sf[z0 * g.sf0 + z1 * g.sf1 + row];
-                ((T*)g.out)[z0 * g.o0 + z1 * g.o1 + row * g.of + col * g.om] = (T)((float)v[e] * (sf * g.alpha) * sm);
+                ((T*)g.out)[z0 * g.o0 + z1 * g.o1 + row * g.of + col * g.om] = scaled<T>(v[e], (g.few_is_a ? sf : sm) * g.alpha, g.few_is_a ? sm : sf);
             }
         }
     }
@@ -550,8 +559,8 @@ extern "C" int bflow_i8_gemm(const bflow_i8_gemm_t* d, bflow_stream_t stream) {
     const hipStream_t st = (hipStream_t)stream;
     // Few rows on one side: 6.4 us against 11.9 for one row at N = K = 4096, 10.0 against 12.1 for 32, 11.9 either way for 48.
     if (d->M <= 32 || d->N <= 32) {
-        const SkinnyArgs s = d->M <= d->N ? SkinnyArgs{g.a, g.b, g.sa, g.sb, g.out, g.a0, g.a1, g.b0, g.b1, g.sa0, g.sa1, g.sb0, g.sb1, g.o0, g.o1, g.lda, g.ldb, g.ldo, 1, g.M, g.N, g.K, g.n1, g.alpha}
-                                          : SkinnyArgs{g.b, g.a, g.sb, g.sa, g.out, g.b0, g.b1, g.a0, g.a1, g.sb0, g.sb1, g.sa0, g.sa1, g.o0, g.o1, g.ldb, g.lda, 1, g.ldo, g.N, g.M, g.K, g.n1, g.alpha};
+        const SkinnyArgs s = d->M <= d->N ? SkinnyArgs{g.a, g.b, g.sa, g.sb, g.out, g.a0, g.a1, g.b0, g.b1, g.sa0, g.sa1, g.sb0, g.sb1, g.o0, g.o1, g.lda, g.ldb, g.ldo, 1, g.M, g.N, g.K, g.n1, g.alpha, 1}
+                                          : SkinnyArgs{g.b, g.a, g.sb, g.sa, g.out, g.b0, g.b1, g.a0, g.a1, g.sb0, g.sb1, g.sa0, g.sa1, g.o0, g.o1, g.ldb, g.lda, 1, g.ldo, g.N, g.M, g.K, g.n1, g.alpha, 0};
         return s.F <= 16 ? launch_skinny<1>(s, d->dtype, (unsigned)batch, st) : launch_skinny<2>(s, d->dtype, (unsigned)batch, st);
     }
     // Short rows, whole 16-byte stores: 55 us against 64 (256 x 256 tiles) for 4 x 4800 x 4800 x 256 in fp16, 81 against 88 in fp32, 709 against 1233
@@ -623,7 +632,9 @@ extern "C" int bflow_i8_quantize_pixels(const float* x, const void* x_hi, const 
                   "i8_quantize_pixels: B = %d, D = %d (a multiple of 16), %d x %d pixels", B, D, h, w);
     BFLOW_REQUIRE(x || (D % 32 == 0 && np >= h * w), BFLOW_E_ARG, "i8_quantize_pixels: packed operand of %d rows for %d pixels, D = %d (a multiple of 32)", np, h * w, D);
     BFLOW_REQUIRE((uintptr_t)q % 16 == 0, BFLOW_E_ARG, "i8_quantize_pixels: q is not aligned to 16 bytes");
-    const int rows = tiled ? (h + 3) / 4 * ((w + 7) / 8) * 32 : h * w;
+    const long long places = tiled ? (long long)((h + 3) / 4) * ((w + 7) / 8) * 32 : (long long)h * w;
+    BFLOW_REQUIRE(places <= 1 << 30, BFLOW_E_LIMIT, "i8_quantize_pixels: %lld places of %d x %d pixels", places, h, w);
+    const int rows = (int)places;
     const dim3 grid((rows + 63) / 64, B);
     if (x) hipLaunchKernelGGL(quantize_pixels_kernel, grid, dim3(1024), 0, (hipStream_t)stream, x, D, h, w, rows, tiled, q, scale);
     else hipLaunchKernelGGL(quantize_packed_kernel, grid, dim3(256), 0, (hipStream_t)stream, (const _Float16*)x_hi, (const _Float16*)x_lo, D / 32, h, w, np, rows, tiled, q, scale);

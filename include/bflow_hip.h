@@ -614,8 +614,8 @@ int bflow_muon_step(const bflow_ns_matrix_t* m, int count, int steps, double a, 
 
 /* 8-bit integers with a scale for each row (csrc/int8_gemm.hip; host side bflow_amd/int8.py).  No counterpart in the reference; the
  * correlation volume (models/raft_utils/corr.py:264-272) is built on it for `correlation.precision: i8` (bflow_amd/corr.py).
- *   bflow_i8_gemm          : out[z, i, j] = alpha scale_a[z, i] scale_b[z, j] sum_k a[z, i, k] b[z, j, k], rounded once to dtype (0 fp32, 1 fp16,
- *                            2 bf16); sums exact in 32-bit integers.  z = (z0, z1) over batch0 x batch1; every operand has its own strides for
+ *   bflow_i8_gemm          : out[z, i, j] = (sum_k a[z, i, k] b[z, j, k]) (alpha scale_a[z, i]) scale_b[z, j], sums exact in 32-bit integers, the
+ *                            rest in fp32 in this order, rounded once more to dtype (0 fp32, 1 fp16, 2 bf16); the same bits whatever M and N.  z = (z0, z1) over batch0 x batch1; every operand has its own strides for
  *                            the two (elements; 0 repeats it).  a: M rows of K bytes, lda apart; b: N rows, ldb apart; addresses, lda, ldb and
  *                            the strides of a and b are multiples of 16 bytes, and a row is READ up to K rounded up to 16 (what stands behind
  *                            K does not count).  out: ldo elements from row to row; not a, b or a scale.

@@ -400,3 +400,57 @@ def test_streaming_form_leaves_the_rest_alone():
         check(view.contiguous(), product(a, sa / 4096, b, sb), kind)
         view.fill_(7.0)
         assert bool((room == 7.0).all())
+
+
+def test_too_many_places_are_refused():
+    """One pixel wide and 2^28 - 1 high: more places than 2^30, in the tiled order.  No GPU is touched."""
+    lib = hip.lib()
+    assert lib.bflow_i8_quantize_pixels(256, None, None, 0, 1, 16, (1 << 28) - 1, 1, 1, 256, 256, None) < 0
+    assert b"places" in lib.bflow_last_error_string()
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("k", [70, 256, 1000])
+def test_rows_have_the_same_bits_alone_and_together(k, kind):
+    """Every kernel adds whole numbers and applies the scales in one order: a token's row does not depend on the batch it stands in."""
+    (a, sa), (b, sb) = rows(600, k, 1), rows(520, k, 2)
+    a, sa, b, sb = (t.to(DEV) for t in (a, sa, b, sb))
+    whole = int8.matmul(a, sa, b, sb, kind, 0.37)
+    for at, n in ((0, 1), (5, 17), (100, 33), (599, 1), (64, 300)):
+        assert torch.equal(int8.matmul(a[at:at + n], sa[at:at + n], b, sb, kind, 0.37), whole[at:at + n])
+        if at + n <= 520:
+            assert torch.equal(int8.matmul(a, sa, b[at:at + n], sb[at:at + n], kind, 0.37), whole[:, at:at + n])
+
+
+@gpu
+def test_quantise_and_multiply_beside_another_stream():
+    """Quantisation and products of two streams at once, and twice in one captured graph, as layers behind one another use them."""
+    g = torch.Generator().manual_seed(3)
+    xs, ws = [torch.randn(n, 200, generator=g).to(DEV) for n in (1, 70, 400)], [torch.randn(200, 200, generator=g).to(DEV) for _ in range(2)]
+    qs = [int8.quantize_rows(w) for w in ws]
+
+    def layers(x):
+        for q, s in qs:
+            x = int8.matmul(*int8.quantize_rows(x), q, s, alpha=1 / 14)
+        return x
+    want = [layers(x) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = []
+    for x, st in zip(xs, streams):
+        with torch.cuda.stream(st):
+            got.append([layers(x) for _ in range(4)])
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, w) for ys, w in zip(got, want) for y in ys)
+    static = [x.clone() for x in xs]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = [layers(x) for x in static]
+    for flip in (False, True, False):
+        for s, x in zip(static, xs):
+            s.copy_(-x if flip else x)
+        graph.replay()
+        layers(xs[1])
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, layers(s)) for y, s in zip(out, static))

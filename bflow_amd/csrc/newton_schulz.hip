@@ -1002,9 +1002,9 @@ __global__ __launch_bounds__(PANEL_THREADS, 2) void ns_panel_square_kernel(Panel
 // worse than 32 bits (X is held to 2^-23, and few terms average).
 // v_mfma_f64_16x16x4: lane l holds row l % 16, k = l / 16 of the left operand, column l % 16 of the right one, and rows l / 16 + 4 e of the result.
 constexpr int TINY_ROWS = 32, TINY_THREADS = 512, TINY_LD = 33;
-// Numbers of a matrix: one workgroup reads them twice, in front of the panels of the list's other matrices (2 x 2: 9 us, 16 x 512 and 32 x 256: 13 and 17
+// Numbers of a matrix: one workgroup reads them twice, in front of the panels of the list's other matrices (2 x 2: 10 us, 16 x 512 and 32 x 256: 13 and 17
 // us, 32 x 640 31 us -- the panels take 13 us a step and any number of matrices).  More of them with 8 rows and less, where pairs would be worse than
-// 32 bits (2 x 1152: by a quarter) and a thread a column is quick (4 x 2304: 13 us, 8 x 8000 37, 2 x 60000 86).
+// 32 bits (2 x 1152: by a quarter) and a thread a column is quick (4 x 2304: 13 us, in the step 17; 8 x 8000 40, 2 x 60000 85).
 constexpr int TINY_FEW = 8;
 constexpr long long TINY_NUMBERS = 1 << 13, TINY_NUMBERS_FEW = 1 << 17;
 typedef double f64x4 __attribute__((ext_vector_type(4)));
@@ -1037,32 +1037,40 @@ __device__ __forceinline__ void tiny_body(const bflow_ns_matrix_t& m, const Tiny
     const bool tall = m.rows > m.cols;
     const int r = tall ? m.cols : m.rows, s = tall ? m.rows : m.cols;
     const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // (i, j) of the r x s matrix, zero outside.  No branch around the loads: those outside read the last element inside, and all of a batch are in
-    // flight together.
-    auto number = [&](int i, int j, bool update) -> float {
-        const bool inside = i < r && j < s;
+    // (i, j) of the r x s matrix, zero outside.  No branch around the loads, those outside read the last element inside; and they stand in front of all
+    // stores of their batch, so that the whole batch is in flight together.
+    struct Raw { float x, v; };
+    auto read = [&](int i, int j) -> Raw {
         const int ic = min(i, r - 1), jc = min(j, s - 1), row = tall ? jc : ic, col = tall ? ic : jc;
         const float x = load1<DT>(m.src, (long long)row * m.src_ld + col);
-        if constexpr (!STEP) return inside ? x : 0.f;
-        float* at = m.momentum + (long long)row * m.cols + col;
-        float v = *at;
+        if constexpr (!STEP) return {x, 0.f};
+        else return {x, m.momentum[(long long)row * m.cols + col]};
+    };
+    auto number = [&](Raw n, int i, int j, bool update) -> float {
+        const bool inside = i < r && j < s;
+        if constexpr (!STEP) return inside ? n.x : 0.f;
         if (update) {
-            v = fmaf(nu.mu, v, x);
-            if (inside) *at = v;
+            n.v = fmaf(nu.mu, n.v, n.x);
+            if (inside) m.momentum[tall ? (long long)j * m.cols + i : (long long)i * m.cols + j] = n.v;
         }
-        return !inside ? 0.f : nu.nesterov ? fmaf(nu.mu, v, x) : v;
+        return !inside ? 0.f : nu.nesterov ? fmaf(nu.mu, n.v, n.x) : n.v;
     };
     if constexpr (NV > 0) {
-        constexpr int PAIRS = NV * (NV + 1) / 2, TOGETHER = 8 / NV;
+        constexpr int PAIRS = NV * (NV + 1) / 2, TOGETHER = NV == 4 ? 4 : 2;
         double acc[PAIRS];
 #pragma unroll
         for (int n = 0; n < PAIRS; ++n) acc[n] = 0;
         for (int j = threadIdx.x; j < s; j += TOGETHER * TINY_THREADS) {
+            Raw raw[TOGETHER][NV];
             float x[TOGETHER][NV];
 #pragma unroll
             for (int u = 0; u < TOGETHER; ++u)
 #pragma unroll
-                for (int i = 0; i < NV; ++i) x[u][i] = number(i, j + u * TINY_THREADS, true);
+                for (int i = 0; i < NV; ++i) raw[u][i] = read(i, j + u * TINY_THREADS);
+#pragma unroll
+            for (int u = 0; u < TOGETHER; ++u)
+#pragma unroll
+                for (int i = 0; i < NV; ++i) x[u][i] = number(raw[u][i], i, j + u * TINY_THREADS, true);
 #pragma unroll
             for (int u = 0; u < TOGETHER; ++u)
 #pragma unroll
@@ -1090,13 +1098,20 @@ __device__ __forceinline__ void tiny_body(const bflow_ns_matrix_t& m, const Tiny
         // S = X X^T, before the norm is known; AHEAD blocks of 16 columns are read together
         f64x4 acc[3] = {{0., 0., 0., 0.}, {0., 0., 0., 0.}, {0., 0., 0., 0.}};
         for (int c0 = w * 16; c0 < s; c0 += AHEAD * WAVES * 16) {
+            Raw raw[AHEAD][NT][4];
             float x[AHEAD][NT][4];
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[u][n][e] = number(n * 16 + l15, c0 + u * WAVES * 16 + g * 4 + e, true);
+                    for (int e = 0; e < 4; ++e) raw[u][n][e] = read(n * 16 + l15, c0 + u * WAVES * 16 + g * 4 + e);
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[u][n][e] = number(raw[u][n][e], n * 16 + l15, c0 + u * WAVES * 16 + g * 4 + e, true);
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
@@ -1162,23 +1177,35 @@ __device__ __forceinline__ void tiny_body(const bflow_ns_matrix_t& m, const Tiny
     // the last X
     const float lr = STEP ? (nu.lr_device ? *nu.lr_device : nu.lr) : 0.f, keep = 1.f - lr * nu.decay, rate = lr * 0.2f * sqrtf((float)s);
     if constexpr (NV > 0) {
-        for (int j = threadIdx.x; j < s; j += TINY_THREADS) {
-            float x[NV], old[NV];
+        constexpr int TOGETHER = NV == 4 ? 4 : 2;
+        for (int j0 = threadIdx.x; j0 < s; j0 += TOGETHER * TINY_THREADS) {
+            Raw raw[TOGETHER][NV];
+            float old[TOGETHER][NV];
+            auto place = [&](int i, int j) { return tall ? (long long)j * m.dst_ld + i : (long long)i * m.dst_ld + j; };
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                x[i] = number(i, j, false);
-                if constexpr (STEP) old[i] = ((const float*)m.dst)[tall ? (long long)j * m.dst_ld + min(i, r - 1) : (long long)min(i, r - 1) * m.dst_ld + j];
-            }
+            for (int u = 0; u < TOGETHER; ++u)
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                double d = 0;
+                for (int i = 0; i < NV; ++i) {
+                    const int j = j0 + u * TINY_THREADS;
+                    raw[u][i] = read(i, j);
+                    if constexpr (STEP) old[u][i] = ((const float*)m.dst)[place(min(i, r - 1), min(j, s - 1))];
+                }
 #pragma unroll
-                for (int k = 0; k < NV; ++k) d = fma(Q[i * TINY_LD + k], (double)x[k], d);
-                if (i >= r) continue;
-                const float v = (float)(d * scale);
-                const long long to = tall ? (long long)j * m.dst_ld + i : (long long)i * m.dst_ld + j;
-                if constexpr (STEP) ((float*)m.dst)[to] = fmaf(-rate, v, old[i] * keep);
-                else store1<DT>(m.dst, to, v);
+            for (int u = 0; u < TOGETHER; ++u) {
+                const int j = j0 + u * TINY_THREADS;
+                double x[NV];
+#pragma unroll
+                for (int i = 0; i < NV; ++i) x[i] = number(raw[u][i], i, j, false);
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    double d = 0;
+#pragma unroll
+                    for (int k = 0; k < NV; ++k) d = fma(Q[i * TINY_LD + k], x[k], d);
+                    if (i >= r || j >= s) continue;
+                    const float v = (float)(d * scale);
+                    if constexpr (STEP) ((float*)m.dst)[place(i, j)] = fmaf(-rate, v, old[u][i] * keep);
+                    else store1<DT>(m.dst, place(i, j), v);
+                }
             }
         }
     } else {
@@ -1192,7 +1219,7 @@ __device__ __forceinline__ void tiny_body(const bflow_ns_matrix_t& m, const Tiny
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
-                for (int k = 0; k < R / 4; ++k) x[u][k] = number(4 * k + g, c0 + u * WAVES * 16 + l15, false);
+                for (int k = 0; k < R / 4; ++k) x[u][k] = number(read(4 * k + g, c0 + u * WAVES * 16 + l15), 4 * k + g, c0 + u * WAVES * 16 + l15, false);
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
                 const int j = c0 + u * WAVES * 16 + l15;

@@ -153,13 +153,12 @@ template <int BN> struct Turn {
 };
 
 // ------------------------------------------------------------------------------------------------------------------------------ entry
-// What enters the iteration at element (i, j) of the user's matrix; `update`: the step's momentum is brought up to date.
+// What enters the iteration at an element of the user's matrix, the step's momentum being up to date.
 template <int DT, bool STEP>
-__device__ __forceinline__ float entering(const Entry& m, long long from, long long dense, float mu, bool nesterov, bool update) {
+__device__ __forceinline__ float entering(const Entry& m, long long from, long long dense, float mu, bool nesterov) {
     const float g = load1<DT>(m.src, from);
     if constexpr (!STEP) return g;
-    float v = m.momentum[dense];
-    if (update) { v = fmaf(mu, v, g); m.momentum[dense] = v; }
+    const float v = m.momentum[dense];
     return nesterov ? fmaf(mu, v, g) : v;
 }
 
@@ -173,11 +172,26 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(Entries t, char* ws, float
     const bool dense = m.ld == cols;
     const unsigned n = (unsigned)m.r * (unsigned)m.s, first = (blockIdx.x - m.tile0) * (unsigned)m.per, last = min(first + (unsigned)m.per, n);   // n <= 2^30
     double sum = 0;
-#pragma unroll 8
-    for (unsigned e = first + threadIdx.x; e < last; e += 256) {
-        const long long from = dense ? (long long)e : (long long)(e / cols) * m.ld + e % cols;
-        const float u = entering<DT, STEP>(m, from, e, mu, nesterov, true);
-        sum += (double)u * (double)u;
+    constexpr int TOGETHER = 8;                         // loads in front of the stores, which would hold them back
+    for (unsigned e0 = first + threadIdx.x; e0 < last; e0 += 256 * TOGETHER) {
+        float g[TOGETHER], v[TOGETHER];
+#pragma unroll
+        for (int u = 0; u < TOGETHER; ++u) {
+            const unsigned e = min(e0 + 256 * u, last - 1);
+            g[u] = load1<DT>(m.src, dense ? (long long)e : (long long)(e / cols) * m.ld + e % cols);
+            if constexpr (STEP) v[u] = m.momentum[e];
+        }
+#pragma unroll
+        for (int u = 0; u < TOGETHER; ++u) {
+            if (e0 + 256 * u >= last) break;
+            float x = g[u];
+            if constexpr (STEP) {
+                const float now = fmaf(mu, v[u], x);
+                m.momentum[e0 + 256 * u] = now;
+                x = nesterov ? fmaf(mu, now, x) : now;
+            }
+            sum += (double)x * (double)x;
+        }
     }
     sum = wave_sum(sum);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
@@ -201,7 +215,7 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(Entries t, char* ws, float
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
         const int i = i0 + slow + 4 * e, j = j0 + fast;
-        v[e] = i < rows && j < cols ? entering<DT, STEP>(m, (long long)i * m.ld + j, (long long)i * cols + j, mu, nesterov, false) : 0.f;
+        v[e] = i < rows && j < cols ? entering<DT, STEP>(m, (long long)i * m.ld + j, (long long)i * cols + j, mu, nesterov) : 0.f;
     }
     const int parts = (int)(((long long)m.r * m.s + m.per - 1) / m.per);
     double sum = 0;

@@ -281,9 +281,14 @@ struct Product {
         return (lane >> 3) * ld + (seg >> 2) * CHUNK + (seg & 3) * 16;
     }
 
-    // Leaves KG tiles in LDS (Turn order); the workgroup is synchronised.  a, b: descriptors of the tile's rows, `columns` (a multiple of 64) long.
-    __device__ static __forceinline__ void run(rsrc_t a, int lda, rsrc_t b, int ldb, int columns, char* lds) {
-        const int chunks = columns / COLUMNS;
+    // rounds of a contraction over `columns`, a multiple of 64: each group of waves takes a chunk in each
+    __host__ __device__ static inline int rounds_of(int columns) { return (columns / COLUMNS + KG - 1) / KG; }
+
+    // Leaves KG tiles in LDS (Turn order); the workgroup is synchronised.  a, b: descriptors of the tile's rows, `columns` (a multiple of 64) long;
+    // rounds first .. last of them.
+    __device__ static __forceinline__ void run(rsrc_t a, int lda, rsrc_t b, int ldb, int columns, char* lds) { run(a, lda, b, ldb, columns, lds, 0, rounds_of(columns)); }
+    __device__ static __forceinline__ void run(rsrc_t a, int lda, rsrc_t b, int ldb, int columns, char* lds, int first, int last) {
+        const int chunks = min(columns / COLUMNS, last * KG);
         const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = w / WAVES, wave = w % WAVES;
         const int wm = wave / ACROSS, wn = wave % ACROSS;
         const int va = source(lane, lda, wave), vb = source(lane, ldb, wave);
@@ -294,10 +299,10 @@ struct Product {
             for (int j = 0; j < NT; ++j)
 #pragma unroll
                 for (int k = 0; k < 16; ++k) { hh[i][j][k] = 0.f; xx[i][j][k] = 0.f; }
-        const int rounds = (chunks + KG - 1) / KG;
+        const int rounds = last - first;
         auto issue = [&](int round) {
             char* stage = lds + (round % STAGES) * STAGE + group * CHUNK_BYTES;
-            const int c = round * KG + group;
+            const int c = (first + round) * KG + group;
             const bool there = c < chunks;                           // behind the last chunk: zeros
             const int at = there ? c * COLUMNS * 4 : 0;
 #pragma unroll
@@ -431,19 +436,13 @@ struct Product {
     };
 };
 
-// Tile t of those that touch the lower triangle, band of BM rows by band; `down` = bands.
-template <class P> __host__ __device__ inline int tiles_of_band(int i, int R) { const int n = ((i + 1) * P::BM + P::BN - 1) / P::BN, all = (R + P::BN - 1) / P::BN; return n < all ? n : all; }
-template <class P> __host__ inline int lower_tiles(int R) {
-    int n = 0;
-    for (int i = 0; i * P::BM < R; ++i) n += tiles_of_band<P>(i, R);
-    return n;
-}
+template <class P> __host__ __device__ inline int lower_tiles(int R) { const int down = (R + P::BM - 1) / P::BM; return down * (down + 1) / 2; }
 // Tile t of a lower triangle, bands of BAND rows of tiles, each walked column by column; an XCD (workgroups go round them) takes an eighth of that walk, so
 // that what it works on at one time shares rows: 4096 x 4096 from the hi halves 189 -> 149 us (traffic through the L2s bounds it; in pairs as before).
 constexpr int BAND = 8;
 template <class P> __device__ __forceinline__ void lower(int t, int R, int& r0, int& c0) {
     static_assert(P::BM == P::BN, "square tiles");
-    const int down = (R + P::BM - 1) / P::BM, total = down * (down + 1) / 2;
+    const int down = (R + P::BM - 1) / P::BM, total = lower_tiles<P>(R);
     const int x = t & 7, at = x * (total >> 3) + min(x, total & 7) + (t >> 3);
     int band = 0;
     while ((band + BAND) * (band + BAND + 1) / 2 <= at) band += BAND;        // rows in front of the band
@@ -465,17 +464,35 @@ template <class P> __device__ __forceinline__ void lower(int t, int R, int& r0, 
 __device__ __forceinline__ bool mine(int row, int col) { return row >> 6 >= col >> 6; }
 __device__ __forceinline__ bool mirrored(int row, int col) { return row >> 6 > col >> 6; }
 
+// The tail of a launch: a tile of the large set takes a CU alone, so 528 of them (4096 rows) are two rounds of 256 and one of 16.  Tiles from `whole` on
+// are cut along the contraction into `parts` workgroups each, which leave 32-bit sums in `room`, and ns_join_kernel adds them in their order.  Whole
+// tiles keep their common walk along the contraction; dealing all of it out evenly lost that, and with it the L2 (189 -> 232 us).
+struct Tail { int whole, parts; float* room; };
+// This workgroup's tile, and its part of n rounds; false: a whole tile.
+__device__ __forceinline__ bool cut_tile(const Tail& l, int wg, int& tile, int& part) {
+    part = 0;
+    tile = wg;
+    if (wg < l.whole) return false;
+    tile = l.whole + (wg - l.whole) / l.parts;
+    part = (wg - l.whole) % l.parts;
+    return true;
+}
+template <class P> __device__ __forceinline__ void leave_part(const Tail& l, int wg, const char* lds) {
+    float* to = l.room + (long long)(wg - l.whole) * P::BM * P::BN;
+#pragma unroll
+    for (int i = 0; i < P::ITEMS; ++i) {
+        int row, col;
+        if (!P::row_piece(i, row, col)) continue;
+        float v[8];
+        P::sum8(lds, row, col, v);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) *reinterpret_cast<float4*>(to + row * P::BN + col + 4 * h) = make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
+    }
+}
+
 // A = X X^T as pairs, both triangles.
-template <class P>
-__global__ __launch_bounds__(P::THREADS, 2) void ns_gram_kernel(Works t, char* ws) {
-    extern __shared__ __attribute__((aligned(1024))) char lds[];
-    const int k = find(t.m, t.count, blockIdx.x);
-    const Work m = t.m[k];
-    const int R = up64(m.r), S = up64(m.s), ld = S * 4;
-    int r0, c0;
-    lower<P>(blockIdx.x - m.tile0, R, r0, c0);
-    const char* x = ws + x_at(m.off);
-    P::run(rows_rsrc(x + (long long)r0 * ld, min(P::BM, R - r0), ld, ld), ld, rows_rsrc(x + (long long)c0 * ld, min(P::BN, R - c0), ld, ld), ld, S, lds);
+template <class P> __device__ __forceinline__ void gram_out(const Work& m, char* ws, int r0, int c0, char* lds) {
+    const int R = up64(m.r);
     const float scale = ldexpf(SA, -2 * m.ex);
     _Float16* a = (_Float16*)(ws + a_at(m.off, m.r, m.s));
     P::rows(lds, [&](int, int, int, float v[8]) {
@@ -490,20 +507,25 @@ __global__ __launch_bounds__(P::THREADS, 2) void ns_gram_kernel(Works t, char* w
         if (r0 + row < R && c0 + col < R && mirrored(r0 + row, c0 + col)) put8(a, at(c0 + col, r0 + row, R), h, l);
     });
 }
+template <class P>
+__global__ __launch_bounds__(P::THREADS, 2) void ns_gram_kernel(Works t, Tail l, char* ws) {
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    int tile, part, r0, c0;
+    const bool cut = cut_tile(l, blockIdx.x, tile, part);
+    const int k = find(t.m, t.count, tile);
+    const Work m = t.m[k];
+    const int R = up64(m.r), S = up64(m.s), ld = S * 4, n = P::rounds_of(S);
+    lower<P>(tile - m.tile0, R, r0, c0);
+    const char* x = ws + x_at(m.off);
+    P::run(rows_rsrc(x + (long long)r0 * ld, min(P::BM, R - r0), ld, ld), ld, rows_rsrc(x + (long long)c0 * ld, min(P::BN, R - c0), ld, ld), ld, S, lds,
+           cut ? (int)((long long)n * part / l.parts) : 0, cut ? (int)((long long)n * (part + 1) / l.parts) : n);
+    if (cut) leave_part<P>(l, blockIdx.x, lds);
+    else gram_out<P>(m, ws, r0, c0, lds);
+}
 
 // B = b A + c A^2, both triangles.
-template <class P>
-__global__ __launch_bounds__(P::THREADS, 2) void ns_poly_kernel(Works t, char* ws, float b, float c, int drop) {
-    extern __shared__ __attribute__((aligned(1024))) char lds[];
-    const int k = find(t.m, t.count, blockIdx.x);
-    const Work m = t.m[k];
-    const int R = up64(m.r), ld = R * 4;
-    int r0, c0;
-    lower<P>(blockIdx.x - m.tile0, R, r0, c0);
-    const char* a = ws + a_at(m.off, m.r, m.s);
-    typename P::Ahead av;
-    av.load((const _Float16*)a, r0, c0, R, R);
-    P::run(rows_rsrc(a + (long long)r0 * ld, min(P::BM, R - r0), ld, ld), ld, rows_rsrc(a + (long long)c0 * ld, min(P::BN, R - c0), ld, ld), ld, R, lds);
+template <class P> __device__ __forceinline__ void poly_out(const Work& m, char* ws, int r0, int c0, char* lds, const typename P::Ahead& av, float b, float c, int drop) {
+    const int R = up64(m.r);
     _Float16* out = (_Float16*)(ws + b_at(m.off, m.r, m.s));
     const float fb = b * (SB / SA), fc = ldexpf(c * (SB / (SA * SA)), -2 * g_of(ws, m.off, drop));
     P::rows(lds, [&](int n, int, int, float v[8]) {
@@ -517,6 +539,69 @@ __global__ __launch_bounds__(P::THREADS, 2) void ns_poly_kernel(Works t, char* w
     P::columns(lds, [&](int row, int col, half8 h, half8 l) {
         if (r0 + row < R && c0 + col < R && mirrored(r0 + row, c0 + col)) put8(out, at(c0 + col, r0 + row, R), h, l);
     });
+}
+template <class P>
+__global__ __launch_bounds__(P::THREADS, 2) void ns_poly_kernel(Works t, Tail l, char* ws, float b, float c, int drop) {
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    int tile, part, r0, c0;
+    const bool cut = cut_tile(l, blockIdx.x, tile, part);
+    const int k = find(t.m, t.count, tile);
+    const Work m = t.m[k];
+    const int R = up64(m.r), ld = R * 4, n = P::rounds_of(R);
+    lower<P>(tile - m.tile0, R, r0, c0);
+    const char* a = ws + a_at(m.off, m.r, m.s);
+    typename P::Ahead av;
+    av.load((const _Float16*)a, r0, c0, R, R);
+    P::run(rows_rsrc(a + (long long)r0 * ld, min(P::BM, R - r0), ld, ld), ld, rows_rsrc(a + (long long)c0 * ld, min(P::BN, R - c0), ld, ld), ld, R, lds,
+           cut ? (int)((long long)n * part / l.parts) : 0, cut ? (int)((long long)n * (part + 1) / l.parts) : n);
+    if (cut) leave_part<P>(l, blockIdx.x, lds);
+    else poly_out<P>(m, ws, r0, c0, lds, av, b, c, drop);
+}
+
+// The tail's tiles, 64 x 64 of one a workgroup: the parts added, then what the product does with a tile.
+enum { GRAM = 0, POLY = 1 };
+template <class P, int WHAT>
+__global__ __launch_bounds__(256) void ns_join_kernel(Works t, Tail l, char* ws, float b, float c, int drop) {
+    typedef Product<64, 64, 32, 32, 1, 2> J;
+    static_assert(J::THREADS == 256, "as launched");
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    constexpr int DOWN = P::BM / 64, ACROSS = P::BN / 64;
+    const int in = blockIdx.x % (DOWN * ACROSS), rank = blockIdx.x / (DOWN * ACROSS), tile = l.whole + rank, dr = in / ACROSS * 64, dc = in % ACROSS * 64;
+    const int k = find(t.m, t.count, tile);
+    const Work m = t.m[k];
+    const int R = up64(m.r);
+    int r0, c0;
+    lower<P>(tile - m.tile0, R, r0, c0);
+    if (r0 + dr >= R || c0 + dc > r0 + dr) return;      // outside, or above the diagonal
+    typename J::Ahead av;
+    if (WHAT == POLY) av.load((const _Float16*)(ws + a_at(m.off, m.r, m.s)), r0 + dr, c0 + dc, R, R);
+    const float* from = l.room + (long long)rank * l.parts * P::BM * P::BN + dr * P::BN + dc;
+    float v[J::ITEMS][8];
+#pragma unroll
+    for (int i = 0; i < J::ITEMS; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
+#pragma unroll 4
+    for (int n = 0; n < l.parts; ++n)
+#pragma unroll
+        for (int i = 0; i < J::ITEMS; ++i) {
+            int row, col;
+            J::row_piece(i, row, col);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float4 y = *reinterpret_cast<const float4*>(from + (long long)n * P::BM * P::BN + row * P::BN + col + 4 * h);
+                v[i][4 * h] += y.x; v[i][4 * h + 1] += y.y; v[i][4 * h + 2] += y.z; v[i][4 * h + 3] += y.w;
+            }
+        }
+#pragma unroll
+    for (int i = 0; i < J::ITEMS; ++i) {
+        int row, col;
+        J::row_piece(i, row, col);
+        J::T::put_row8((float*)lds, row, col, v[i]);
+    }
+    __syncthreads();
+    if (WHAT == GRAM) gram_out<J>(m, ws, r0 + dr, c0 + dc, lds);
+    else poly_out<J>(m, ws, r0 + dr, c0 + dc, lds, av, b, c, drop);
 }
 
 // X <- a X + B X, by rows (in place: a tile reads and writes its own part alone) and by columns (from one Xt to the other).
@@ -1304,7 +1389,7 @@ struct SmallSet {
     typedef Product<64, 128, 32, 32, 1, 3> Panel;      // X
 };
 struct LargeSet {
-    typedef Product<128, 128, 64, 64, 2, 2> Square;
+    typedef Product<128, 128, 64, 64, 2, 2> Square;    // (a CU alone)
     typedef Product<128, 128, 64, 64, 1, 2> Panel;
 };
 
@@ -1314,6 +1399,8 @@ struct Plan {
     Exits leave;
     long long tiles_square, tiles_panel, tiles_sum, tiles_norm, tiles_pack, bytes;
     bool large;
+    int whole, cut_parts;  // tiles of a square product that are not cut; parts of those behind them (0: none)
+    long long room;        // where the parts stand
     bool panels;           // every matrix of at most PANEL_ROWS rows: `works` instead of `square` and `panel`
     PanelWorks works;
     int lds_panel, lds_square;
@@ -1415,6 +1502,28 @@ bool lay_out(const bflow_ns_matrix_t* m, int count, Plan& p) {
     p.large = blocks >= LARGE_BLOCKS;
     if (p.large) lay_out_products<LargeSet>(p);
     else lay_out_products<SmallSet>(p);
+    // The last tiles, where they leave half of the CUs idle or more; each part has CUT_ROUNDS rounds at least.  Calls without and with it: 2944 x 2944 in fp32
+    // 2255 / 1985 us, 4096 x 4096 4495 / 4075 (bf16 3910 / 3620), 8 of 1024 x 1024 892 / 856, 8192 x 8192 31.7 / 31.0 ms.  (Two rounds at least: 24 of 640 x
+    // 640 893 / 937; eight: 2944 x 2944 2079.)
+    constexpr int CUS = 256, CUT_ROUNDS = 4;
+    p.whole = (int)p.tiles_square;
+    p.cut_parts = 0;
+    p.room = off;
+    if (p.large && p.tiles_square > CUS) {
+        const int last = (int)(p.tiles_square % CUS);
+        int shortest = 1 << 30;
+        for (int i = 0, seen = 0; i < count; ++i) {
+            const int R = up64(p.square.m[i].r);
+            seen += lower_tiles<LargeSet::Square>(R);
+            if (seen > p.tiles_square - last) shortest = std::min(shortest, LargeSet::Square::Halves::rounds_of(R));      // (R <= S: of either product, in either form)
+        }
+        const int parts = last ? std::min(CUS / last, shortest / CUT_ROUNDS) : 0;
+        if (parts > 1) {
+            p.whole -= last;
+            p.cut_parts = parts;
+            off += (long long)last * parts * LargeSet::Square::TILE;
+        }
+    }
     p.bytes = off;
     return p.tiles_pack < (1LL << 30);
 }
@@ -1472,11 +1581,15 @@ int launch_products(const Plan& p, int steps, float a, float b, float c, double 
     const auto leave = ns_leave_kernel<P, DT, STEP>;
     for (const int rc : {allow_lds(gram, G::LDS), allow_lds(poly, Q::LDS), allow_lds(apply, P::LDS), allow_lds(leave, P::LDS)})
         if (rc) return rc;
+    const Tail tail = {p.whole, p.cut_parts, (float*)(ws + p.room)};
+    const int cut = (int)p.tiles_square - p.whole, squares = p.whole + cut * p.cut_parts, joins = cut * (Q::BM / 64) * (Q::BN / 64);
     const double bits = log2(gain);
     for (int k = 0; k < steps; ++k) {
         const int drop = (int)std::ceil(k * bits), next = (int)std::ceil((k + 1) * bits);
-        hipLaunchKernelGGL(gram, dim3(p.tiles_square), dim3(G::THREADS), G::LDS, st, p.square, ws);
-        hipLaunchKernelGGL(poly, dim3(p.tiles_square), dim3(Q::THREADS), Q::LDS, st, p.square, ws, b, c, drop);
+        hipLaunchKernelGGL(gram, dim3(squares), dim3(G::THREADS), G::LDS, st, p.square, tail, ws);
+        if (cut) hipLaunchKernelGGL((ns_join_kernel<Q, GRAM>), dim3(joins), dim3(256), 64 * 64 * 4, st, p.square, tail, ws, b, c, drop);
+        hipLaunchKernelGGL(poly, dim3(squares), dim3(Q::THREADS), Q::LDS, st, p.square, tail, ws, b, c, drop);
+        if (cut) hipLaunchKernelGGL((ns_join_kernel<Q, POLY>), dim3(joins), dim3(256), 64 * 64 * 4, st, p.square, tail, ws, b, c, drop);
         if (k + 1 < steps) hipLaunchKernelGGL(apply, dim3(p.tiles_panel), dim3(P::THREADS), P::LDS, st, p.panel, ws, k & 1, a, drop, next);
         else hipLaunchKernelGGL(leave, dim3(p.tiles_panel), dim3(P::THREADS), P::LDS, st, p.leave, ws, k & 1, a, drop, lr, lr_device, decay);
     }

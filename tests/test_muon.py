@@ -292,6 +292,35 @@ def test_on_another_stream_and_in_a_graph():
         assert all(torch.equal(p, q) for p, q in zip(out, want))
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shapes", [[(2900, 2950)], [(1000, 1020)] * 8, [(70, 3000)] + [(1000, 1020)] * 8], ids=["one", "eight", "nine"])
+def test_last_tiles_cut_along_the_contraction(shapes, dtype):
+    """276, 288 and 289 tiles of 128 x 128: those behind the 256th are cut.  Against 64 bits on the device, in front of and behind other calls; twice the same
+    bits; and through a step."""
+    xs = [gradient(*s, seed=k).to(dtype).to(DEV) for k, s in enumerate(shapes)]
+
+    def exact(x):
+        a, b, c = muon.COEFFICIENTS
+        y = x.double() / (x.double().norm() + 1e-7)
+        for _ in range(5):
+            g = y @ y.t()
+            y = a * y + (b * g + c * g @ g) @ y
+        return y
+    ys = muon.orthogonalize(xs)
+    muon.orthogonalize([xs[-1][:300, :310]])
+    assert all(torch.equal(y, z) for y, z in zip(ys, muon.orthogonalize(xs)))
+    for x, y in zip(xs, ys):
+        assert off(y, exact(x).cpu()) < TOL[dtype]
+    if dtype is torch.float32:
+        ps = [torch.nn.Parameter(torch.zeros_like(x)) for x in xs]
+        for p, x in zip(ps, xs):
+            p.grad = x
+        muon.Muon(ps, lr=0.5, momentum=0.0).step()
+        for p, y in zip(ps, ys):
+            assert off(p, y.cpu() * (-0.1 * math.sqrt(max(y.shape)))) < 2.0 ** -22
+
+
 # ------------------------------------------------------------------------------------------------------------------------------- the step
 def plain_step(p, g, v, lr, decay, mu, nesterov, **kw):
     p, g, v = (t.detach().cpu().double() for t in (p, g, v))

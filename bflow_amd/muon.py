@@ -126,11 +126,14 @@ class Muon(torch.optim.Optimizer):
         super().add_param_group(group)
         group = self.param_groups[-1]
         for p in group["params"]:
+            why = None
             if p.dtype != torch.float32:
-                raise hip.BflowHipError(f"Muon: parameters are float32, got {p.dtype}")
-            if not group["adamw"] and (p.dim() < 2 or not p.is_contiguous()):
-                raise hip.BflowHipError(f"Muon: a parameter of shape {tuple(p.shape)}, strides {p.stride()}: dense matrices or filters; put the others into a "
-                                        "group with adamw=True")
+                why = f"parameters are float32, got {p.dtype}"
+            elif not group["adamw"] and (p.dim() < 2 or not p.is_contiguous()):
+                why = f"a parameter of shape {tuple(p.shape)}, strides {p.stride()}: dense matrices or filters; put the others into a group with adamw=True"
+            if why is not None:
+                self.param_groups.pop()
+                raise hip.BflowHipError(f"Muon: {why}")
 
     @torch.no_grad()
     def step(self, closure=None):

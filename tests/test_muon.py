@@ -109,6 +109,9 @@ def test_optimizer_checks_its_arguments():
     with pytest.raises(hip.BflowHipError, match="float32"):
         muon.Muon([torch.nn.Parameter(torch.zeros(4, 4, dtype=torch.float16))])
     opt = muon.Muon([{"params": [w]}, {"params": [torch.nn.Parameter(torch.zeros(4))], "adamw": True}])
+    with pytest.raises(hip.BflowHipError, match="adamw=True"):       # a refused group is not kept
+        opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(3))]})
+    assert len(opt.param_groups) == 2
     opt.step()                                                       # no gradients: nothing to do, on any device
     w.grad = torch.zeros(4, 4)
     with pytest.raises(hip.BflowHipError, match="no CPU fallback"):

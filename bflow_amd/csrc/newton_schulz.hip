@@ -203,7 +203,7 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(Entries t, char* ws, float
 // X and (`both`) Xt of a 64 x 64 tile, scaled to sx / (|X| + eps), zeros in the padding.  Bound by memory: the same 12.6 million numbers (8 bytes in, 8
 // out each) 43 us, 4.7 TB/s; a list of small ones by its latency (a network's filters, 5.3 million numbers: 20 us).
 template <int DT, bool STEP>
-__global__ __launch_bounds__(256) void ns_pack_kernel(Entries t, char* ws, float mu, int nesterov, float eps, int both) {
+__global__ __launch_bounds__(256) void ns_pack_kernel(Entries t, char* ws, float mu, int nesterov, double eps, int both) {
     __shared__ double part[4];
     __shared__ __attribute__((aligned(16))) float tile[64 * 64];
     const int k = find(t.m, t.count, blockIdx.x);
@@ -228,9 +228,9 @@ __global__ __launch_bounds__(256) void ns_pack_kernel(Entries t, char* ws, float
     sum = part[0] + part[1] + part[2] + part[3];
     const double norm = sqrt(sum);
     // (NaN and infinite norms: the comparison is false, g = 0)
-    const int g = norm > 0. && norm < (double)eps ? (int)log2((norm + (double)eps) / norm) : 0;
+    const int g = norm > 0. && norm < eps ? (int)log2((norm + eps) / norm) : 0;
     if (w == 0 && threadIdx.x == 0) *(int*)(ws + g_at(m.off)) = g;
-    const double scale = ldexp(1.0, m.ex + g) / (norm + (double)eps);
+    const double scale = ldexp(1.0, m.ex + g) / (norm + eps);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
         _Float16 h, l;
@@ -1276,7 +1276,10 @@ __device__ __forceinline__ void tiny_body(const bflow_ns_matrix_t& m, const Tiny
     for (int i = 0; i < R; ++i) trace += S[i * TINY_LD + i];
     const double scale = 1. / (sqrt(trace) + nu.eps);
     __syncthreads();
-    for (int i = threadIdx.x; i < R * R; i += TINY_THREADS) S[(i / R) * TINY_LD + i % R] *= scale * scale;
+    for (int i = threadIdx.x; i < R * R; i += TINY_THREADS) {
+        double& v = S[(i / R) * TINY_LD + i % R];
+        v = v * scale * scale;                          // (the square of 1 / eps may be infinite)
+    }
     __syncthreads();
     // four waves make P Q, four P S and then P S P
     const int tile = w & 3, ti = tile >> (NT - 1), tj = tile & (NT - 1);
@@ -1604,9 +1607,11 @@ int launch_products(const Plan& p, int steps, float a, float b, float c, double 
     for (int k = 0; k < steps; ++k) {
         const int drop = (int)std::ceil(k * bits), next = (int)std::ceil((k + 1) * bits);
         hipLaunchKernelGGL(gram, dim3(squares), dim3(G::THREADS), G::LDS, st, p.square, tail, ws);
-        if (cut) hipLaunchKernelGGL((ns_join_kernel<Q, GRAM>), dim3(joins), dim3(256), 64 * 64 * 4, st, p.square, tail, ws, b, c, drop);
+        if constexpr (std::is_same_v<Set, LargeSet>)
+            if (cut) hipLaunchKernelGGL((ns_join_kernel<Q, GRAM>), dim3(joins), dim3(256), 64 * 64 * 4, st, p.square, tail, ws, b, c, drop);
         hipLaunchKernelGGL(poly, dim3(squares), dim3(Q::THREADS), Q::LDS, st, p.square, tail, ws, b, c, drop);
-        if (cut) hipLaunchKernelGGL((ns_join_kernel<Q, POLY>), dim3(joins), dim3(256), 64 * 64 * 4, st, p.square, tail, ws, b, c, drop);
+        if constexpr (std::is_same_v<Set, LargeSet>)
+            if (cut) hipLaunchKernelGGL((ns_join_kernel<Q, POLY>), dim3(joins), dim3(256), 64 * 64 * 4, st, p.square, tail, ws, b, c, drop);
         if (k + 1 < steps) hipLaunchKernelGGL(apply, dim3(p.tiles_panel), dim3(P::THREADS), P::LDS, st, p.panel, ws, k & 1, a, drop, next);
         else hipLaunchKernelGGL(leave, dim3(p.tiles_panel), dim3(P::THREADS), P::LDS, st, p.leave, ws, k & 1, a, drop, lr, lr_device, decay);
     }
@@ -1636,7 +1641,7 @@ int launch_panels(const Plan& p, int steps, float a, float b, float c, double ga
 }
 
 template <int DT, bool STEP>
-int launch_all(const Plan& p, int steps, float a, float b, float c, float eps, double gain, char* ws, float mu, int nesterov, float lr, const float* lr_device, float decay,
+int launch_all(const Plan& p, int steps, float a, float b, float c, double eps, double gain, char* ws, float mu, int nesterov, float lr, const float* lr_device, float decay,
                hipStream_t st) {
     hipLaunchKernelGGL((ns_norm_kernel<DT, STEP>), dim3(p.tiles_norm), dim3(256), 0, st, p.norm, ws, mu, nesterov);
     hipLaunchKernelGGL((ns_pack_kernel<DT, STEP>), dim3(p.tiles_pack), dim3(256), 0, st, p.pack, ws, mu, nesterov, eps, (int)!p.panels);
@@ -1648,7 +1653,7 @@ int check(const bflow_ns_matrix_t* m, int count, int steps, double a, double b, 
     const char* why = bad(m, count);
     BFLOW_REQUIRE(!why, BFLOW_E_ARG, "newton_schulz: %s", why);
     BFLOW_REQUIRE(steps >= 1 && steps <= 32, BFLOW_E_ARG, "newton_schulz: %d steps (1 .. 32)", steps);
-    BFLOW_REQUIRE(eps > 0.f && eps < 1.f, BFLOW_E_ARG, "newton_schulz: eps %g outside (0, 1)", (double)eps);
+    BFLOW_REQUIRE(eps >= 1e-300 && eps < 1, BFLOW_E_ARG, "newton_schulz: eps %g outside [1e-300, 1)", eps);
     const double most = reach(steps, a, b, c, gain);
     BFLOW_REQUIRE(most <= 1.9 && std::fabs(b) * 4 + std::fabs(c) * 16 < 63, BFLOW_E_ARG,
                   "newton_schulz: coefficients (%g, %g, %g) take a singular value in [0, 1] to %g: the iterates must stay below 1.9", a, b, c, most);
@@ -1692,7 +1697,7 @@ int launch_list(const bflow_ns_matrix_t* m, int count, int steps, double a, doub
     return (int)for_groups(m, count, false, [&](const bflow_ns_matrix_t* group, int n) -> long long {
         static thread_local Plan p;
         lay_out(group, n, p);
-        return launch_all<DT, STEP>(p, steps, (float)a, (float)b, (float)c, (float)eps, gain, ws, mu, nesterov, lr, lr_device, decay, st);
+        return launch_all<DT, STEP>(p, steps, (float)a, (float)b, (float)c, eps, gain, ws, mu, nesterov, lr, lr_device, decay, st);
     });
 }
 }  // namespace

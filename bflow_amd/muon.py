@@ -47,8 +47,8 @@ def _check_numbers(steps: int, coefficients: Sequence[float], eps: float):
         raise hip.BflowHipError(f"coefficients: three numbers a, b, c, got {coefficients!r}")
     if int(steps) != steps or not 1 <= steps <= 32:
         raise hip.BflowHipError(f"steps: a whole number in 1 .. 32, got {steps!r}")
-    if not 0.0 < eps < 1.0:
-        raise hip.BflowHipError(f"eps: a number in (0, 1), got {eps!r}")
+    if not 1e-300 <= eps < 1.0:
+        raise hip.BflowHipError(f"eps: a number in [1e-300, 1), got {eps!r}")
 
 
 @torch.no_grad()

@@ -596,7 +596,7 @@ int bflow_l1_masked_grad(const float* src, const float* tgt, const unsigned char
  * stays zero.
  * ws: bflow_ns_workspace_bytes(m, count) bytes (rows and cols alone are read; 0 where all are small: ws may be NULL), aligned to 256, free for
  * other use once the call's launches ran: calls that may run at the same time need one each.
- * steps 1 .. 32, eps in (0, 1), |a x + b x^3 + c x^5| iterated from [0, 1] has to stay below 1.9 and 4 |b| + 16 |c| below 63.                    */
+ * steps 1 .. 32, eps in [1e-300, 1), |a x + b x^3 + c x^5| iterated from [0, 1] has to stay below 1.9 and 4 |b| + 16 |c| below 63.                    */
 #define BFLOW_NS_MAX_MATRICES 64          /* of one round of launches  */
 #define BFLOW_NS_MAX_SIDE     (1 << 20)   /* rows or cols of one matrix; 2^30 elements at most */
 typedef struct bflow_ns_matrix {

@@ -63,7 +63,7 @@ def test_refuses_what_it_cannot_take():
     for bad in (0, 33, 2.5):
         with pytest.raises(hip.BflowHipError, match="steps"):
             muon.orthogonalize([], steps=bad)
-    for bad in (0.0, 1.0, float("nan")):
+    for bad in (0.0, 1e-310, 1.0, float("nan")):
         with pytest.raises(hip.BflowHipError, match="eps"):
             muon.orthogonalize([], eps=bad)
     with pytest.raises(hip.BflowHipError, match="three"):
@@ -202,6 +202,16 @@ def test_zero_tiny_huge_and_lost_values():
     assert torch.isnan(ys[3]).all() and torch.isnan(ys[4]).all()
     assert off(ys[5], plain(rank1)) < RANK_ONE_TOL and off(ys[6], plain(one_row)) < F32_TOL      # (one row: the others hold no rounding either)
     assert not ys[6][:17].any() and not ys[6][18:].any()
+
+
+@gpu
+@pytest.mark.parametrize("eps", [1e-60, 1e-300])
+def test_eps_below_32_bits(eps):
+    """eps only has to keep zero matrices apart from 0 / 0, and may be smaller than a 32-bit number."""
+    xs = [gradient(40, 100, seed=1), gradient(300, 280, seed=2), gradient(6, 40, seed=3), torch.zeros(40, 100), torch.zeros(300, 280), torch.zeros(6, 40)]
+    for group in (xs, xs[:1] + xs[3:4]):
+        for x, y in zip(group, muon.orthogonalize([x.to(DEV) for x in group], eps=eps)):
+            assert off(y, plain(x, eps=eps)) < F32_TOL if x.any() else not y.any()
 
 
 @gpu

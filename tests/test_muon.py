@@ -334,6 +334,33 @@ def test_last_tiles_cut_along_the_contraction(shapes, dtype):
             assert off(p, y.cpu() * (-0.1 * math.sqrt(max(y.shape)))) < 2.0 ** -22
 
 
+@gpu
+@pytest.mark.parametrize("shape,dtype", [((1024, 1 << 20), torch.bfloat16), ((1 << 20, 200), torch.float32), ((8192, 100), torch.float16)], ids=["wide", "tall", "panels"])
+def test_longest_rows(shape, dtype):
+    """Byte offsets behind 2^32 in the workspace, 2^20 columns or rows, against 64 bits on the device: slices of the result, from the Gram matrix."""
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randn(shape, generator=g, device=DEV).to(dtype)
+    tall = shape[0] > shape[1]
+    (y,) = muon.orthogonalize([x])
+    wide, out = (x.t(), y.t()) if tall else (x, y)
+    S = torch.zeros(wide.shape[0], wide.shape[0], dtype=torch.float64, device=DEV)
+    for c in range(0, wide.shape[1], 1 << 16):
+        part = wide[:, c:c + (1 << 16)].double()
+        S += part @ part.t()
+    # every step is a polynomial of S; all singular values of these matrices are within a factor of two
+    norm, Q, eye = S.trace().sqrt() + 1e-7, None, torch.eye(S.shape[0], dtype=torch.float64, device=DEV)
+    S = S / norm ** 2
+    for _ in range(5):
+        a, b, c = muon.COEFFICIENTS
+        P = a * eye + b * S + c * S @ S
+        Q, S = P if Q is None else P @ Q, P @ S @ P
+    for c in (0, wide.shape[1] // 2 + 57, wide.shape[1] - 300):
+        want = (Q @ wide[:, c:c + 300].double() / norm).cpu()
+        assert off(out[:, c:c + 300], want) < TOL[dtype]
+    del x, y, wide, out
+    torch.cuda.empty_cache()
+
+
 # ------------------------------------------------------------------------------------------------------------------------------- the step
 def plain_step(p, g, v, lr, decay, mu, nesterov, **kw):
     p, g, v = (t.detach().cpu().double() for t in (p, g, v))

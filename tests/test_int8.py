@@ -454,3 +454,35 @@ def test_quantise_and_multiply_beside_another_stream():
         layers(xs[1])
         torch.cuda.synchronize()
         assert all(torch.equal(y, layers(s)) for y, s in zip(out, static))
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k,kind", [(70000, 70008, 64, torch.float16), (70000, 70001, 300, torch.bfloat16), (20, 1 << 27, 16, torch.float16), (1 << 27, 17, 16, torch.float16)],
+                         ids=["streamed", "tiles", "few rows", "few columns"])
+def test_results_behind_32_bits(m, n, k, kind):
+    """Offsets past 2^32 bytes: the corners and the middle of a result of 4 to 10 GB against 64 bits."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    a = torch.randint(-128, 128, (m, (k + 15) // 16 * 16), generator=g, device=DEV, dtype=torch.int8)[:, :k]
+    b = torch.randint(-128, 128, (n, (k + 15) // 16 * 16), generator=g, device=DEV, dtype=torch.int8)[:, :k]
+    sa, sb = torch.rand(m, generator=g, device=DEV) + 0.01, torch.rand(n, generator=g, device=DEV) + 0.01
+    y = int8.matmul(a, sa, b, sb, kind, 1e-3)
+    for r in (0, m // 2, max(m - 40, 0)):
+        for c in (0, n // 2 + 3, max(n - 40, 0)):
+            part = [t.cpu() for t in (a[r:r + 40], sa[r:r + 40], b[c:c + 40], sb[c:c + 40])]
+            check(y[r:r + 40, c:c + 40], product(*part, 1e-3), kind)
+    del y, a, b
+    torch.cuda.empty_cache()
+
+
+@gpu
+def test_quantise_behind_32_bits():
+    """2^20 + 3 rows of 4100 numbers, 4.3 GB of whole numbers and 8.6 of input."""
+    g = torch.Generator(device=DEV).manual_seed(6)
+    x = torch.randn((1 << 20) + 3, 4100, generator=g, device=DEV, dtype=torch.float16)
+    q, s = int8.quantize_rows(x)
+    for r in (0, 1 << 19, (1 << 20) - 5):
+        want, scale = quantised(x[r:r + 8].cpu())
+        assert torch.equal(q[r:r + 8].cpu().double(), want)
+        assert ((s[r:r + 8].cpu().double() - scale.double()).abs() <= scale.double() * 2.0 ** -23).all()
+    del x, q, s
+    torch.cuda.empty_cache()

@@ -234,13 +234,13 @@ class CorrComputation:
             tg = f2.shape[0]
             if packed is not None:
                 if precision in I8:
-                    build_i8(int8.quantize_packed(packed[0], h, w), int8.quantize_packed(packed[1], h, w, tiled=True), vol[t0:t0 + tg], tg)
+                    build_i8(*int8.quantize_operands(packed[0], packed[1], (h, w)), vol[t0:t0 + tg], tg)
                 else:
                     build(packed[0], packed[1], vol[t0:t0 + tg], tg, t0)
                 t0 += tg
                 continue
             if precision in I8:
-                build_i8(int8.quantize_pixels(f1.float()), int8.quantize_pixels(f2.float(), tiled=True), vol[t0:t0 + tg], tg)
+                build_i8(*int8.quantize_operands(f1.float(), f2.float()), vol[t0:t0 + tg], tg)
                 t0 += tg
                 continue
             f1 = f1.float().contiguous().view(B, D, N)

@@ -456,12 +456,26 @@ __device__ __forceinline__ int pixel_of(int r, int rows, int tiled, int h, int w
 // Maps (B, D, h, w) in 32 bits.  A workgroup takes 64 rows of the result, a lane a row, a wave a sixteenth of the channels (of 256 of them at a
 // time): all loads of a thread are in flight at once and are kept, the whole numbers are turned in LDS and leave as whole rows.  10 us for
 // 4 x 256 x 60 x 80 (19.7 MB in, 4.9 out); four waves walking the channels twice took 43.
+// Both operands of a volume share a launch (the second one's maps behind the first one's): 11 + 6 us -> 12 for 1 and 4 maps of 256 x 60 x 80.
 constexpr int SEG = 256;
-__global__ __launch_bounds__(1024) void quantize_pixels_kernel(const float* x, int D, int h, int w, int rows, int tiled, signed char* q, float* scale) {
+struct Maps { bflow_i8_maps_t v[2]; int rows[2]; };
+// the operand of a map of the launch, and which of its maps
+__device__ __forceinline__ int operand_of(const Maps& m, int& b) {
+    b = blockIdx.y;
+    if (b < m.v[0].B) return 0;
+    b -= m.v[0].B;
+    return 1;
+}
+__global__ __launch_bounds__(1024) void quantize_pixels_kernel(Maps m, int D, int h, int w) {
     __shared__ unsigned most[16][64];
     __shared__ __attribute__((aligned(16))) signed char turn[64][SEG + 16];
-    const int b = blockIdx.y, p = threadIdx.x & 63, c = threadIdx.x >> 6, r0 = blockIdx.x * 64, pix = pixel_of(r0 + p, rows, tiled, h, w);
-    const float* from = x + (long long)b * D * h * w + pix;
+    int b;
+    const int item = operand_of(m, b), rows = m.rows[item], p = threadIdx.x & 63, c = threadIdx.x >> 6, r0 = blockIdx.x * 64;
+    if (r0 >= rows) return;                         // (the other operand has more)
+    const int pix = pixel_of(r0 + p, rows, m.v[item].tiled, h, w);
+    const float* from = m.v[item].x + (long long)b * D * h * w + pix;
+    signed char* q = m.v[item].q;
+    float* scale = m.v[item].scale;
     const long long plane = (long long)h * w;
     float v[16];
     auto load = [&](int d0) {                       // this thread's channels of the segment: d0 + c * per ..
@@ -469,17 +483,17 @@ __global__ __launch_bounds__(1024) void quantize_pixels_kernel(const float* x, i
 #pragma unroll
         for (int e = 0; e < 16; ++e) v[e] = e < per && pix >= 0 ? from[(d0 + c * per + e) * plane] : 0.f;
     };
-    unsigned m = 0;
+    unsigned top = 0;
     for (int d0 = 0; d0 < D; d0 += SEG) {
         load(d0);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) m = max(m, magnitude(v[e]));
+        for (int e = 0; e < 16; ++e) top = max(top, magnitude(v[e]));
     }
-    most[c][p] = m;
+    most[c][p] = top;
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < 16; ++e) m = max(m, most[e][p]);
-    const Quant f(m);
+    for (int e = 0; e < 16; ++e) top = max(top, most[e][p]);
+    const Quant f(top);
     const bool none = f.none();
     if (c == 0 && r0 + p < rows) scale[(long long)b * rows + r0 + p] = f.scale();
     for (int d0 = 0; d0 < D; d0 += SEG) {
@@ -498,9 +512,13 @@ __global__ __launch_bounds__(1024) void quantize_pixels_kernel(const float* x, i
 }
 
 // The conv engine's operand: hi and lo planes, 32 channels of a pixel together.  Four lanes a row, eight channels each of a block of 32.
-__global__ __launch_bounds__(256) void quantize_packed_kernel(const _Float16* hi, const _Float16* lo, int KB, int h, int w, int np, int rows, int tiled, signed char* q,
-                                                              float* scale) {
-    const int lane = threadIdx.x & 63, b = blockIdx.y, r = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 16 + (lane >> 2), pix = pixel_of(r, rows, tiled, h, w);
+__global__ __launch_bounds__(256) void quantize_packed_kernel(Maps mm, int KB, int h, int w) {
+    int b;
+    const int item = operand_of(mm, b), rows = mm.rows[item], np = mm.v[item].np;
+    const _Float16 *hi = (const _Float16*)mm.v[item].x_hi, *lo = (const _Float16*)mm.v[item].x_lo;
+    signed char* q = mm.v[item].q;
+    float* scale = mm.v[item].scale;
+    const int lane = threadIdx.x & 63, r = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 16 + (lane >> 2), pix = pixel_of(r, rows, mm.v[item].tiled, h, w);
     const long long at = ((long long)b * KB * np + max(pix, 0)) * 32 + (lane & 3) * 8, step = (long long)np * 32;
     constexpr int KEEP = 8;                         // blocks of 32 channels kept in registers; further ones are read twice
     half8 vh[KEEP], vl[KEEP];
@@ -628,18 +646,37 @@ extern "C" int bflow_i8_quantize_rows(const void* x, int dtype, long long ld, lo
     return launch_status("i8_quantize_rows");
 }
 
+extern "C" int bflow_i8_quantize_maps(const bflow_i8_maps_t* items, int count, int D, int h, int w, bflow_stream_t stream) {
+    BFLOW_REQUIRE(items && count >= 1 && count <= 2, BFLOW_E_ARG, "i8_quantize_pixels: one or two operands");
+    BFLOW_REQUIRE(D >= 16 && D % 16 == 0 && h >= 1 && w >= 1 && (long long)h * w < (1LL << 28), BFLOW_E_ARG, "i8_quantize_pixels: D = %d (a multiple of 16), %d x %d pixels",
+                  D, h, w);
+    Maps m = {};
+    long long maps = 0;
+    int most = 0;
+    const bool plain = items[0].x;
+    for (int i = 0; i < count; ++i) {
+        const bflow_i8_maps_t& v = items[i];
+        BFLOW_REQUIRE(v.q && v.scale && (v.x || (v.x_hi && v.x_lo)) && !(v.x && v.x_hi), BFLOW_E_ARG, "i8_quantize_pixels: null pointer, or both forms of x");
+        BFLOW_REQUIRE(plain == (v.x != nullptr), BFLOW_E_ARG, "i8_quantize_pixels: two operands of different form");
+        BFLOW_REQUIRE(v.B >= 1 && v.B <= 65535, BFLOW_E_ARG, "i8_quantize_pixels: B = %d", v.B);
+        BFLOW_REQUIRE(plain || (D % 32 == 0 && v.np >= h * w), BFLOW_E_ARG, "i8_quantize_pixels: packed operand of %d rows for %d pixels, D = %d (a multiple of 32)", v.np, h * w, D);
+        BFLOW_REQUIRE((uintptr_t)v.q % 16 == 0, BFLOW_E_ARG, "i8_quantize_pixels: q is not aligned to 16 bytes");
+        const long long places = v.tiled ? (long long)((h + 3) / 4) * ((w + 7) / 8) * 32 : (long long)h * w;
+        BFLOW_REQUIRE(places <= 1 << 30, BFLOW_E_LIMIT, "i8_quantize_pixels: %lld places of %d x %d pixels", places, h, w);
+        m.v[i] = v;
+        m.rows[i] = (int)places;
+        maps += v.B;
+        most = m.rows[i] > most ? m.rows[i] : most;
+    }
+    BFLOW_REQUIRE(maps <= 65535, BFLOW_E_LIMIT, "i8_quantize_pixels: %lld maps > 65535", maps);
+    const dim3 grid((most + 63) / 64, (unsigned)maps);
+    if (plain) hipLaunchKernelGGL(quantize_pixels_kernel, grid, dim3(1024), 0, (hipStream_t)stream, m, D, h, w);
+    else hipLaunchKernelGGL(quantize_packed_kernel, grid, dim3(256), 0, (hipStream_t)stream, m, D / 32, h, w);
+    return launch_status("i8_quantize_pixels");
+}
+
 extern "C" int bflow_i8_quantize_pixels(const float* x, const void* x_hi, const void* x_lo, int np, int B, int D, int h, int w, int tiled, signed char* q, float* scale,
                                         bflow_stream_t stream) {
-    BFLOW_REQUIRE(q && scale && (x || (x_hi && x_lo)) && !(x && x_hi), BFLOW_E_ARG, "i8_quantize_pixels: null pointer, or both forms of x");
-    BFLOW_REQUIRE(B >= 1 && B <= 65535 && D >= 16 && D % 16 == 0 && h >= 1 && w >= 1 && (long long)h * w < (1LL << 28), BFLOW_E_ARG,
-                  "i8_quantize_pixels: B = %d, D = %d (a multiple of 16), %d x %d pixels", B, D, h, w);
-    BFLOW_REQUIRE(x || (D % 32 == 0 && np >= h * w), BFLOW_E_ARG, "i8_quantize_pixels: packed operand of %d rows for %d pixels, D = %d (a multiple of 32)", np, h * w, D);
-    BFLOW_REQUIRE((uintptr_t)q % 16 == 0, BFLOW_E_ARG, "i8_quantize_pixels: q is not aligned to 16 bytes");
-    const long long places = tiled ? (long long)((h + 3) / 4) * ((w + 7) / 8) * 32 : (long long)h * w;
-    BFLOW_REQUIRE(places <= 1 << 30, BFLOW_E_LIMIT, "i8_quantize_pixels: %lld places of %d x %d pixels", places, h, w);
-    const int rows = (int)places;
-    const dim3 grid((rows + 63) / 64, B);
-    if (x) hipLaunchKernelGGL(quantize_pixels_kernel, grid, dim3(1024), 0, (hipStream_t)stream, x, D, h, w, rows, tiled, q, scale);
-    else hipLaunchKernelGGL(quantize_packed_kernel, grid, dim3(256), 0, (hipStream_t)stream, (const _Float16*)x_hi, (const _Float16*)x_lo, D / 32, h, w, np, rows, tiled, q, scale);
-    return launch_status("i8_quantize_pixels");
+    const bflow_i8_maps_t one = {x, x_hi, x_lo, q, scale, np, B, tiled, 0};
+    return bflow_i8_quantize_maps(&one, 1, D, h, w, stream);
 }

@@ -37,7 +37,7 @@ EXPORTS = (
     "bflow_flow_metrics_accumulate", "bflow_traj_len", "bflow_pad_replicate", "bflow_voxel_grid_rectified", "bflow_voxel_grid_rectified_window", "bflow_maxabs_diff",
     "bflow_corr_lookup_bwd", "bflow_corr_lookup_bezier_bwd", "bflow_corr_pool2x2_bwd", "bflow_cvx_upsample_bwd", "bflow_l1_masked_accumulate",
     "bflow_l1_masked_grad", "bflow_conv_split_pair", "bflow_corr_lookup_im2col", "bflow_cvx_upsample_blocked",
-    "bflow_ns_workspace_bytes", "bflow_ns_orthogonalize", "bflow_muon_step", "bflow_i8_gemm", "bflow_i8_pad_rows", "bflow_i8_quantize_rows", "bflow_i8_quantize_pixels",
+    "bflow_ns_workspace_bytes", "bflow_ns_orthogonalize", "bflow_muon_step", "bflow_i8_gemm", "bflow_i8_pad_rows", "bflow_i8_quantize_rows", "bflow_i8_quantize_pixels", "bflow_i8_quantize_maps",
 )
 
 
@@ -101,6 +101,7 @@ class NormDesc(ctypes.Structure):
 # struct bflow_i8_gemm_desc, bflow_i8_pad (include/bflow_hip.h), packed by the caller: these calls are short, and a ctypes structure of 25 fields costs
 # as much as the launch
 I8_GEMM = struct.Struct("5Q11q8if4x")       # a b scale_a scale_b out | strides 0, 1 of a, b, sa, sb, out; ldo | lda ldb M N K batch0 batch1 dtype | alpha
+I8_MAPS = struct.Struct("5Q4i")             # x x_hi x_lo q scale | np B tiled 0
 I8_PAD = struct.Struct("2Q2q2i")            # src dst | ld rows | K ldd
 
 
@@ -207,6 +208,7 @@ def lib() -> ctypes.CDLL:
         "bflow_i8_pad_rows": [ctypes.c_char_p, i, vp],
         "bflow_i8_quantize_rows": [vp, i, ll, ll, i, vp, i, vp, vp],
         "bflow_i8_quantize_pixels": [vp, vp, vp, i, i, i, i, i, i, vp, vp, vp],
+        "bflow_i8_quantize_maps": [ctypes.c_char_p, i, i, i, i, vp],
         "bflow_ns_workspace_bytes": [vp, i],
         "bflow_ns_orthogonalize": [vp, i, i, i, d, d, d, d, vp, ll, vp],
         "bflow_muon_step": [vp, i, i, d, d, d, d, f, i, f, vp, f, vp, ll, vp],

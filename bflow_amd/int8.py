@@ -10,6 +10,7 @@ The correlation volume runs on it with `correlation.precision: i8` (corr.py).
 """
 from __future__ import annotations
 
+import math
 from typing import Optional, Tuple
 
 import torch
@@ -43,34 +44,64 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 def quantize_pixels(maps: torch.Tensor, tiled: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
     """maps (..., D, h, w) float32, D a multiple of 16 -> int8 (..., P, D), float32 scales (..., P): P = h * w pixels in order, or (tiled) the
     `hip.tiled_plane_size(h, w)` places of the tiled correlation volume, those outside the map zero with scale 0."""
-    if maps.dim() < 3:
-        raise hip.BflowHipError(f"quantize_pixels: maps (..., D, h, w), got {tuple(maps.shape)}")
-    lead, (D, h, w) = maps.shape[:-3], maps.shape[-3:]
-    hip._dev(maps, torch.float32, "maps", contiguous=False)
+    lead, D, h, w = _maps_shape(maps)
     maps = maps.contiguous()
-    return _quantize_pixels(maps.data_ptr(), None, None, 0, maps.device, lead, D, h, w, tiled)
+    return _quantize_maps([(maps.data_ptr(), 0, 0, 0, lead, tiled)], maps.device, D, h, w)[0]
 
 
 def quantize_packed(planes: torch.Tensor, h: int, w: int, tiled: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
     """quantize_pixels of maps in the conv engine's operand form (2, R, D/32, Np, 32) (hip.split_pack): int8 (R, P, D), scales (R, P)."""
-    _, R, KB, Np, width = planes.shape
-    if planes.dtype != torch.float16 or not planes.is_cuda or width != 32 or not (planes[0].is_contiguous() and planes[1].is_contiguous()):
+    return _quantize_maps([_packed(planes, tiled)], planes.device, planes.shape[2] * 32, h, w)[0]
+
+
+def quantize_operands(f1: torch.Tensor, f2: torch.Tensor, packed_hw: Optional[Tuple[int, int]] = None):
+    """Both sides of a correlation volume in one launch: quantize_pixels(f1), quantize_pixels(f2, tiled=True) of maps of one D, h, w; with `packed_hw`
+    = (h, w) quantize_packed of operand planes."""
+    if packed_hw is not None:
+        items, (h, w), D = [_packed(f1, False), _packed(f2, True)], packed_hw, f1.shape[2] * 32
+        if f2.shape[2] * 32 != D:
+            raise hip.BflowHipError(f"quantize_operands: {D} and {f2.shape[2] * 32} channels")
+    else:
+        (lead1, D, h, w), (lead2, *size) = _maps_shape(f1), _maps_shape(f2)
+        if size != [D, h, w]:
+            raise hip.BflowHipError(f"quantize_operands: maps {tuple(f1.shape)} and {tuple(f2.shape)} of different channels or sizes")
+        f1, f2 = f1.contiguous(), f2.contiguous()
+        items = [(f1.data_ptr(), 0, 0, 0, lead1, False), (f2.data_ptr(), 0, 0, 0, lead2, True)]
+    if f1.device != f2.device:
+        raise hip.BflowHipError("quantize_operands: all tensors on one device")
+    return _quantize_maps(items, f1.device, D, h, w)
+
+
+def _maps_shape(maps):
+    if maps.dim() < 3:
+        raise hip.BflowHipError(f"quantize_pixels: maps (..., D, h, w), got {tuple(maps.shape)}")
+    hip._dev(maps, torch.float32, "maps", contiguous=False)
+    shape = maps.shape
+    return (tuple(shape[:-3]),) + tuple(shape[-3:])
+
+
+def _packed(planes, tiled):
+    if planes.dim() != 5 or planes.dtype != torch.float16 or not planes.is_cuda or planes.shape[4] != 32 or not (planes[0].is_contiguous() and planes[1].is_contiguous()):
         raise hip.BflowHipError("quantize_packed: the operand planes of hip.split_pack")
-    return _quantize_pixels(None, planes[0].data_ptr(), planes[1].data_ptr(), Np, planes.device, (R,), KB * 32, h, w, tiled)
+    return 0, planes[0].data_ptr(), planes[1].data_ptr(), planes.shape[3], (planes.shape[1],), tiled
 
 
-def _quantize_pixels(x, hi, lo, np_rows, device, lead, D, h, w, tiled):
-    rows = hip.tiled_plane_size(h, w) if tiled else h * w
-    q = torch.empty(tuple(lead) + (rows, D), dtype=torch.int8, device=device)
-    scale = torch.empty(tuple(lead) + (rows,), device=device)
-    B = scale.numel() // rows if rows else 0
+def _quantize_maps(items, device, D, h, w):
     if D < 16 or D % 16:
         raise hip.BflowHipError(f"quantize_pixels: {D} channels, a multiple of 16 is needed")
-    if B:
+    out, table = [], []
+    for x, hi, lo, np_rows, lead, tiled in items:
+        rows = hip.tiled_plane_size(h, w) if tiled else h * w
+        q = torch.empty(lead + (rows, D), dtype=torch.int8, device=device)
+        scale = torch.empty(lead + (rows,), device=device)
+        out.append((q, scale))
+        B = math.prod(lead)
+        if B and rows:
+            table.append(hip.I8_MAPS.pack(x, hi, lo, q.data_ptr(), scale.data_ptr(), np_rows, B, int(tiled), 0))
+    if table:
         with hip._on(device):
-            hip._check(hip.lib().bflow_i8_quantize_pixels(x, hi, lo, np_rows, B, D, h, w, int(tiled), q.data_ptr(), scale.data_ptr(), hip._stream()),
-                       "bflow_i8_quantize_pixels")
-    return q, scale
+            hip._check(hip.lib().bflow_i8_quantize_maps(b"".join(table), len(table), D, h, w, hip._stream()), "bflow_i8_quantize_maps")
+    return out
 
 
 def _ready(t: torch.Tensor, K: int) -> bool:

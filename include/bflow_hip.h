@@ -626,6 +626,7 @@ int bflow_muon_step(const bflow_ns_matrix_t* m, int count, int steps, double a, 
  *                            (x NULL) the fp16-pair operand x_hi, x_lo (B, D/32, np, 32) of bflow_split_pack.  tiled 0: rows = h w, pixels in
  *                            order; 1: rows = ceil(h/4) ceil(w/8) 32, pixels in the 4 x 8 tile order of the tiled volume (row r of a tile row by
  *                            row), rows outside the map zero with scale 0.
+ *   bflow_i8_quantize_maps : the same for one or two operands (a HOST table) of one D, h, w and form in a launch: both sides of a volume
  * Quantisation: scale = max|x| / 127, q = the nearest whole number to 127 x / max|x|, halves to even, exactly.  A row of zeros has scale 0; a row
  * with an infinity or a NaN has q = 0 and an infinite or NaN scale, so that its products are NaN.                                              */
 #define BFLOW_I8_MAX_K  131071
@@ -650,6 +651,15 @@ int bflow_i8_quantize_rows(const void* x, int dtype, long long ld, long long row
                            bflow_stream_t stream);
 int bflow_i8_quantize_pixels(const float* x, const void* x_hi, const void* x_lo, int np, int B, int D, int h, int w, int tiled, signed char* q,
                              float* scale, bflow_stream_t stream);
+
+typedef struct bflow_i8_maps {
+    const float *x;                 /* (B, D, h, w), or NULL */
+    const void *x_hi, *x_lo;        /* (B, D/32, np, 32) */
+    signed char* q;
+    float* scale;
+    int np, B, tiled, reserved;
+} bflow_i8_maps_t;
+int bflow_i8_quantize_maps(const bflow_i8_maps_t* items, int count, int D, int h, int w, bflow_stream_t stream);
 
 #pragma GCC visibility pop
 #ifdef __cplusplus

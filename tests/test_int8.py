@@ -486,3 +486,35 @@ def test_quantise_behind_32_bits():
         assert ((s[r:r + 8].cpu().double() - scale.double()).abs() <= scale.double() * 2.0 ** -23).all()
     del x, q, s
     torch.cuda.empty_cache()
+
+
+def test_maps_entry_refuses_bad_tables():
+    """The C entry's own checks, before any launch: no GPU is touched."""
+    lib = hip.lib()
+    fine = dict(x=256, hi=0, lo=0, q=256, scale=256, np=0, B=2, tiled=0)
+    packed = dict(fine, x=0, hi=256, lo=256, np=20)
+
+    def call(*items, count=None, D=32, h=4, w=5):
+        return lib.bflow_i8_quantize_maps(b"".join(hip.I8_MAPS.pack(*v.values(), 0) for v in items), len(items) if count is None else count, D, h, w, None)
+    assert lib.bflow_i8_quantize_maps(None, 1, 32, 4, 5, None) < 0
+    for bad in (call(fine, count=0), call(fine, fine, fine), call(fine, D=17), call(fine, D=0), call(fine, h=0), call(fine, w=-1), call(fine, h=1 << 15, w=1 << 15), call(fine, packed),
+                call(dict(fine, x=0)), call(dict(fine, q=0)), call(dict(fine, scale=0)), call(dict(fine, hi=256, lo=256)), call(dict(fine, B=0)), call(dict(fine, B=65536)),
+                call(fine, dict(fine, B=65534)), call(dict(packed, np=19)), call(packed, D=48), call(dict(fine, q=264))):
+        assert bad < 0 and b"i8_quantize_pixels" in lib.bflow_last_error_string()
+
+
+@gpu
+@pytest.mark.parametrize("B1,B2,D,h,w", [(1, 4, 256, 13, 21), (2, 2, 64, 8, 16), (3, 1, 288, 5, 3), (1, 1, 32, 1, 1)])
+def test_both_operands_in_one_launch(B1, B2, D, h, w):
+    g = torch.Generator().manual_seed(D + h)
+    f1, f2 = torch.randn(B1, D, h, w, generator=g).to(DEV), torch.randn(B2, D, h, w, generator=g).to(DEV)
+    f2[0, :, 0, 0] = float("nan")
+    want = int8.quantize_pixels(f1) + int8.quantize_pixels(f2, tiled=True)
+    got = sum(int8.quantize_operands(f1, f2), ())
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(got, want))
+    p1, p2 = (hip.split_pack(f.reshape(f.shape[0], D, h * w).nan_to_num()) for f in (f1, f2))
+    want = int8.quantize_packed(p1, h, w) + int8.quantize_packed(p2, h, w, tiled=True)
+    got = sum(int8.quantize_operands(p1, p2, (h, w)), ())
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    with pytest.raises(hip.BflowHipError, match="different"):
+        int8.quantize_operands(f1, f2[..., :-1] if w > 1 else f2[:, :16])

@@ -480,7 +480,7 @@ __device__ __forceinline__ bool mirrored(int row, int col) { return row >> 6 > c
 // The tail of a launch: a tile of the large set takes a CU alone, so 528 of them (4096 rows) are two rounds of 256 and one of 16.  Tiles from `whole` on
 // are cut along the contraction into `parts` workgroups each, which leave 32-bit sums in `room`, and ns_join_kernel adds them in their order.  Whole
 // tiles keep their common walk along the contraction; dealing all of it out evenly lost that, and with it the L2 (189 -> 232 us).
-struct Tail { int whole, parts; float* room; };
+struct Tail { int whole, parts, first; float* room; };      // first: the last workgroup is dispatched first
 // This workgroup's tile, and its part of n rounds; false: a whole tile.
 __device__ __forceinline__ bool cut_tile(const Tail& l, int wg, int& tile, int& part) {
     part = 0;
@@ -524,7 +524,8 @@ template <class P>
 __global__ __launch_bounds__(P::THREADS, 2) void ns_gram_kernel(Works t, Tail l, char* ws) {
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     int tile, part, r0, c0;
-    const bool cut = cut_tile(l, blockIdx.x, tile, part);
+    const int wg = l.first ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+    const bool cut = cut_tile(l, wg, tile, part);
     const int k = find(t.m, t.count, tile);
     const Work m = t.m[k];
     const int R = up64(m.r), S = up64(m.s), ld = S * 4, n = P::rounds_of(S);
@@ -532,7 +533,7 @@ __global__ __launch_bounds__(P::THREADS, 2) void ns_gram_kernel(Works t, Tail l,
     const char* x = ws + x_at(m.off);
     P::run(rows_rsrc(x + (long long)r0 * ld, min(P::BM, R - r0), ld, ld), ld, rows_rsrc(x + (long long)c0 * ld, min(P::BN, R - c0), ld, ld), ld, S, lds,
            cut ? (int)((long long)n * part / l.parts) : 0, cut ? (int)((long long)n * (part + 1) / l.parts) : n);
-    if (cut) leave_part<P>(l, blockIdx.x, lds);
+    if (cut) leave_part<P>(l, wg, lds);
     else gram_out<P>(m, ws, r0, c0, lds);
 }
 
@@ -557,7 +558,8 @@ template <class P>
 __global__ __launch_bounds__(P::THREADS, 2) void ns_poly_kernel(Works t, Tail l, char* ws, float b, float c, int drop) {
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     int tile, part, r0, c0;
-    const bool cut = cut_tile(l, blockIdx.x, tile, part);
+    const int wg = l.first ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+    const bool cut = cut_tile(l, wg, tile, part);
     const int k = find(t.m, t.count, tile);
     const Work m = t.m[k];
     const int R = up64(m.r), ld = R * 4, n = P::rounds_of(R);
@@ -567,7 +569,7 @@ __global__ __launch_bounds__(P::THREADS, 2) void ns_poly_kernel(Works t, Tail l,
     av.load((const _Float16*)a, r0, c0, R, R);
     P::run(rows_rsrc(a + (long long)r0 * ld, min(P::BM, R - r0), ld, ld), ld, rows_rsrc(a + (long long)c0 * ld, min(P::BN, R - c0), ld, ld), ld, R, lds,
            cut ? (int)((long long)n * part / l.parts) : 0, cut ? (int)((long long)n * (part + 1) / l.parts) : n);
-    if (cut) leave_part<P>(l, blockIdx.x, lds);
+    if (cut) leave_part<P>(l, wg, lds);
     else poly_out<P>(m, ws, r0, c0, lds, av, b, c, drop);
 }
 
@@ -1413,14 +1415,17 @@ struct LargeSet {
     typedef Product<128, 128, 64, 64, 1, 2> Panel;
 };
 
+// Tiles of a square product that are not cut; parts of those behind them (0: none); whether they are dispatched from the last one on.
+struct Cut { int whole, parts, first; };
+
 struct Plan {
     Works square, panel;
     Entries norm, pack;
     Exits leave;
     long long tiles_square, tiles_panel, tiles_sum, tiles_norm, tiles_pack, bytes;
     bool large;
-    int whole, cut_parts;  // tiles of a square product that are not cut; parts of those behind them (0: none)
-    long long room;        // where the parts stand
+    Cut gram, poly;
+    long long room;        // where the parts of cut tiles stand
     bool panels;           // every matrix of at most PANEL_ROWS rows: `works` instead of `square` and `panel`
     PanelWorks works;
     int lds_panel, lds_square;
@@ -1435,6 +1440,99 @@ template <class Set> void lay_out_products(Plan& p) {
         p.tiles_square += lower_tiles<typename Set::Square>(R);
         p.tiles_panel += (long long)((R + Set::Panel::BM - 1) / Set::Panel::BM) * ((S + Set::Panel::BN - 1) / Set::Panel::BN);
     }
+}
+
+// Loads of the CUs as pieces of work are dealt out in order, each to the least loaded: CUs of one load stand together.
+constexpr int CUS = 256;
+struct Loads {
+    struct { double load; long long cus; } at[2 * MOST + 8];
+    int count = 1;
+    double most = 0;
+    Loads() { at[0] = {0, CUS}; }
+    void deal(double length, long long pieces) {
+        while (pieces > 0) {
+            const double load = at[0].load + length;
+            const long long n = pieces < at[0].cus ? pieces : at[0].cus;
+            pieces -= n;
+            if (n == at[0].cus) {
+                for (int i = 1; i < count; ++i) at[i - 1] = at[i];
+                --count;
+            } else {
+                at[0].cus -= n;
+            }
+            int i = count;
+            while (i > 0 && at[i - 1].load > load) --i;
+            if (i > 0 && at[i - 1].load == load) {
+                at[i - 1].cus += n;
+            } else {
+                for (int j = count; j > i; --j) at[j] = at[j - 1];
+                at[i] = {load, n};
+                ++count;
+            }
+            most = std::max(most, load);
+        }
+    }
+};
+
+// Which tiles of a product of the large set are cut, by the time that the dealing gives, in rounds (1.3 us): a whole tile
+// takes 3 more and a part 2, the join 4, and writing and reading a part a 40th.  Either the
+// last tiles that would leave most CUs idle, as many parts as there are CUs for them, or all tiles of the list's longest matrices (they stand last) in two
+// to four parts; a part has CUT_ROUNDS rounds at least.  Calls without and with it: 2944 x 2944 in fp32 2255 / 1985 us,
+// 4096 x 4096 4495 / 4075 (bf16 3910 / 3620), 8 of 1024 x 1024 892 / 856, a step of 4 of 1024 x 1024 and 2 of 1024 x 4096 1073 / 1004; 2048 x 2048 whole 790,
+// in three parts 829.  (Two rounds at least: 24 of 640 x 640 893 / 937; eight: 2944 x 2944 2079.)
+constexpr int CUT_ROUNDS = 4;
+constexpr long long CUT_PIECES = 1024;
+template <int WHAT> Cut plan_cut(const Works& w) {
+    typedef LargeSet::Square Q;
+    const auto columns = [&](int i) { return up64(WHAT == GRAM ? w.m[i].s : w.m[i].r); };
+    const auto tiles = [&](int i) { return (long long)lower_tiles<Q>(up64(w.m[i].r)); };
+    long long total = 0;
+    for (int i = 0; i < w.count; ++i) total += tiles(i);
+    const auto time = [&](long long whole, int parts) {      // the last matrix' tiles start first
+        Loads loads;
+        long long left = total - whole, skip = left;
+        for (int i = w.count - 1; i >= 0 && left > 0; --i) {
+            const long long n = std::min(left, tiles(i));
+            loads.deal((double)Q::rounds_of(columns(i)) / parts + 2, n * parts);
+            left -= n;
+        }
+        for (int i = w.count - 1; i >= 0; --i) {
+            const long long n = std::min(skip, tiles(i));
+            skip -= n;
+            loads.deal(Q::rounds_of(columns(i)) + 3, tiles(i) - n);
+        }
+        return loads.most + (whole < total ? 4 + (double)(total - whole) * parts / 40 : 0);
+    };
+    const auto most_parts = [&](long long whole) {           // by the shortest of the cut tiles, in the form with fewer rounds
+        int shortest = 1 << 30;
+        long long seen = total;
+        for (int i = w.count - 1; i >= 0 && seen > whole; --i) {
+            shortest = std::min(shortest, Q::Halves::rounds_of(columns(i)));
+            seen -= tiles(i);
+        }
+        return shortest / CUT_ROUNDS;
+    };
+    // Lengths that differ start with the longest, which stand last.  The last tiles of many alike come last: in front they would end the common walk of the
+    // others (4096 x 4096 in bf16 3.69 -> 3.77 ms).
+    const int differ = columns(0) != columns(w.count - 1);
+    Cut best = {(int)total, 0, differ};
+    double least = time(total, 1);
+    const auto consider = [&](long long whole, int parts, int first) {
+        if (parts < 2 || whole >= total || (total - whole) * parts > CUT_PIECES || parts > most_parts(whole)) return;
+        const double t = time(whole, parts);
+        if (t < least) { least = t; best = {(int)whole, parts, first}; }
+    };
+    const long long last = total % CUS;
+    if (total > CUS && last) consider(total - last, (int)std::min<long long>(CUS / last, most_parts(total - last)), 0);
+    long long whole = total;
+    int borders = 0;
+    for (int i = w.count - 1; i >= 0 && borders < 4; --i) {
+        whole -= tiles(i);
+        if (i > 0 && columns(i - 1) == columns(i)) continue;
+        ++borders;
+        for (int parts = 2; parts <= 4; ++parts) consider(whole, parts, 1);
+    }
+    return best;
 }
 
 // Panels of a workgroup.  A panel takes COST microseconds by its rows; the workgroups of a list (one for each CU at most, where that can be) should take
@@ -1487,8 +1585,13 @@ void lay_out_panels(Plan& p) {
 }
 
 // The launches of one group of matrices; returns false where a count passes what a grid holds.
-bool lay_out(const bflow_ns_matrix_t* m, int count, Plan& p) {
+bool lay_out(const bflow_ns_matrix_t* given, int count, Plan& p) {
     long long off = 0, blocks = 0;
+    bflow_ns_matrix_t m[MOST];
+    std::copy(given, given + count, m);
+    const auto shorter = [](const bflow_ns_matrix_t& a, const bflow_ns_matrix_t& b) { return std::max(a.rows, a.cols) < std::max(b.rows, b.cols); };
+    for (int i = 1; i < count; ++i)                     // the longest contractions last
+        for (int j = i; j > 0 && shorter(m[j], m[j - 1]); --j) std::swap(m[j], m[j - 1]);
     p.tiles_square = p.tiles_panel = p.tiles_norm = p.tiles_pack = 0;
     p.square.count = p.panel.count = p.norm.count = p.pack.count = p.leave.count = count;
     for (int i = 0; i < count; ++i) {
@@ -1522,27 +1625,13 @@ bool lay_out(const bflow_ns_matrix_t* m, int count, Plan& p) {
     p.large = blocks >= LARGE_BLOCKS;
     if (p.large) lay_out_products<LargeSet>(p);
     else lay_out_products<SmallSet>(p);
-    // The last tiles, where they leave half of the CUs idle or more; each part has CUT_ROUNDS rounds at least.  Calls without and with it: 2944 x 2944 in fp32
-    // 2255 / 1985 us, 4096 x 4096 4495 / 4075 (bf16 3910 / 3620), 8 of 1024 x 1024 892 / 856, 8192 x 8192 31.7 / 31.0 ms.  (Two rounds at least: 24 of 640 x
-    // 640 893 / 937; eight: 2944 x 2944 2079.)
-    constexpr int CUS = 256, CUT_ROUNDS = 4;
-    p.whole = (int)p.tiles_square;
-    p.cut_parts = 0;
+    p.gram = p.poly = {(int)p.tiles_square, 0, 0};
     p.room = off;
-    if (p.large && p.tiles_square > CUS) {
-        const int last = (int)(p.tiles_square % CUS);
-        int shortest = 1 << 30;
-        for (int i = 0, seen = 0; i < count; ++i) {
-            const int R = up64(p.square.m[i].r);
-            seen += lower_tiles<LargeSet::Square>(R);
-            if (seen > p.tiles_square - last) shortest = std::min(shortest, LargeSet::Square::Halves::rounds_of(R));      // (R <= S: of either product, in either form)
-        }
-        const int parts = last ? std::min(CUS / last, shortest / CUT_ROUNDS) : 0;
-        if (parts > 1) {
-            p.whole -= last;
-            p.cut_parts = parts;
-            off += (long long)last * parts * LargeSet::Square::TILE;
-        }
+    if (p.large) {
+        p.gram = plan_cut<GRAM>(p.square);
+        p.poly = plan_cut<POLY>(p.square);
+        const long long most = std::max((p.tiles_square - p.gram.whole) * p.gram.parts, (p.tiles_square - p.poly.whole) * p.poly.parts);
+        off += most * LargeSet::Square::TILE;
     }
     p.bytes = off;
     return p.tiles_pack < (1LL << 30);
@@ -1601,17 +1690,19 @@ int launch_products(const Plan& p, int steps, float a, float b, float c, double 
     const auto leave = ns_leave_kernel<P, DT, STEP>;
     for (const int rc : {allow_lds(gram, G::LDS), allow_lds(poly, Q::LDS), allow_lds(apply, P::LDS), allow_lds(leave, P::LDS)})
         if (rc) return rc;
-    const Tail tail = {p.whole, p.cut_parts, (float*)(ws + p.room)};
-    const int cut = (int)p.tiles_square - p.whole, squares = p.whole + cut * p.cut_parts, joins = cut * (Q::BM / 64) * (Q::BN / 64);
+    const auto tail = [&](Cut c) { return Tail{c.whole, c.parts, c.first, (float*)(ws + p.room)}; };
+    const auto cut = [&](Cut c) { return (int)p.tiles_square - c.whole; };
+    const auto grid = [&](Cut c) { return dim3(c.whole + cut(c) * c.parts); };
+    const auto joins = [&](Cut c) { return dim3(cut(c) * (Q::BM / 64) * (Q::BN / 64)); };
     const double bits = log2(gain);
     for (int k = 0; k < steps; ++k) {
         const int drop = (int)std::ceil(k * bits), next = (int)std::ceil((k + 1) * bits);
-        hipLaunchKernelGGL(gram, dim3(squares), dim3(G::THREADS), G::LDS, st, p.square, tail, ws);
+        hipLaunchKernelGGL(gram, grid(p.gram), dim3(G::THREADS), G::LDS, st, p.square, tail(p.gram), ws);
         if constexpr (std::is_same_v<Set, LargeSet>)
-            if (cut) hipLaunchKernelGGL((ns_join_kernel<Q, GRAM>), dim3(joins), dim3(256), 64 * 64 * 4, st, p.square, tail, ws, b, c, drop);
-        hipLaunchKernelGGL(poly, dim3(squares), dim3(Q::THREADS), Q::LDS, st, p.square, tail, ws, b, c, drop);
+            if (cut(p.gram)) hipLaunchKernelGGL((ns_join_kernel<Q, GRAM>), joins(p.gram), dim3(256), 64 * 64 * 4, st, p.square, tail(p.gram), ws, b, c, drop);
+        hipLaunchKernelGGL(poly, grid(p.poly), dim3(Q::THREADS), Q::LDS, st, p.square, tail(p.poly), ws, b, c, drop);
         if constexpr (std::is_same_v<Set, LargeSet>)
-            if (cut) hipLaunchKernelGGL((ns_join_kernel<Q, POLY>), dim3(joins), dim3(256), 64 * 64 * 4, st, p.square, tail, ws, b, c, drop);
+            if (cut(p.poly)) hipLaunchKernelGGL((ns_join_kernel<Q, POLY>), joins(p.poly), dim3(256), 64 * 64 * 4, st, p.square, tail(p.poly), ws, b, c, drop);
         if (k + 1 < steps) hipLaunchKernelGGL(apply, dim3(p.tiles_panel), dim3(P::THREADS), P::LDS, st, p.panel, ws, k & 1, a, drop, next);
         else hipLaunchKernelGGL(leave, dim3(p.tiles_panel), dim3(P::THREADS), P::LDS, st, p.leave, ws, k & 1, a, drop, lr, lr_device, decay);
     }

@@ -307,19 +307,22 @@ def test_on_another_stream_and_in_a_graph():
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("shapes", [[(2900, 2950)], [(1000, 1020)] * 8, [(70, 3000)] + [(1000, 1020)] * 8], ids=["one", "eight", "nine"])
+@pytest.mark.parametrize("shapes", [[(2900, 2950)], [(1000, 1020)] * 8, [(70, 3000)] + [(1000, 1020)] * 8,
+                                    [(1000, 4000)] + [(1000, 1020)] * 4 + [(4000, 1000), (1000, 900)]], ids=["one", "eight", "nine", "lengths"])
 def test_last_tiles_cut_along_the_contraction(shapes, dtype):
-    """276, 288 and 289 tiles of 128 x 128: those behind the 256th are cut.  Against 64 bits on the device, in front of and behind other calls; twice the same
+    """276, 288 and 289 tiles of 128 x 128: those behind the 256th are cut; tiles of two lengths: the long ones are.  Against 64 bits on the device, in front of and behind other calls; twice the same
     bits; and through a step."""
     xs = [gradient(*s, seed=k).to(dtype).to(DEV) for k, s in enumerate(shapes)]
 
     def exact(x):
         a, b, c = muon.COEFFICIENTS
+        tall = x.shape[0] > x.shape[1]
         y = x.double() / (x.double().norm() + 1e-7)
+        y = y.t().contiguous() if tall else y
         for _ in range(5):
             g = y @ y.t()
             y = a * y + (b * g + c * g @ g) @ y
-        return y
+        return y.t() if tall else y
     ys = muon.orthogonalize(xs)
     muon.orthogonalize([xs[-1][:300, :310]])
     assert all(torch.equal(y, z) for y, z in zip(ys, muon.orthogonalize(xs)))

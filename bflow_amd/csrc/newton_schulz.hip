@@ -675,6 +675,33 @@ __global__ __launch_bounds__(P::THREADS, 2) void ns_leave_kernel(Exits t, const 
     // element by element along the user's rows (any address, whole lines), the weights of sixteen of them read together
     constexpr int N = P::BM * P::BN / P::THREADS, AT_ONCE = 16;
     static_assert(N % AT_ONCE == 0, "whole batches");
+    if constexpr (DT == F32) {
+        // four of a row at a time where they stand at multiples of 16 bytes: a step of 4 of 1024 x 1024 and 2 of 1024 x 4096
+        // 132 -> 110 us (the same in the panels below: 1 of 236 us, left out)
+        if (!m.tall && ((uintptr_t)m.dst | (unsigned long long)m.ld * 4) % 16 == 0 && m.s % 4 == 0) {
+            constexpr int FOURS = N / 4 < 8 ? N / 4 : 8;
+            static_assert(N / 4 % FOURS == 0, "whole batches");
+#pragma unroll 1
+            for (int n0 = 0; n0 < N / 4; n0 += FOURS) {
+                float4 v[FOURS], p[FOURS];
+                float* at[FOURS];
+#pragma unroll
+                for (int n = 0; n < FOURS; ++n) {
+                    const int i = threadIdx.x + (n0 + n) * P::THREADS, row = i / (P::BN / 4), col = i % (P::BN / 4) * 4;
+                    at[n] = r0 + row < m.r && s0 + col < m.s ? (float*)m.dst + (long long)(r0 + row) * m.ld + s0 + col : nullptr;
+                    v[n] = *reinterpret_cast<const float4*>((const float*)lds + P::T::at(row, col));
+                    if constexpr (STEP) p[n] = at[n] ? *reinterpret_cast<const float4*>(at[n]) : float4{0.f, 0.f, 0.f, 0.f};
+                }
+#pragma unroll
+                for (int n = 0; n < FOURS; ++n) {
+                    if (!at[n]) continue;
+                    if constexpr (STEP) v[n] = make_float4(fmaf(-rate, v[n].x, p[n].x * keep), fmaf(-rate, v[n].y, p[n].y * keep), fmaf(-rate, v[n].z, p[n].z * keep), fmaf(-rate, v[n].w, p[n].w * keep));
+                    *reinterpret_cast<float4*>(at[n]) = v[n];
+                }
+            }
+            return;
+        }
+    }
 #pragma unroll 1
     for (int n0 = 0; n0 < N; n0 += AT_ONCE) {
         long long at[AT_ONCE];

@@ -264,26 +264,18 @@ __device__ __forceinline__ int g_of(const char* ws, long long off, int drop) { r
 
 // --------------------------------------------------------------------------------------------------------------------------- products
 // BM x BN tile of A B^T.  A group of waves has WM x WN of it each; KG groups share the contraction (a stage holds a chunk for each) and are summed
-// in LDS, in a fixed order.  PAIRS: three matrix passes over 32 columns a chunk.  Otherwise the hi halves alone, one pass over 64 columns: the hi
-// halves of two neighbouring chunks stand in one of the stage.
-// At 4096 x 4096 (three passes counted): X 1.10 PFLOP/s of fp16, B 1.00, matrix cores busy 65 and 55 % of the cycles at a clock that power holds down; A from
-// the hi halves 0.61, bound by what the L2s deliver (half of every line that it reads is lo).  A library product of plain fp16 reaches 1.49 here.
-template <int BM_, int BN_, int WM, int WN, int KG_, int STAGES, bool PAIRS = true>
+// in LDS, in a fixed order.  Three matrix passes over the 32 columns of a chunk.
+// At 4096 x 4096 (three passes counted): X 1.10 PFLOP/s of fp16, B 1.00, matrix cores busy 65 and 55 % of the cycles at a clock that power holds down.
+// A library product of plain fp16 reaches 1.49 here.
+template <int BM_, int BN_, int WM, int WN, int KG_, int STAGES>
 struct Product {
     static constexpr int BM = BM_, BN = BN_, KG = KG_;
     static constexpr int ACROSS = BN / WN, WAVES = (BM / WM) * ACROSS, THREADS = 64 * WAVES * KG, MT = WM / 32, NT = WN / 32;
-    static constexpr int COLUMNS = PAIRS ? 32 : 64;      // of a chunk
-    typedef Product<BM_, BN_, WM, WN, KG_, STAGES, false> Halves;
+    static constexpr int COLUMNS = 32;                   // of a chunk
     static constexpr int CHUNK_BYTES = (BM + BN) * CHUNK, STAGE = KG * CHUNK_BYTES, TILE = BM * BN * 4;
     static constexpr int LDS = STAGES * STAGE > KG * TILE ? STAGES * STAGE : KG * TILE;
     static_assert(BM / 8 % WAVES == 0 && BN / 8 % WAVES == 0 && WAVES % 2 == 0, "whole pieces of either operand for every wave, all odd or all even");
     typedef Turn<BN> T;
-
-    __device__ static __forceinline__ int source(int lane, int ld, int wave) {
-        if constexpr (PAIRS) return lane_offset(lane, ld, wave);
-        const int seg = lane_segment(lane, wave);
-        return (lane >> 3) * ld + (seg >> 2) * CHUNK + (seg & 3) * 16;
-    }
 
     // rounds of a contraction over `columns`, a multiple of 64: each group of waves takes a chunk in each
     __host__ __device__ static inline int rounds_of(int columns) { return (columns / COLUMNS + KG - 1) / KG; }
@@ -295,7 +287,7 @@ struct Product {
         const int chunks = min(columns / COLUMNS, last * KG);
         const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = w / WAVES, wave = w % WAVES;
         const int wm = wave / ACROSS, wn = wave % ACROSS;
-        const int va = source(lane, lda, wave), vb = source(lane, ldb, wave);
+        const int va = lane_offset(lane, lda, wave), vb = lane_offset(lane, ldb, wave);
         f32x16 hh[MT][NT], xx[MT][NT];
 #pragma unroll
         for (int i = 0; i < MT; ++i)
@@ -328,27 +320,25 @@ struct Product {
             const char* as = lds + (r % STAGES) * STAGE + group * CHUNK_BYTES + wm * WM * CHUNK;
             const char* bs = lds + (r % STAGES) * STAGE + group * CHUNK_BYTES + (BM + wn * WN) * CHUNK;
 #pragma unroll
-            for (int sub = 0; sub < (PAIRS ? 2 : 4); ++sub) {
+            for (int sub = 0; sub < 2; ++sub) {
                 half8 ah[MT], al[MT], bh[NT], bl[NT];
 #pragma unroll
                 for (int i = 0; i < MT; ++i) {
                     ah[i] = __builtin_bit_cast(half8, frag(as + i * 32 * CHUNK, lane, sub));
-                    if (PAIRS) al[i] = __builtin_bit_cast(half8, frag(as + i * 32 * CHUNK, lane, 2 + sub));
+                    al[i] = __builtin_bit_cast(half8, frag(as + i * 32 * CHUNK, lane, 2 + sub));
                 }
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     bh[j] = __builtin_bit_cast(half8, frag(bs + j * 32 * CHUNK, lane, sub));
-                    if (PAIRS) bl[j] = __builtin_bit_cast(half8, frag(bs + j * 32 * CHUNK, lane, 2 + sub));
+                    bl[j] = __builtin_bit_cast(half8, frag(bs + j * 32 * CHUNK, lane, 2 + sub));
                 }
 #pragma unroll
                 for (int i = 0; i < MT; ++i)
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
                         hh[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], hh[i][j], 0, 0, 0);
-                        if (PAIRS) {
-                            xx[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], xx[i][j], 0, 0, 0);
-                            xx[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], xx[i][j], 0, 0, 0);
-                        }
+                        xx[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], xx[i][j], 0, 0, 0);
+                        xx[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], xx[i][j], 0, 0, 0);
                     }
             }
         }
@@ -361,7 +351,7 @@ struct Product {
             for (int j = 0; j < NT; ++j)
 #pragma unroll
                 for (int k = 0; k < 16; ++k)
-                    t[T::at(wm * WM + i * 32 + (k >> 2) * 8 + (lane >> 5) * 4 + (k & 3), wn * WN + j * 32 + (lane & 31))] = PAIRS ? fmaf(xx[i][j][k], SPLIT_LO_INV, hh[i][j][k]) : hh[i][j][k];
+                    t[T::at(wm * WM + i * 32 + (k >> 2) * 8 + (lane >> 5) * 4 + (k & 3), wn * WN + j * 32 + (lane & 31))] = fmaf(xx[i][j][k], SPLIT_LO_INV, hh[i][j][k]);
         __syncthreads();
     }
 
@@ -442,7 +432,7 @@ struct Product {
 
 template <class P> __host__ __device__ inline int lower_tiles(int R) { const int down = (R + P::BM - 1) / P::BM; return down * (down + 1) / 2; }
 // Tile t of a lower triangle, bands of BAND rows of tiles, each walked column by column; an XCD (workgroups go round them) takes an eighth of that walk, so
-// that what it works on at one time shares rows: 4096 x 4096 from the hi halves 189 -> 149 us (traffic through the L2s bounds it; in pairs as before).
+// that what it works on at one time shares rows: 4096 x 4096 4147 -> 4082 us, 8 of 1024 x 1024 870 -> 852 (whole calls, fp32).
 constexpr int BAND = 8;
 template <class P> __device__ __forceinline__ void lower(int t, int R, int& r0, int& c0) {
     static_assert(P::BM == P::BN, "square tiles");
@@ -463,8 +453,8 @@ template <class P> __device__ __forceinline__ void lower(int t, int R, int& r0, 
     r0 = i * P::BM;
     c0 = j * P::BN;
 }
-// Tile t of a rectangle, in the same order: 24 of 640 x 640 in bf16 881 -> 815 us, 3 of 1500 x 2000 1038 -> 1007; powers of two lose 0 to 1.5 % (8 of 1024 x
-// 1024 809 -> 821, 4096 x 4096 3674 -> 3684: there any order shares).
+// Tile t of a rectangle, in the same order: 24 of 640 x 640 903 -> 835 us, 2944 x 2944 2012 -> 1990; powers of two lose or gain up to 1 % (8 of 1024 x
+// 1024 868 -> 872, 4096 x 4096 4217 -> 4242 in fp32, 4250 -> 4212 in bf16: there any order shares).
 template <class P> __device__ __forceinline__ void panel(int t, int R, int S, int& r0, int& s0) {
     const int down = (R + P::BM - 1) / P::BM, across = (S + P::BN - 1) / P::BN, total = down * across;
     const int x = t & 7, at = x * (total >> 3) + min(x, total & 7) + (t >> 3);
@@ -1504,10 +1494,10 @@ struct Loads {
 // Which tiles of a product of the large set are cut, by the time that the dealing gives, in rounds (1.3 us): a whole tile
 // takes 3 more and a part 2, the join 4, and writing and reading a part a 40th.  Either the
 // last tiles that would leave most CUs idle, as many parts as there are CUs for them, or all tiles of the list's longest matrices (they stand last) in two
-// to four parts; a part has CUT_ROUNDS rounds at least.  Calls without and with it: 2944 x 2944 in fp32 2255 / 1985 us,
-// 4096 x 4096 4495 / 4075 (bf16 3910 / 3620), 8 of 1024 x 1024 892 / 856, a step of 4 of 1024 x 1024 and 2 of 1024 x 4096 1073 / 1004; 2048 x 2048 whole 790,
-// in three parts 829.  (Two rounds at least: 24 of 640 x 640 893 / 937; eight: 2944 x 2944 2079.)
-constexpr int CUT_ROUNDS = 4;
+// to four parts; a part has eight rounds or so (CUT_COLUMNS) at least.  Calls without and with it: 2944 x 2944 in fp32 2255 / 1985 us,
+// 4096 x 4096 4495 / 4075, 8 of 1024 x 1024 892 / 856, a step of 4 of 1024 x 1024 and 2 of 1024 x 4096 1073 / 1004; 2048 x 2048 whole 790,
+// in three parts 829.  (256 columns at least: 24 of 640 x 640 893 / 937; 1024: 2944 x 2944 2079.)
+constexpr int CUT_COLUMNS = 512;
 constexpr long long CUT_PIECES = 1024;
 template <int WHAT> Cut plan_cut(const Works& w) {
     typedef LargeSet::Square Q;
@@ -1530,17 +1520,17 @@ template <int WHAT> Cut plan_cut(const Works& w) {
         }
         return loads.most + (whole < total ? 4 + (double)(total - whole) * parts / 40 : 0);
     };
-    const auto most_parts = [&](long long whole) {           // by the shortest of the cut tiles, in the form with fewer rounds
+    const auto most_parts = [&](long long whole) {           // by the shortest of the cut tiles, to the nearest 128 columns upwards
         int shortest = 1 << 30;
         long long seen = total;
         for (int i = w.count - 1; i >= 0 && seen > whole; --i) {
-            shortest = std::min(shortest, Q::Halves::rounds_of(columns(i)));
+            shortest = std::min(shortest, columns(i));
             seen -= tiles(i);
         }
-        return shortest / CUT_ROUNDS;
+        return (shortest + 64) / CUT_COLUMNS;
     };
     // Lengths that differ start with the longest, which stand last.  The last tiles of many alike come last: in front they would end the common walk of the
-    // others (4096 x 4096 in bf16 3.69 -> 3.77 ms).
+    // others (4096 x 4096 4.08 -> 4.12 ms).
     const int differ = columns(0) != columns(w.count - 1);
     Cut best = {(int)total, 0, differ};
     double least = time(total, 1);
@@ -1708,14 +1698,11 @@ template <class Set, int DT, bool STEP>
 int launch_products(const Plan& p, int steps, float a, float b, float c, double gain, char* ws, float lr, const float* lr_device, float decay, hipStream_t st) {
     typedef typename Set::Square Q;
     typedef typename Set::Panel P;
-    // Where the result is rounded to bf16 (2^-9 of it, 1.7e-3 in all), the Gram matrix may come from the hi halves alone: it then adds 2e-4 to 5e-4.
-    // (In fp16, whose own rounding is 2e-4, it may not.)
-    typedef std::conditional_t<DT == BF16, typename Q::Halves, Q> G;
-    const auto gram = ns_gram_kernel<G>;
+    const auto gram = ns_gram_kernel<Q>;
     const auto poly = ns_poly_kernel<Q>;
     const auto apply = ns_apply_kernel<P>;
     const auto leave = ns_leave_kernel<P, DT, STEP>;
-    for (const int rc : {allow_lds(gram, G::LDS), allow_lds(poly, Q::LDS), allow_lds(apply, P::LDS), allow_lds(leave, P::LDS)})
+    for (const int rc : {allow_lds(gram, Q::LDS), allow_lds(poly, Q::LDS), allow_lds(apply, P::LDS), allow_lds(leave, P::LDS)})
         if (rc) return rc;
     const auto tail = [&](Cut c) { return Tail{c.whole, c.parts, c.first, (float*)(ws + p.room)}; };
     const auto cut = [&](Cut c) { return (int)p.tiles_square - c.whole; };
@@ -1724,7 +1711,7 @@ int launch_products(const Plan& p, int steps, float a, float b, float c, double 
     const double bits = log2(gain);
     for (int k = 0; k < steps; ++k) {
         const int drop = (int)std::ceil(k * bits), next = (int)std::ceil((k + 1) * bits);
-        hipLaunchKernelGGL(gram, grid(p.gram), dim3(G::THREADS), G::LDS, st, p.square, tail(p.gram), ws);
+        hipLaunchKernelGGL(gram, grid(p.gram), dim3(Q::THREADS), Q::LDS, st, p.square, tail(p.gram), ws);
         if constexpr (std::is_same_v<Set, LargeSet>)
             if (cut(p.gram)) hipLaunchKernelGGL((ns_join_kernel<Q, GRAM>), joins(p.gram), dim3(256), 64 * 64 * 4, st, p.square, tail(p.gram), ws, b, c, drop);
         hipLaunchKernelGGL(poly, grid(p.poly), dim3(Q::THREADS), Q::LDS, st, p.square, tail(p.poly), ws, b, c, drop);

@@ -55,10 +55,10 @@ def _check_numbers(steps: int, coefficients: Sequence[float], eps: float):
 def orthogonalize(matrices: Sequence[torch.Tensor], steps: int = STEPS, coefficients: Sequence[float] = COEFFICIENTS, eps: float = EPS) -> List[torch.Tensor]:
     """Newton-Schulz steps on every matrix of a list: new tensors of the same shapes and types (float32, float16 or bfloat16, mixed as you like).
 
-    Sums are held in 32 bits, products in fp16 pairs (fp32-class; small matrices in 64 bits); a 16-bit result is rounded once, and its Gram matrices
-    come from the pairs' leading halves.  Tensors of more than two dimensions are taken as (shape[0], everything else).  The results of one type share
-    a buffer.  An empty matrix stays empty, a zero matrix zero; one with a NaN or an infinity becomes all NaN.  The same list gives the same bits; a
-    matrix in another list may be tiled another way and differ by roundings.  Not differentiable: the results carry no graph."""
+    Sums are held in 32 bits, products in fp16 pairs (fp32-class whatever the type; small matrices in 64 bits); a 16-bit result is rounded once.
+    Tensors of more than two dimensions are taken as (shape[0], everything else).  The results of one type share a buffer.  An empty matrix stays
+    empty, a zero matrix zero; one with a NaN or an infinity becomes all NaN.  The same list gives the same bits; a matrix in another list may be
+    tiled another way and differ by roundings.  Not differentiable: the results carry no graph."""
     _check_numbers(steps, coefficients, eps)
     if isinstance(matrices, torch.Tensor):
         raise hip.BflowHipError("orthogonalize takes a list of matrices")

@@ -590,8 +590,8 @@ int bflow_l1_masked_grad(const float* src, const float* tgt, const unsigned char
  *   bflow_muon_step       : per matrix, all fp32:  momentum = mu momentum + src (dense);  u = src + mu momentum (nesterov) or momentum;
  *                           dst = dst (1 - lr weight_decay) - lr 0.2 sqrt(max(rows, cols)) X(u).  lr: *lr_device (device float) when given.
  * `m` is a HOST table, read during the call (it travels in the launches' arguments; lists of any length, 64 matrices a round).  Matrices are
- * row-major, *_ld elements from row to row, and none overlaps another but dst = src.  Arithmetic: fp16 pairs with fp32 sums (fp32-class accuracy;
- * for 16-bit results A from the leading halves), small matrices in fp64, norms in fp64.  A list gives the same bits every time; its matrices one
+ * row-major, *_ld elements from row to row, and none overlaps another but dst = src.  Arithmetic: fp16 pairs with fp32 sums (fp32-class accuracy
+ * whatever the dtype; a 16-bit result is rounded once), small matrices in fp64, norms in fp64.  A list gives the same bits every time; its matrices one
  * by one, or in another list, may be tiled another way and differ by roundings.  A matrix with a NaN or an infinity becomes all NaN, a zero matrix
  * stays zero.
  * ws: bflow_ns_workspace_bytes(m, count) bytes (rows and cols alone are read; 0 where all are small: ws may be NULL), aligned to 256, free for

@@ -581,3 +581,32 @@ def test_results_of_one_type_share_a_buffer_and_stay_apart():
     keep = [y.clone() for y in ys]
     ys[1].fill_(7.0)
     assert torch.equal(ys[0], keep[0]) and torch.equal(ys[2], keep[2]) and all(y.data_ptr() % 256 == 0 for y in ys)
+
+
+# ------------------------------------------------------------------------------------------------------------ results rounded once
+def spectrum(kind, m, n, seed):
+    """Matrices whose singular values are no gradient's: all alike, a Gaussian's, one alone, a few and no others."""
+    rs = np.random.RandomState(seed)
+    if kind == "orthogonal":
+        q = torch.linalg.qr(torch.from_numpy(rs.standard_normal((max(m, n), min(m, n)))))[0]
+        return q if m >= n else q.t().contiguous()
+    if kind == "gaussian":
+        return torch.from_numpy(rs.standard_normal((m, n)))
+    if kind == "constant":
+        return torch.full((m, n), 0.75, dtype=torch.float64)
+    return torch.from_numpy(np.round(rs.standard_normal((m, 3)) * 4) @ np.round(rs.standard_normal((3, n)) * 4))      # "rank three": whole numbers, most below 256
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("kind", ["orthogonal", "gaussian", "constant", "rank three"])
+def test_16_bit_results_are_those_of_32_bits_rounded(kind, dtype):
+    """An entry of the result is a 32-bit-class number z, next to the exact x, rounded once.  A number's distance from the nearest 16-bit number changes by no
+    more than the number itself does, so |y - x| <= |z - rounded(z)| + |z - x| <= |x - rounded(x)| + 2 |z - x|, whatever the spectrum; |z - x| is held as in
+    32 bits (few directions: as the rank-one matrices above).  Panels, and both sets of tiles of the products."""
+    for k, shapes in enumerate(([(200, 230)], [(300, 300)], [(400, 500), (500, 400)], [(390 + j, 385 + 3 * j) for j in range(20)])):
+        xs = [spectrum(kind, *s, seed=7 * k + j).to(dtype) for j, s in enumerate(shapes)]
+        for x, y in zip(xs, muon.orthogonalize([x.to(DEV) for x in xs])):
+            want = plain(x)
+            few = kind in ("constant", "rank three")
+            assert off(y, want) < off(want.to(dtype), want) + 2 * (RANK_ONE_TOL if few else F32_TOL), tuple(x.shape)

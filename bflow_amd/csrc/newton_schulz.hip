@@ -18,6 +18,7 @@
 // with zeros.  X is held twice, by rows (X, for the Gram product) and by columns (Xt, the right operand of B X): both products then read
 // both operands along the contraction.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 #include "common.h"
@@ -94,6 +95,12 @@ template <int DT> __device__ __forceinline__ void store1(void* p, long long i, f
     if constexpr (DT == F32) ((float*)p)[i] = v;
     else if constexpr (DT == F16) ((_Float16*)p)[i] = (_Float16)v;
     else ((__bf16*)p)[i] = (__bf16)v;      // round to nearest even
+}
+
+// p (1 - lr decay) - rate x, the decay beside the update: 1 - lr decay in 32 bits is 1 where lr decay is below 2^-25, as it is in training (1e-4 each).
+// (An infinite weight stays what it is: its decay is that of the largest number.)
+__device__ __forceinline__ float stepped(float p, float x, float rate, float shrink) {
+    return p - fmaf(shrink, __builtin_amdgcn_fmed3f(p, -FLT_MAX, FLT_MAX), rate * x);
 }
 
 // position of (row, col) in an operand of `cols` padded columns, in halves; the lo half is 32 further
@@ -656,7 +663,7 @@ __global__ __launch_bounds__(P::THREADS, 2) void ns_leave_kernel(Exits t, const 
     const int g = g_of(ws, m.off, drop), unit = -m.ex - g;
     const float fd = ldexpf(1.f / SB, -2 * g);
     if constexpr (STEP) lr = lr_device ? *lr_device : lr;
-    const float keep = 1.f - lr * decay, rate = lr * m.size;
+    const float shrink = lr * decay, rate = lr * m.size;
     P::values(lds, [&](int n, int, int, float v[8]) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = ldexpf(fmaf(a, xv(n, e), v[e] * fd), unit);
@@ -685,7 +692,7 @@ __global__ __launch_bounds__(P::THREADS, 2) void ns_leave_kernel(Exits t, const 
 #pragma unroll
                 for (int n = 0; n < FOURS; ++n) {
                     if (!at[n]) continue;
-                    if constexpr (STEP) v[n] = make_float4(fmaf(-rate, v[n].x, p[n].x * keep), fmaf(-rate, v[n].y, p[n].y * keep), fmaf(-rate, v[n].z, p[n].z * keep), fmaf(-rate, v[n].w, p[n].w * keep));
+                    if constexpr (STEP) v[n] = make_float4(stepped(p[n].x, v[n].x, rate, shrink), stepped(p[n].y, v[n].y, rate, shrink), stepped(p[n].z, v[n].z, rate, shrink), stepped(p[n].w, v[n].w, rate, shrink));
                     *reinterpret_cast<float4*>(at[n]) = v[n];
                 }
             }
@@ -708,7 +715,7 @@ __global__ __launch_bounds__(P::THREADS, 2) void ns_leave_kernel(Exits t, const 
 #pragma unroll
         for (int n = 0; n < AT_ONCE; ++n)
             if (at[n] >= 0) {
-                if constexpr (STEP) ((float*)m.dst)[at[n]] = fmaf(-rate, v[n], p[n] * keep);
+                if constexpr (STEP) ((float*)m.dst)[at[n]] = stepped(p[n], v[n], rate, shrink);
                 else store1<DT>(m.dst, at[n], v[n]);
             }
     }
@@ -921,7 +928,7 @@ __device__ __forceinline__ void panel_body(const PanelWork& m, const PanelExit& 
             }
         }
         if (MODE == LAST) {
-            const float lr = STEP ? (nu.lr_device ? *nu.lr_device : nu.lr) : 0.f, keep = 1.f - lr * nu.decay, rate = lr * o.size;
+            const float lr = STEP ? (nu.lr_device ? *nu.lr_device : nu.lr) : 0.f, shrink = lr * nu.decay, rate = lr * o.size;
             // element by element along the user's rows, eight of a thread together
             constexpr int AT_ONCE = 8;
 #pragma unroll 1
@@ -940,7 +947,7 @@ __device__ __forceinline__ void panel_body(const PanelWork& m, const PanelExit& 
 #pragma unroll
                 for (int n = 0; n < AT_ONCE; ++n)
                     if (to[n] >= 0) {
-                        if constexpr (STEP) ((float*)o.dst)[to[n]] = fmaf(-rate, v[n], old[n] * keep);
+                        if constexpr (STEP) ((float*)o.dst)[to[n]] = stepped(old[n], v[n], rate, shrink);
                         else store1<DT>(o.dst, to[n], v[n]);
                     }
             }
@@ -1329,7 +1336,7 @@ __device__ __forceinline__ void tiny_body(const bflow_ns_matrix_t& m, const Tiny
         __syncthreads();
     }
     // the last X
-    const float lr = STEP ? (nu.lr_device ? *nu.lr_device : nu.lr) : 0.f, keep = 1.f - lr * nu.decay, rate = lr * 0.2f * sqrtf((float)s);
+    const float lr = STEP ? (nu.lr_device ? *nu.lr_device : nu.lr) : 0.f, shrink = lr * nu.decay, rate = lr * 0.2f * sqrtf((float)s);
     if constexpr (NV > 0) {
         constexpr int TOGETHER = NV == 4 ? 4 : 2;
         for (int j0 = threadIdx.x; j0 < s; j0 += TOGETHER * TINY_THREADS) {
@@ -1357,7 +1364,7 @@ __device__ __forceinline__ void tiny_body(const bflow_ns_matrix_t& m, const Tiny
                     for (int k = 0; k < NV; ++k) d = fma(Q[i * TINY_LD + k], x[k], d);
                     if (i >= r || j >= s) continue;
                     const float v = (float)(d * scale);
-                    if constexpr (STEP) ((float*)m.dst)[place(i, j)] = fmaf(-rate, v, old[u][i] * keep);
+                    if constexpr (STEP) ((float*)m.dst)[place(i, j)] = stepped(old[u][i], v, rate, shrink);
                     else store1<DT>(m.dst, place(i, j), v);
                 }
             }
@@ -1400,7 +1407,7 @@ __device__ __forceinline__ void tiny_body(const bflow_ns_matrix_t& m, const Tiny
                     for (int e = 0; e < 4; ++e)
                         if (to[n][e] >= 0) {
                             const float v = (float)d[n][e];
-                            if constexpr (STEP) ((float*)m.dst)[to[n][e]] = fmaf(-rate, v, old[n][e] * keep);
+                            if constexpr (STEP) ((float*)m.dst)[to[n][e]] = stepped(old[n][e], v, rate, shrink);
                             else store1<DT>(m.dst, to[n][e], v);
                         }
             }

@@ -11,6 +11,7 @@ A filter (out, in, kh, kw) is the matrix (out, in * kh * kw).  All filters of a 
     p = p * (1 - lr * weight_decay) - lr * 0.2 * sqrt(max(out, in * kh * kw)) * X
 
 The factor 0.2 sqrt(max) gives the update the root mean square of a usual AdamW update, so a learning rate and its schedule carry over.
+The decay is part of the update's sum and rounded with it, so that it acts, on average, at lr * weight_decay below half a step of the weights (1e-8).
 The reference trains with AdamW alone (modules/raft_spline.py:321-356).
 """
 from __future__ import annotations

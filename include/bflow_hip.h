@@ -589,6 +589,8 @@ int bflow_l1_masked_grad(const float* src, const float* tgt, const unsigned char
  *   bflow_ns_orthogonalize: dst = the last X, for every matrix of a list; dtype of src and dst: 0 fp32, 1 fp16, 2 bf16.  dst may be src.
  *   bflow_muon_step       : per matrix, all fp32:  momentum = mu momentum + src (dense);  u = src + mu momentum (nesterov) or momentum;
  *                           dst = dst (1 - lr weight_decay) - lr 0.2 sqrt(max(rows, cols)) X(u).  lr: *lr_device (device float) when given.
+ *                           The decay is added to the update before the weight is rounded, so that it acts, on average, where it is less than
+ *                           half a step of the weight (lr = weight_decay = 1e-4); without an update beside it such a decay is rounded away.
  * `m` is a HOST table, read during the call (it travels in the launches' arguments; lists of any length, 64 matrices a round).  Matrices are
  * row-major, *_ld elements from row to row, and none overlaps another but dst = src.  Arithmetic: fp16 pairs with fp32 sums (fp32-class accuracy
  * whatever the dtype; a 16-bit result is rounded once), small matrices in fp64, norms in fp64.  A list gives the same bits every time; its matrices one

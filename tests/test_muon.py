@@ -610,3 +610,43 @@ def test_16_bit_results_are_those_of_32_bits_rounded(kind, dtype):
             want = plain(x)
             few = kind in ("constant", "rank three")
             assert off(y, want) < off(want.to(dtype), want) + 2 * (RANK_ONE_TOL if few else F32_TOL), tuple(x.shape)
+
+
+@gpu
+@pytest.mark.parametrize("shapes", [[(4, 2304), (7, 1500)], [(16, 512)], [(32, 256)], [(64, 576), (576, 64), (128, 300)], [(300, 281)], [(300, 280), (280, 300)],
+                                    [(390, 388 + 4 * k) for k in range(20)]], ids=["4 and 8 rows", "16 rows", "32 rows", "panels", "products", "products by fours", "large tiles"])
+def test_decay_below_half_a_step_of_the_weights(shapes):
+    """lr = decay = 1e-4, as the training configuration has it: 1e-8 of a weight, a sixth of half its step.  It is lost on any one weight, not on all: along p,
+    p' - (p - rate X) is -lr decay p plus the weights' roundings, each uniform over at most 2^-24 |p| to either side and independent of p beside an update
+    of many steps.  Their share is sqrt(sum p^4) / sum p^2 * 2^-24 / sqrt(3), 2^-24 / sqrt(n) for Gaussian weights; X's own error, F32_TOL of an update of
+    2e-5 against weights of 0.04, lies across p but for 1 / sqrt(n) of it: 1e-8 / sqrt(n).  Six times the two together, below half of what is looked for."""
+    lr = decay = 1e-4
+    ps = [torch.nn.Parameter((0.04 * torch.randn(s, generator=torch.Generator().manual_seed(k))).to(DEV)) for k, s in enumerate(shapes)]
+    before = [p.detach().cpu().double() for p in ps]
+    for k, p in enumerate(ps):
+        p.grad = gradient(*shapes[k], seed=30 + k).to(DEV)
+    rate = torch.tensor(lr, device=DEV) if len(shapes) == 1 else lr
+    muon.Muon(ps, lr=rate, weight_decay=decay, momentum=0.0).step()
+    moved = total = n = 0
+    for p, old in zip(ps, before):
+        left = p.detach().cpu().double() - (old - lr * 0.2 * math.sqrt(max(p.shape)) * plain(p.grad))
+        moved, total, n = moved + float((left * old).sum()), total + float((old * old).sum()), n + old.numel()
+    tolerance = 6 * (2.0 ** -24 + 1e-8) / math.sqrt(n)
+    assert tolerance < 0.5 * lr * decay and abs(moved / total + lr * decay) < tolerance, moved / total
+
+
+@gpu
+@pytest.mark.parametrize("decay", [0.0, 0.1])
+def test_lost_weights_stay_alone(decay):
+    """An infinite weight stays infinite and a NaN stays one, with and without decay; their neighbours do not see them.  A matrix of each kernel."""
+    for shape in ((6, 300), (20, 40), (64, 577), (300, 280), (280, 299)):
+        p = torch.nn.Parameter(gradient(*shape, seed=1, size=1.0).to(DEV))
+        q = torch.nn.Parameter(p.detach().clone())
+        with torch.no_grad():
+            p[0, 0], p[1, 2], p[5, 39] = float("inf"), float("-inf"), float("nan")
+        p.grad = q.grad = gradient(*shape, seed=2).to(DEV)
+        muon.Muon([p, q], lr=0.1, weight_decay=decay).step()
+        assert p[0, 0] == float("inf") and p[1, 2] == float("-inf") and torch.isnan(p[5, 39])
+        with torch.no_grad():
+            p[0, 0], p[1, 2], p[5, 39] = q[0, 0], q[1, 2], q[5, 39]
+        assert torch.equal(p, q)

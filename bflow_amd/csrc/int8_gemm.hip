@@ -613,10 +613,10 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(PadArgs p) {
         unsigned x[5];
 #pragma unroll
         for (int e = 0; e < 5; ++e) x[e] = 4 * e < bytes ? w[e] : 0u;
-        u32x4 v;
+        i32x4 v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_alignbyte(x[e + 1], x[e], shift);
-        *reinterpret_cast<u32x4*>((char*)d.dst + row * d.ldd + k) = v;
+        for (int e = 0; e < 4; ++e) v[e] = (int)__builtin_amdgcn_alignbyte(x[e + 1], x[e], shift);
+        *reinterpret_cast<i32x4*>((char*)d.dst + row * d.ldd + k) = cut(v, k, d.K);      // (the last word may hold bytes of what follows the row)
     }
 }
 

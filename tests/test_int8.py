@@ -518,3 +518,20 @@ def test_both_operands_in_one_launch(B1, B2, D, h, w):
     assert all(torch.equal(x, y) for x, y in zip(got, want))
     with pytest.raises(hip.BflowHipError, match="different"):
         int8.quantize_operands(f1, f2[..., :-1] if w > 1 else f2[:, :16])
+
+
+@gpu
+@pytest.mark.parametrize("k,ldd,at,ld", [(17, 32, 0, 17), (17, 32, 1, 19), (16, 32, 3, 16), (1, 16, 2, 1), (3, 48, 1, 5), (567, 576, 0, 567), (30, 32, 3, 31), (48, 48, 1, 48), (13, 64, 0, 40)])
+def test_padded_rows_hold_zeros_behind_their_end(k, ldd, at, ld):
+    """bflow_i8_pad_rows: the row, then zeros, whatever stands behind it in memory and at whatever address; two operands in a launch, the rest untouched."""
+    r = 37
+    src = torch.randint(1, 127, (at + r * ld + k,), generator=torch.Generator().manual_seed(k), dtype=torch.int8)
+    dev = src.to(DEV)
+    room = torch.full((2, r + 2, ldd), 9, dtype=torch.int8, device=DEV)
+    lib = hip.lib()
+    items = b"".join(hip.I8_PAD.pack(dev.data_ptr() + at, room[i, 1].data_ptr(), ld, r, k, ldd) for i in range(2))
+    assert lib.bflow_i8_pad_rows(items, 2, torch.cuda.current_stream().cuda_stream) == 0
+    got = room.cpu()
+    want = torch.stack([src[at + i * ld:at + i * ld + k] for i in range(r)])
+    assert torch.equal(got[0, 1:-1, :k], want) and torch.equal(got[1], got[0])
+    assert not got[:, 1:-1, k:].any() and bool((got[:, 0] == 9).all()) and bool((got[:, -1] == 9).all())

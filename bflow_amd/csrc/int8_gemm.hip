@@ -362,11 +362,14 @@ __global__ __launch_bounds__(256) void i8_skinny_kernel(SkinnyArgs g) {
     }
 }
 
+// A launch has fewer than 2^32 threads along x.
+bool fits(long long wgs, int threads) { return wgs * threads < (1LL << 32); }
+
 template <class Tile>
 int launch_tiles(GemmArgs g, int dtype, unsigned batch, hipStream_t st) {
     g.tiles_m = ceil_div(g.M, Tile::M);
     g.tiles_n = ceil_div(g.N, Tile::N);
-    BFLOW_REQUIRE((long long)g.tiles_m * g.tiles_n < (1LL << 30), BFLOW_E_LIMIT, "i8_gemm: too many tiles");
+    BFLOW_REQUIRE(fits((long long)g.tiles_m * g.tiles_n, Tile::THREADS), BFLOW_E_LIMIT, "i8_gemm: too many tiles for %d x %d", g.M, g.N);
     const auto kernel = dtype == F32 ? i8_gemm_kernel<Tile, F32> : dtype == F16 ? i8_gemm_kernel<Tile, F16> : i8_gemm_kernel<Tile, BF16>;
     if (Tile::LDS > 65536) {
         const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, Tile::LDS);
@@ -382,7 +385,7 @@ int launch_stream(const GemmArgs& g, int dtype, unsigned batch, hipStream_t st) 
     per = per > STREAM_ROWS / 32 ? STREAM_ROWS / 32 : per;
     s.rows = (int)per * 32;
     s.ranges = ceil_div(g.M, s.rows);
-    BFLOW_REQUIRE((long long)s.panels * s.ranges < (1LL << 30), BFLOW_E_LIMIT, "i8_gemm: too many panels");
+    BFLOW_REQUIRE(fits((long long)s.panels * s.ranges, 256), BFLOW_E_LIMIT, "i8_gemm: too many panels for %d x %d", g.M, g.N);
     const bool one = g.K <= CHUNK;
     const auto kernel = one ? (dtype == F32 ? i8_stream_kernel<1, F32> : dtype == F16 ? i8_stream_kernel<1, F16> : i8_stream_kernel<1, BF16>)
                             : (dtype == F32 ? i8_stream_kernel<2, F32> : dtype == F16 ? i8_stream_kernel<2, F16> : i8_stream_kernel<2, BF16>);
@@ -391,6 +394,7 @@ int launch_stream(const GemmArgs& g, int dtype, unsigned batch, hipStream_t st) 
 }
 template <int RT>
 int launch_skinny(const SkinnyArgs& g, int dtype, unsigned batch, hipStream_t st) {
+    BFLOW_REQUIRE(fits((g.M + 15LL) / 16, 256), BFLOW_E_LIMIT, "i8_gemm: %d rows beside %d, fewer than 2^28 are taken", g.M, g.F);
     const auto kernel = dtype == F32 ? i8_skinny_kernel<RT, F32> : dtype == F16 ? i8_skinny_kernel<RT, F16> : i8_skinny_kernel<RT, BF16>;
     hipLaunchKernelGGL(kernel, dim3((g.M + 15) / 16, batch), dim3(256), 0, st, g);
     return launch_status("i8_gemm");
@@ -565,6 +569,7 @@ extern "C" int bflow_i8_gemm(const bflow_i8_gemm_t* d, bflow_stream_t stream) {
     BFLOW_REQUIRE(d->M >= 1 && d->N >= 1 && d->K >= 1 && d->batch0 >= 1 && d->batch1 >= 1, BFLOW_E_ARG, "i8_gemm: sizes %d x %d x %d, batch %d x %d", d->M, d->N, d->K,
                   d->batch0, d->batch1);
     BFLOW_REQUIRE(d->K <= BFLOW_I8_MAX_K, BFLOW_E_LIMIT, "i8_gemm: K = %d > %d (32-bit sums)", d->K, BFLOW_I8_MAX_K);
+    BFLOW_REQUIRE(d->M <= BFLOW_I8_MAX_SIZE && d->N <= BFLOW_I8_MAX_SIZE, BFLOW_E_LIMIT, "i8_gemm: %d x %d, a side above %d", d->M, d->N, BFLOW_I8_MAX_SIZE);
     BFLOW_REQUIRE(d->dtype >= F32 && d->dtype <= BF16, BFLOW_E_ARG, "i8_gemm: dtype %d", d->dtype);
     const int row = (d->K + 15) & ~15;
     BFLOW_REQUIRE(d->lda >= row && d->ldb >= row && d->lda <= BFLOW_I8_MAX_LD && d->ldb <= BFLOW_I8_MAX_LD && d->ldo >= d->N, BFLOW_E_ARG,
@@ -640,6 +645,7 @@ extern "C" int bflow_i8_quantize_rows(const void* x, int dtype, long long ld, lo
     BFLOW_REQUIRE(rows >= 1 && K >= 1 && ld >= 0 && ldq >= K && ldq % 16 == 0 && (uintptr_t)q % 16 == 0, BFLOW_E_ARG, "i8_quantize_rows: %lld rows of %d, strides %lld, %d", rows, K, ld,
                   ldq);
     BFLOW_REQUIRE(dtype >= F32 && dtype <= BF16, BFLOW_E_ARG, "i8_quantize_rows: dtype %d", dtype);
+    BFLOW_REQUIRE(K <= BFLOW_I8_MAX_SIZE && ldq <= BFLOW_I8_MAX_SIZE, BFLOW_E_LIMIT, "i8_quantize_rows: rows of %d, %d apart, above %d", K, ldq, BFLOW_I8_MAX_SIZE);
     const auto kernel = dtype == F32 ? quantize_rows_kernel<F32> : dtype == F16 ? quantize_rows_kernel<F16> : quantize_rows_kernel<BF16>;
     const long long wgs = (rows + 3) / 4;
     hipLaunchKernelGGL(kernel, dim3((unsigned)(wgs < 65536 ? wgs : 65536)), dim3(256), 0, (hipStream_t)stream, x, ld, rows, K, q, ldq, scale);
@@ -669,6 +675,7 @@ extern "C" int bflow_i8_quantize_maps(const bflow_i8_maps_t* items, int count, i
         most = m.rows[i] > most ? m.rows[i] : most;
     }
     BFLOW_REQUIRE(maps <= 65535, BFLOW_E_LIMIT, "i8_quantize_pixels: %lld maps > 65535", maps);
+    BFLOW_REQUIRE(fits((most + 63) / 64, plain ? 1024 : 256), BFLOW_E_LIMIT, "i8_quantize_pixels: %d places of %d x %d pixels", most, h, w);
     const dim3 grid((most + 63) / 64, (unsigned)maps);
     if (plain) hipLaunchKernelGGL(quantize_pixels_kernel, grid, dim3(1024), 0, (hipStream_t)stream, m, D, h, w);
     else hipLaunchKernelGGL(quantize_packed_kernel, grid, dim3(256), 0, (hipStream_t)stream, m, D / 32, h, w);

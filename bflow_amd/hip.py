@@ -103,6 +103,7 @@ class NormDesc(ctypes.Structure):
 I8_GEMM = struct.Struct("5Q11q8if4x")       # a b scale_a scale_b out | strides 0, 1 of a, b, sa, sb, out; ldo | lda ldb M N K batch0 batch1 dtype | alpha
 I8_MAPS = struct.Struct("5Q4i")             # x x_hi x_lo q scale | np B tiled 0
 I8_PAD = struct.Struct("2Q2q2i")            # src dst | ld rows | K ldd
+I8_MAX_SIZE = 0x7ffffe00                    # BFLOW_I8_MAX_SIZE: what passes it does not reach the C entries' ints
 
 
 # struct bflow_ns_matrix (include/bflow_hip.h), as rows of a host table

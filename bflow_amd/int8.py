@@ -22,9 +22,16 @@ def _padded(k: int) -> int:
     return (k + 15) & ~15
 
 
+def _sizes(what: str, *sizes: int):
+    if any(n > hip.I8_MAX_SIZE for n in sizes):
+        raise hip.BflowHipError(f"{what}: sizes {sizes}, at most {hip.I8_MAX_SIZE} are taken")
+
+
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """x (..., rows, K) float32 / float16 / bfloat16 -> int8 (..., rows, K), float32 scales (..., rows).  The rows of the result start 16 bytes
-    apart or a multiple (zeros in between), as `matmul` wants them; x (K,) is one row."""
+    apart or a multiple (zeros in between), as `matmul` wants them; x (K,) is one row.  K is at most 2^31 - 512."""
+    if isinstance(x, torch.Tensor) and x.dim():
+        _sizes("quantize_rows", x.shape[-1])
     hip._dev(x, None, "x", contiguous=False)
     if x.dtype not in hip.FLOAT_CODES or x.dim() < 1:
         raise hip.BflowHipError(f"quantize_rows: rows of {sorted(str(d) for d in hip.FLOAT_CODES)}, got {tuple(x.shape)} {x.dtype}")
@@ -43,7 +50,8 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 
 def quantize_pixels(maps: torch.Tensor, tiled: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
     """maps (..., D, h, w) float32, D a multiple of 16 -> int8 (..., P, D), float32 scales (..., P): P = h * w pixels in order, or (tiled) the
-    `hip.tiled_plane_size(h, w)` places of the tiled correlation volume, those outside the map zero with scale 0."""
+    `hip.tiled_plane_size(h, w)` places of the tiled correlation volume, those outside the map zero with scale 0.  Fewer than 2^28 places, 65535 maps
+    at most."""
     lead, D, h, w = _maps_shape(maps)
     maps = maps.contiguous()
     return _quantize_maps([(maps.data_ptr(), 0, 0, 0, lead, tiled)], maps.device, D, h, w)[0]
@@ -75,6 +83,7 @@ def quantize_operands(f1: torch.Tensor, f2: torch.Tensor, packed_hw: Optional[Tu
 def _maps_shape(maps):
     if maps.dim() < 3:
         raise hip.BflowHipError(f"quantize_pixels: maps (..., D, h, w), got {tuple(maps.shape)}")
+    _sizes("quantize_pixels", maps.shape[-3], maps.shape[-2] * maps.shape[-1])
     hip._dev(maps, torch.float32, "maps", contiguous=False)
     shape = maps.shape
     return (tuple(shape[:-3]),) + tuple(shape[-3:])
@@ -185,13 +194,16 @@ def _fold(batch, strides):
 def matmul(a: torch.Tensor, scale_a: torch.Tensor, b: torch.Tensor, scale_b: torch.Tensor, out_dtype: torch.dtype = torch.float32, alpha: float = 1.0,
            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """a (..., M, K) int8 with scales (..., M), b (..., N, K) int8 with scales (..., N) -> (..., M, N) of out_dtype (float32, float16, bfloat16):
-    alpha * scale_a * scale_b * (a @ b^T), rounded once.  Leading dimensions broadcast.  Operands whose rows are not spaced by multiples of 16 bytes
-    are copied first (quantize_rows spaces them).  out: where the result goes, dense in its last dimension.  Not differentiable."""
+    (alpha * scale_a) * scale_b * (a @ b^T): sums exact, rounded to 32 bits, as are the products with the scales, then to out_dtype.  Leading dimensions
+    broadcast.  Operands whose rows are not spaced by multiples of 16 bytes are copied first (quantize_rows spaces them).  out: where the result goes,
+    dense in its last dimension.  Refused: K above 131071, more than 65535 matrices, 2^28 rows or more on one side where the other has at most 32.
+    Not differentiable."""
     ashape, bshape = a.shape, b.shape
     if len(ashape) < 2 or len(bshape) < 2 or ashape[-1] != bshape[-1]:
         raise hip.BflowHipError(f"matmul: rows of the same length, got {tuple(ashape)} and {tuple(bshape)}")
     if scale_a.shape != ashape[:-1] or scale_b.shape != bshape[:-1]:
         raise hip.BflowHipError(f"matmul: a scale for each row, got {tuple(scale_a.shape)}, {tuple(scale_b.shape)} for {tuple(ashape)}, {tuple(bshape)}")
+    _sizes("matmul", ashape[-2], bshape[-2], ashape[-1])
     for t, kind, name in ((a, torch.int8, "a"), (b, torch.int8, "b"), (scale_a, torch.float32, "scale_a"), (scale_b, torch.float32, "scale_b")):
         hip._dev(t, kind, name, contiguous=False)
     code = hip.FLOAT_CODES.get(out_dtype)

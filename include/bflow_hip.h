@@ -631,8 +631,10 @@ int bflow_muon_step(const bflow_ns_matrix_t* m, int count, int steps, double a, 
  *   bflow_i8_quantize_maps : the same for one or two operands (a HOST table) of one D, h, w and form in a launch: both sides of a volume
  * Quantisation: scale = max|x| / 127, q = the nearest whole number to 127 x / max|x|, halves to even, exactly.  A row of zeros has scale 0; a row
  * with an infinity or a NaN has q = 0 and an infinite or NaN scale, so that its products are NaN.                                              */
-#define BFLOW_I8_MAX_K  131071
-#define BFLOW_I8_MAX_LD (1 << 22)
+#define BFLOW_I8_MAX_K    131071
+#define BFLOW_I8_MAX_LD   (1 << 22)
+#define BFLOW_I8_MAX_SIZE 0x7ffffe00      /* M, N; numbers of a quantised row.  Launches take fewer than 2^32 threads: with at most 32 rows on one side of
+                                           * a product, fewer than 2^28 on the other; fewer than 2^28 places of a map (2^30 of a packed one)        */
 typedef struct bflow_i8_gemm_desc {
     const void *a, *b;
     const float *scale_a, *scale_b;

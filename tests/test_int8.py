@@ -535,3 +535,26 @@ def test_padded_rows_hold_zeros_behind_their_end(k, ldd, at, ld):
     want = torch.stack([src[at + i * ld:at + i * ld + k] for i in range(r)])
     assert torch.equal(got[0, 1:-1, :k], want) and torch.equal(got[1], got[0])
     assert not got[:, 1:-1, k:].any() and bool((got[:, 0] == 9).all()) and bool((got[:, -1] == 9).all())
+
+
+def test_sizes_beyond_the_entries_integers_are_refused():
+    """Sizes that a C int would cut off, or a kernel's 32-bit loop or a launch cannot count to: an error, before anything is allocated or launched."""
+    one, s = torch.zeros(1, 16, dtype=torch.int8), torch.zeros(1)
+    for n in ((1 << 31) - 256, (1 << 31) + 5, (1 << 32) + 3):
+        for call in (lambda: int8.quantize_rows(torch.zeros(1, 1).expand(1, n)), lambda: int8.matmul(one.expand(n, 16), s.expand(n), one, s),
+                     lambda: int8.matmul(one, s, one.expand(n, 16), s.expand(n)), lambda: int8.matmul(one[:, :1].expand(1, n), s, one[:, :1].expand(1, n), s),
+                     lambda: int8.quantize_pixels(torch.zeros(1).expand(16, n, 1)), lambda: int8.quantize_pixels(torch.zeros(1).expand(16, 1 << 20, 1 << 12)),
+                     lambda: int8.quantize_pixels(torch.zeros(1).expand(n, 1, 1))):
+            with pytest.raises(hip.BflowHipError, match="at most"):
+                call()
+    lib = hip.lib()
+    top = (1 << 31) - 1
+    for K, ldq in ((top - 15, top - 15), (16, top - 15)):
+        assert lib.bflow_i8_quantize_rows(256, 0, K, 4, K, 256, ldq, 256, None) == -2 and b"quantize_rows" in lib.bflow_last_error_string()
+
+    def gemm(M, N):
+        return lib.bflow_i8_gemm(hip.I8_GEMM.pack(256, 256, 256, 256, 256, *[0] * 10, N, 16, 16, M, N, 16, 1, 1, 0, 1.0), None)
+    for M, N in ((top, 1), (1, top), (top, top), (1 << 28, 3), (32, 1 << 28), (1 << 24, 1 << 24), (top - 511, top - 511)):
+        assert gemm(M, N) == -2 and b"i8_gemm" in lib.bflow_last_error_string()
+    for h, w, hi in ((1 << 14, (1 << 14) - 1, 0), (1, (1 << 27) + 8, 0), (1, (1 << 28) - 1, 256)):
+        assert lib.bflow_i8_quantize_pixels(0 if hi else 256, hi, hi, 1 << 28, 1, 32, h, w, 1, 256, 256, None) == -2 and b"places" in lib.bflow_last_error_string()

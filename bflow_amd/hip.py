@@ -110,6 +110,8 @@ I8_MAX_SIZE = 0x7ffffe00                    # BFLOW_I8_MAX_SIZE: what passes it 
 NS_MATRIX = np.dtype([("src", np.uint64), ("dst", np.uint64), ("momentum", np.uint64), ("src_ld", np.int64), ("dst_ld", np.int64), ("rows", np.int32),
                       ("cols", np.int32)])
 
+NS_MAX_SIDE, NS_MAX_NUMBERS = 1 << 20, 1 << 30      # BFLOW_NS_MAX_SIDE; of one matrix
+
 _lib = None
 
 

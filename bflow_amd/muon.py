@@ -39,6 +39,14 @@ def _as_matrix(t: torch.Tensor, what: str) -> torch.Tensor:
     return t.contiguous().view(t.shape[0], math.prod(t.shape[1:]))
 
 
+def _refused_size(shape: Sequence[int]) -> str:
+    """Why a matrix or filter of this shape is too large for the kernels; empty where it is not."""
+    rows, cols = shape[0], math.prod(shape[1:])
+    if max(rows, cols) > hip.NS_MAX_SIDE or rows * cols > hip.NS_MAX_NUMBERS:
+        return f"shape {tuple(shape)}: at most {hip.NS_MAX_SIDE} rows or columns and {hip.NS_MAX_NUMBERS} numbers are taken"
+    return ""
+
+
 def _table(entries: Sequence[Tuple[int, int, int, int, int, int, int]]) -> np.ndarray:
     return np.array(entries, dtype=hip.NS_MATRIX)
 
@@ -59,7 +67,7 @@ def orthogonalize(matrices: Sequence[torch.Tensor], steps: int = STEPS, coeffici
     Sums are held in 32 bits, products in fp16 pairs (fp32-class whatever the type; small matrices in 64 bits); a 16-bit result is rounded once.
     Tensors of more than two dimensions are taken as (shape[0], everything else).  The results of one type share a buffer.  An empty matrix stays
     empty, a zero matrix zero; one with a NaN or an infinity becomes all NaN.  The same list gives the same bits; a matrix in another list may be
-    tiled another way and differ by roundings.  Not differentiable: the results carry no graph."""
+    tiled another way and differ by roundings.  At most 2^20 rows or columns, 2^30 numbers.  Not differentiable: the results carry no graph."""
     _check_numbers(steps, coefficients, eps)
     if isinstance(matrices, torch.Tensor):
         raise hip.BflowHipError("orthogonalize takes a list of matrices")
@@ -68,6 +76,8 @@ def orthogonalize(matrices: Sequence[torch.Tensor], steps: int = STEPS, coeffici
     for i, t in enumerate(matrices):
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
             hip._dev(t, None, f"matrix {i}", contiguous=False)                    # says why not
+        if t.dim() > 1 and t.numel() > hip.NS_MAX_SIDE and _refused_size(t.shape):
+            raise hip.BflowHipError(f"matrix {i}: {_refused_size(t.shape)}")
         key = (t.dtype, t.device)
         if key not in groups:
             if t.dtype not in hip.FLOAT_CODES:
@@ -106,8 +116,8 @@ class Muon(torch.optim.Optimizer):
     """Muon for matrices and filters; AdamW for the groups marked `adamw=True` (biases, the scales and shifts of norms).
 
     lr may be a float32 scalar tensor on the parameters' device: the kernels read it when they run, so a captured graph follows a schedule.
-    Parameters, gradients and states are float32.  capturable: a step may be captured, after a first one that creates the states; the AdamW step
-    counters live on the device (torch.optim.AdamW)."""
+    Parameters, gradients and states are float32; a matrix has at most 2^20 rows or columns and 2^30 numbers.  capturable: a step may be captured,
+    after a first one that creates the states; the AdamW step counters live on the device (torch.optim.AdamW)."""
 
     def __init__(self, params, lr=1e-3, momentum: float = 0.95, weight_decay: float = 0.0, nesterov: bool = True, steps: int = STEPS,
                  coefficients: Sequence[float] = COEFFICIENTS, eps: float = EPS, betas: Tuple[float, float] = (0.9, 0.999), adamw_eps: float = 1e-8,
@@ -132,6 +142,8 @@ class Muon(torch.optim.Optimizer):
                 why = f"parameters are float32, got {p.dtype}"
             elif not group["adamw"] and (p.dim() < 2 or not p.is_contiguous()):
                 why = f"a parameter of shape {tuple(p.shape)}, strides {p.stride()}: dense matrices or filters; put the others into a group with adamw=True"
+            elif not group["adamw"] and _refused_size(p.shape):
+                why = _refused_size(p.shape)
             if why is not None:
                 self.param_groups.pop()
                 raise hip.BflowHipError(f"Muon: {why}")

@@ -650,3 +650,21 @@ def test_lost_weights_stay_alone(decay):
         with torch.no_grad():
             p[0, 0], p[1, 2], p[5, 39] = q[0, 0], q[1, 2], q[5, 39]
         assert torch.equal(p, q)
+
+
+def test_matrices_beyond_the_kernels_are_refused_early():
+    """Where a parameter is given to the optimiser, not in its first step, and with the same error whatever the size."""
+    long, many = torch.nn.Parameter(torch.zeros((1 << 20) + 1, 1)), torch.nn.Parameter(torch.empty(1 << 16, (1 << 14) + 1, device="meta"))
+    for p in (long, many, torch.nn.Parameter(torch.empty(1 << 33, 2, device="meta")), torch.nn.Parameter(torch.empty(4, 1 << 11, 1 << 10, device="meta"))):
+        with pytest.raises(hip.BflowHipError, match="at most"):
+            muon.Muon([p])
+        assert muon.Muon([{"params": [p], "adamw": True}])
+    assert muon.Muon([torch.nn.Parameter(torch.empty(1 << 20, 1 << 10, device="meta"))])
+
+
+@gpu
+def test_orthogonalize_refuses_what_is_too_large():
+    one = torch.zeros(1, 1, device=DEV)
+    for shape in (((1 << 20) + 1, 2), (2, (1 << 32) + 7), (1 << 16, 1 << 16), (1 << 40, 1)):
+        with pytest.raises(hip.BflowHipError, match="matrix 1: .*at most"):
+            muon.orthogonalize([one, one.expand(shape)])

@@ -65,9 +65,9 @@ def orthogonalize(matrices: Sequence[torch.Tensor], steps: int = STEPS, coeffici
     """Newton-Schulz steps on every matrix of a list: new tensors of the same shapes and types (float32, float16 or bfloat16, mixed as you like).
 
     Sums are held in 32 bits, products in fp16 pairs (fp32-class whatever the type; small matrices in 64 bits); a 16-bit result is rounded once.
-    Tensors of more than two dimensions are taken as (shape[0], everything else).  The results of one type share a buffer.  An empty matrix stays
-    empty, a zero matrix zero; one with a NaN or an infinity becomes all NaN.  The same list gives the same bits; a matrix in another list may be
-    tiled another way and differ by roundings.  At most 2^20 rows or columns, 2^30 numbers.  Not differentiable: the results carry no graph."""
+    Tensors of more than two dimensions are taken as (shape[0], everything else).  An empty matrix stays empty, a zero matrix zero; one with a NaN or
+    an infinity becomes all NaN.  The same list gives the same bits; a matrix in another list may be tiled another way and differ by roundings.  At
+    most 2^20 rows or columns, 2^30 numbers.  Not differentiable: the results carry no graph."""
     _check_numbers(steps, coefficients, eps)
     if isinstance(matrices, torch.Tensor):
         raise hip.BflowHipError("orthogonalize takes a list of matrices")
@@ -87,26 +87,16 @@ def orthogonalize(matrices: Sequence[torch.Tensor], steps: int = STEPS, coeffici
     results: List[torch.Tensor] = [None] * len(matrices)
     held = []                                             # contiguous copies live until the launches are enqueued
     for (dtype, device), members in groups.items():
-        # one buffer for the results of a type, each on a boundary of 64 elements: an allocation each would cost as much as the launches
-        starts, total = [], 0
+        entries = []
         for i in members:
-            starts.append(total)
-            total += (matrices[i].numel() + 63) & ~63
-        room = torch.empty(total, dtype=dtype, device=device)
-        base, size, entries = room.data_ptr(), room.element_size(), []
-        for i, start in zip(members, starts):
             t = matrices[i]
             x = _as_matrix(t, f"matrix {i}")
-            shape, rows, cols = t.shape, x.shape[0], x.shape[1]
-            strides, n = [], 1
-            for d in reversed(shape):
-                strides.append(n)
-                n *= max(d, 1)
-            results[i] = room.as_strided(shape, strides[::-1], start)
+            y = results[i] = torch.empty_like(t, memory_format=torch.contiguous_format)
+            rows, cols = x.shape
             if rows and cols:
                 if x is not t:
                     held.append(x)
-                entries.append((x.data_ptr(), base + start * size, 0, x.stride(0) if rows > 1 else cols, cols, rows, cols))
+                entries.append((x.data_ptr(), y.data_ptr(), 0, x.stride(0) if rows > 1 else cols, cols, rows, cols))
         if entries:
             hip.ns_orthogonalize(_table(entries), dtype, device, int(steps), coefficients, eps)
     return results

@@ -668,3 +668,20 @@ def test_orthogonalize_refuses_what_is_too_large():
     for shape in (((1 << 20) + 1, 2), (2, (1 << 32) + 7), (1 << 16, 1 << 16), (1 << 40, 1)):
         with pytest.raises(hip.BflowHipError, match="matrix 1: .*at most"):
             muon.orthogonalize([one, one.expand(shape)])
+
+
+@gpu
+def test_results_are_tensors_of_their_own():
+    """Writing into one result neither bumps the version of another that a graph has saved nor touches it; each holds its own storage."""
+    xs = [gradient(30, 50, seed=k).to(DEV) for k in range(3)] + [gradient(300, 20, seed=4).to(DEV), gradient(2, 3, seed=5).to(DEV)]
+    ys = muon.orthogonalize(xs)
+    w = torch.ones(30, 50, device=DEV, requires_grad=True)
+    loss = (w * ys[0]).sum()
+    keep = [y.clone() for y in ys]
+    for y in ys[1:]:
+        y.fill_(7.0)
+    loss.backward()
+    assert torch.equal(w.grad, keep[0]) and torch.equal(ys[0], keep[0])
+    for y, x in zip(ys, xs):
+        assert y._base is None and y.storage_offset() == 0 and y.untyped_storage().nbytes() == 4 * x.numel()
+    assert len({y.untyped_storage().data_ptr() for y in ys}) == len(ys)

@@ -538,3 +538,21 @@ def test_window_descriptors_of_the_twostep_assembly_on_the_host():
     asm.version = 0
     with pytest.raises(AssertionError, match="extended_voxel_grid"):
         asm.window_descriptor(ev, int(ts[0][0]), int(ts[0][1]))
+
+
+def test_hip_code_is_compiled_without_packed_32_bit_instructions():
+    """Every compiler line of the repository, tools and their instructions among them, names the flag (some forms of those instructions have given wrong
+    results); link lines compile nothing."""
+    seen = 0
+    for folder, dirs, files in os.walk(ROOT):
+        dirs[:] = [d for d in dirs if not d.startswith((".", "_")) and d not in ("gpurun_out", "tests")]
+        for name in files:
+            if not name.endswith((".py", ".sh", ".hip", ".h")):
+                continue
+            text = open(os.path.join(folder, name)).read().replace("\\\n", " ")
+            for line in re.findall(r"[^\n]*--offload-arch=gfx950.*?(?:check=True|\n)", text, re.S if name.endswith(".py") else 0):
+                if "-O3" not in line:
+                    continue
+                seen += 1
+                assert "-packed-fp32-ops" in line, (name, line)
+    assert seen >= 13

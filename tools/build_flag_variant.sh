@@ -14,7 +14,7 @@ for o in "$ROOT"/bflow_amd/lib/*.o; do
   [ $skip = 1 ] || OBJS+=("$o")
 done
 for f in "$@"; do
-  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -fvisibility=hidden -munsafe-fp-atomics $FLAGS -c "$ROOT/bflow_amd/csrc/$f" -o "$TMP/${f%.hip}.o" &
+  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -fvisibility=hidden -munsafe-fp-atomics -Xclang -target-feature -Xclang -packed-fp32-ops $FLAGS -c "$ROOT/bflow_amd/csrc/$f" -o "$TMP/${f%.hip}.o" &
   OBJS+=("$TMP/${f%.hip}.o")
 done
 wait

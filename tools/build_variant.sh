@@ -9,7 +9,7 @@ mkdir -p "$TMP/bflow_amd/csrc" "$TMP/include" "$ROOT/bflow_amd/lib/ab"
 for f in $(git -C "$ROOT" ls-tree --name-only "$REV" bflow_amd/csrc/ include/); do git -C "$ROOT" show "$REV:$f" > "$TMP/$f"; done
 OBJS=()
 for f in "$TMP"/bflow_amd/csrc/*.hip; do
-  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -fvisibility=hidden -munsafe-fp-atomics -c "$f" -o "${f%.hip}.o" &
+  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -fvisibility=hidden -munsafe-fp-atomics -Xclang -target-feature -Xclang -packed-fp32-ops -c "$f" -o "${f%.hip}.o" &
   OBJS+=("${f%.hip}.o")
 done
 wait

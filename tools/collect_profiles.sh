@@ -10,7 +10,7 @@ R=r06
 cd /tmp && export TMPDIR=/tmp
 # the measurement binaries are git-ignored: build them HERE if the snapshot did not carry them (round 5 lost its calibration pass to that)
 for t in fp8_cross store_patterns; do
-  [ -x "$REPO/tools/micro/$t" ] || /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -w -o "$REPO/tools/micro/$t" "$REPO/tools/micro/$t.hip" || { echo "collect_profiles: cannot build tools/micro/$t" >&2; exit 1; }
+  [ -x "$REPO/tools/micro/$t" ] || /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -w -o "$REPO/tools/micro/$t" "$REPO/tools/micro/$t.hip" || { echo "collect_profiles: cannot build tools/micro/$t" >&2; exit 1; }
 done
 PROBE="python $REPO/tools/roofline_probe.py"
 KEYS="${KEYS:-roofline roofline_update_conv roofline_corr_build roofline_corr_build_split roofline_lookup roofline_lookup_c4_shard roofline_corr_build_c5 roofline_conv3x3_c4 roofline_conv_stream_nin_c4 roofline_gru_conv_c4}"     # (KEYS=... QUICK=1: a dry run of the counter passes on a subset, nothing copied to profiles/)

@@ -8,7 +8,7 @@ mkdir -p "$ROOT/bflow_amd/lib/ab"
 OTHERS=$(ls "$ROOT"/bflow_amd/lib/*.o | grep -v corr_stream.o)
 for spec in "$@"; do
   name="${spec%%:*}"; flags="${spec#*:}"
-  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -fvisibility=hidden -munsafe-fp-atomics $flags \
+  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -fvisibility=hidden -munsafe-fp-atomics -Xclang -target-feature -Xclang -packed-fp32-ops $flags \
      -c "$ROOT/bflow_amd/csrc/corr_stream.hip" -o "/tmp/cs_$name.o" &
 done
 wait

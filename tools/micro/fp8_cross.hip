@@ -4,7 +4,7 @@
 //      kernel needs: a dot product is invariant under a common permutation of k) and that zero scale operands mean "unscaled".
 //  (2) rate: every CU, 2 waves per SIMD, random operands: per 32-channel block either 6 fp16 MFMAs (today's 3-pass split) or
 //      2 fp16 MFMAs + 1 fp8 K=64 MFMA; wall time, shader clock (s_memtime / wall clock).
-//   hipcc --offload-arch=gfx950 -O3 -o fp8_cross fp8_cross.hip && ./fp8_cross
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o fp8_cross fp8_cross.hip && ./fp8_cross
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cmath>

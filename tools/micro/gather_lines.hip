@@ -6,7 +6,7 @@
 // PATCHES_WG patches (= 14 pairs of the kernel: 7 planes x 2 pixels) in flight, waits for them (s_waitcnt vmcnt(0) + barrier), and takes the next
 // -- 8 workgroups per CU like the kernel (20 KB of LDS each).  Modes: stream (consecutive lines, the DRAM-friendly upper bound), runs 3x3, runs
 // 4x3, single random lines.  Prints TB/s of LINE bytes.
-//   hipcc --offload-arch=gfx950 -O3 -o gather_lines gather_lines.hip && ./gather_lines
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o gather_lines gather_lines.hip && ./gather_lines
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

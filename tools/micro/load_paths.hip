@@ -5,7 +5,7 @@
 //   both    half of the waves each
 // Every workgroup (8 waves, one per CU) re-reads its own 96-KB slice (L2-resident: 3 MB per XCD); `inflight` loads per wave between
 // waits.  Prints bytes per clock per CU from the shader clock (s_memtime) of the kernel.
-//   hipcc --offload-arch=gfx950 -O3 -o load_paths load_paths.hip && ./load_paths
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o load_paths load_paths.hip && ./load_paths
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

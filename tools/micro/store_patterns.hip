@@ -7,7 +7,7 @@
 //               write ADJACENT panels of the SAME rows (best-case DRAM-page locality for this tile shape)
 // each with per-lane store width 4 B (one register = two full lines per wave instruction, what K5 issues today) or 16 B (lane = 16 B of a
 // line, 8 full lines per wave instruction, what an LDS-transposed epilogue would issue), and aux = 0 / nt.
-//   hipcc --offload-arch=gfx950 -O3 -o store_patterns store_patterns.hip && ./store_patterns
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o store_patterns store_patterns.hip && ./store_patterns
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

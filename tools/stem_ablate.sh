@@ -8,7 +8,7 @@ mkdir -p "$ROOT/bflow_amd/lib/ab"
 if [ "$MODE" = build ]; then
   for b in $BITS; do
     if [ -n "${STEMP:-}" ]; then DEFS="-DSTEM_ABL=0 -DSTEMP_ABL=$b"; else DEFS="-DSTEM_ABL=$b"; fi
-    /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -fvisibility=hidden -munsafe-fp-atomics $DEFS -c "$ROOT/bflow_amd/csrc/conv_split.hip" -o "/tmp/stem_abl_$b.o" &
+    /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -fvisibility=hidden -munsafe-fp-atomics -Xclang -target-feature -Xclang -packed-fp32-ops $DEFS -c "$ROOT/bflow_amd/csrc/conv_split.hip" -o "/tmp/stem_abl_$b.o" &
   done
   wait
   for b in $BITS; do

@@ -6,7 +6,7 @@ MODE="$1"; BITS="$2"
 mkdir -p "$ROOT/bflow_amd/lib/ab"
 if [ "$MODE" = build ]; then
   for b in $BITS; do
-    /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -fvisibility=hidden -munsafe-fp-atomics -DWG_ABL=$b -c "$ROOT/bflow_amd/csrc/wgrad_halo.hip" -o "/tmp/wg_abl_$b.o" &
+    /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -fvisibility=hidden -munsafe-fp-atomics -Xclang -target-feature -Xclang -packed-fp32-ops -DWG_ABL=$b -c "$ROOT/bflow_amd/csrc/wgrad_halo.hip" -o "/tmp/wg_abl_$b.o" &
   done
   wait
   for b in $BITS; do

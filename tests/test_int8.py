@@ -558,3 +558,31 @@ def test_sizes_beyond_the_entries_integers_are_refused():
         assert gemm(M, N) == -2 and b"i8_gemm" in lib.bflow_last_error_string()
     for h, w, hi in ((1 << 14, (1 << 14) - 1, 0), (1, (1 << 27) + 8, 0), (1, (1 << 28) - 1, 256)):
         assert lib.bflow_i8_quantize_pixels(0 if hi else 256, hi, hi, 1 << 28, 1, 32, h, w, 1, 256, 256, None) == -2 and b"places" in lib.bflow_last_error_string()
+
+
+@gpu
+@pytest.mark.parametrize("T,B,D,h,w", [(1, 1, 32, 3, 5), (4, 1, 256, 24, 40), (2, 3, 128, 13, 19), (3, 2, 256, 9, 31)])
+@pytest.mark.parametrize("name", ["i8", "i8/w"])
+def test_volume_of_packed_operands(T, B, D, h, w, name):
+    """What the model's forward pass builds: the encoder's planes, references and targets of several samples behind one another in one tensor, quantised as the
+    values that they hold (hi + lo * 2^-11); against 64 bits, and the block on them against the block on maps of those values."""
+    f1, f2 = maps(T, B, D, h, w, 7)
+    planes = hip.split_pack(torch.cat([f1, f2.flatten(0, 1)]).flatten(-2).to(DEV))
+    held = (planes[0].double() + planes[1].double() / 2048)[:, :, :h * w].permute(0, 2, 1, 3).reshape(B * (1 + T), h * w, D).cpu()
+    assert torch.equal(held.float().double(), held)
+    (q1, s1), (q2, s2) = quantised(held[:B]), quantised(held[B:].view(T, B, h * w, D))
+    want = product(q1, s1, q2, s2, float(np.float32(1 / math.sqrt(D))))
+    kind = torch.float16 if name == "i8" else torch.float32
+    packed = lambda: CorrComputation.from_packed(planes[:, :B], planes[:, B:], B, D, h, w, [2] * T)
+    vol = packed().get_correlation_volume(tiled=True, precision=name)
+    order = tile_order(h, w)
+    inside = order >= 0
+    assert vol.shape == (T, B, h * w, len(order)) and not vol[..., ~inside].any()
+    check(vol[..., inside].contiguous(), want[..., order[inside]], kind)
+    room = torch.empty_like(vol)
+    assert packed().get_correlation_volume(tiled=True, precision=name, out=room) is room and torch.equal(room, vol)
+    as_maps = held.float().transpose(1, 2).reshape(-1, D, h, w).to(DEV).contiguous()
+    plain = CorrComputation(as_maps[:B], as_maps[B:].view(T, B, D, h, w), [2] * T)
+    coords = torch.rand(T, B, 2, h, w, generator=torch.Generator().manual_seed(1)).to(DEV) * max(h, w)
+    blocks = [CorrBlockParallelMultiTarget(c, layout="tiled", precision=name)(coords) for c in (packed(), plain)]
+    assert torch.equal(*blocks)

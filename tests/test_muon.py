@@ -685,3 +685,69 @@ def test_results_are_tensors_of_their_own():
     for y, x in zip(ys, xs):
         assert y._base is None and y.storage_offset() == 0 and y.untyped_storage().nbytes() == 4 * x.numel()
     assert len({y.untyped_storage().data_ptr() for y in ys}) == len(ys)
+
+
+@gpu
+def test_the_recorded_step_moves_every_filter_as_the_formula_says():
+    """Three replays of a captured training step: each moves every filter by the plain step of its own gradient, at the scheduled rate, from the momentum of the
+    step before (none in front of the first: warm-up steps leave nothing behind).  Beside it the eager step from the same start: all filters' movements
+    together.  Gradients of the two differ by the order of the look-up adjoint's sums, 1e-5 of a filter's gradient at most; that is multiplied by 485 / 0.68
+    where it is all that a direction holds: 7e-3 a step, 2e-2 in three.  A rate that did not follow the schedule would show as 0.35."""
+    from bflow_amd import configs, synthetic
+    from bflow_amd.weights import deterministic_state_dict
+    B, H, W = 1, 64, 96
+    tp = dict(learning_rate=2e-4, weight_decay=1e-4, optimizer="muon", lr_scheduler=dict(use=True, total_steps=50, pct_start=0.3))
+
+    def batch(seed):
+        rs = np.random.RandomState(seed)
+        to = lambda a: torch.from_numpy(a).to(DEV)
+        return {DataLoading.EV_REPR: to(synthetic.voxel_grid(B, 9, H, W, seed=seed)), DataLoading.FLOW: to(rs.standard_normal((B, 2, H, W)).astype(np.float32) * 4),
+                DataLoading.FLOW_VALID: to(rs.rand(B, H, W) > 0.2), DataLoading.DATASET_TYPE: [DataSetType.DSEC] * B}
+
+    def make(capturable):
+        m = bflow_amd.RAFTSpline(configs.model_config("E_LU4_BD2"))
+        m.load_state_dict(deterministic_state_dict(m, seed=0))
+        m.to(DEV).train()
+        return (m,) + tuple(training.configure_optimizers(m, tp, capturable=capturable))
+
+    batches = [batch(5), batch(6), batch(7)]
+    m1, opt1, sch1 = make(False)
+    start = [p.detach().cpu().double() for p in opt1.param_groups[0]["params"]]
+    step1 = training.TrainStep(m1, num_iter_train=2)
+    for b in batches:
+        opt1.zero_grad(set_to_none=True)
+        step1(b)["loss"].backward()
+        opt1.step()
+        sch1.step()
+    opt1.zero_grad(set_to_none=True)
+
+    m2, opt2, sch2 = make(True)
+    gstep = training.GraphedTrainStep(training.TrainStep(m2, num_iter_train=2), opt2, sch2)
+    filters, rest = (g["params"] for g in opt2.param_groups)
+    rates, vs, moments = [], [torch.zeros(p.shape, dtype=torch.float64) for p in filters], [torch.zeros(p.shape, dtype=torch.float64) for p in rest]
+    for n, b in enumerate(batches):
+        before = [p.detach().cpu().double() for p in filters]
+        rates.append(float(opt2.param_groups[0]["lr"]))
+        gstep(b)
+        torch.cuda.synchronize()
+        for k, p in enumerate(filters):
+            assert bool(p.grad.any())
+            want, vs[k] = plain_step(before[k], p.grad, vs[k], rates[-1], 1e-4, 0.95, True)
+            v = opt2.state[p]["momentum_buffer"].cpu().double()
+            assert off(v, vs[k]) < 2.0 ** -22
+            moved, wanted = p.detach().cpu().double() - before[k], want - before[k]
+            assert float((moved - wanted).norm()) < F32_TOL * float(wanted.norm()) + 2.0 ** -23 * float(want.norm())
+            vs[k] = v
+        for k, p in enumerate(rest):
+            state = opt2.state[p]
+            want = 0.9 * moments[k] + 0.1 * p.grad.cpu().double()
+            assert float(state["step"]) == n + 1
+            moments[k] = state["exp_avg"].cpu().double()
+            assert float((moments[k] - want).norm()) <= 2.0 ** -22 * (float(want.norm()) + float(p.grad.norm()))
+    assert 0 < rates[0] < rates[1] < rates[2]
+    apart = total = 0.0
+    for p, q, s in zip(opt1.param_groups[0]["params"], filters, start):
+        moved = p.detach().cpu().double() - s
+        assert bool(moved.any())
+        apart, total = apart + float((q.detach().cpu().double() - s - moved).norm()) ** 2, total + float(moved.norm()) ** 2
+    assert apart < (2e-2) ** 2 * total, math.sqrt(apart / total)

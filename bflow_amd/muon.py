@@ -112,18 +112,24 @@ class Muon(torch.optim.Optimizer):
     def __init__(self, params, lr=1e-3, momentum: float = 0.95, weight_decay: float = 0.0, nesterov: bool = True, steps: int = STEPS,
                  coefficients: Sequence[float] = COEFFICIENTS, eps: float = EPS, betas: Tuple[float, float] = (0.9, 0.999), adamw_eps: float = 1e-8,
                  capturable: bool = False):
+        defaults = dict(lr=lr, momentum=momentum, weight_decay=weight_decay, nesterov=nesterov, steps=steps, coefficients=tuple(coefficients), eps=eps,
+                        betas=betas, adamw_eps=adamw_eps, capturable=capturable, adamw=False)
+        self._check_group(defaults)
+        super().__init__(params, defaults)
+
+    @staticmethod
+    def _check_group(group):
+        lr, momentum, decay = group["lr"], group["momentum"], group["weight_decay"]
         if not torch.is_tensor(lr) and not lr >= 0.0:
             raise ValueError(f"lr: {lr!r}")
         if not 0.0 <= momentum < 1.0:
             raise ValueError(f"momentum: a number in [0, 1), got {momentum!r}")
-        if not weight_decay >= 0.0:
-            raise ValueError(f"weight_decay: {weight_decay!r}")
-        _check_numbers(steps, coefficients, eps)
-        defaults = dict(lr=lr, momentum=momentum, weight_decay=weight_decay, nesterov=nesterov, steps=steps, coefficients=tuple(coefficients), eps=eps,
-                        betas=betas, adamw_eps=adamw_eps, capturable=capturable, adamw=False)
-        super().__init__(params, defaults)
+        if not decay >= 0.0:
+            raise ValueError(f"weight_decay: {decay!r}")
+        _check_numbers(group["steps"], group["coefficients"], group["eps"])
 
     def add_param_group(self, group):
+        self._check_group({**self.defaults, **group})
         super().add_param_group(group)
         group = self.param_groups[-1]
         for p in group["params"]:

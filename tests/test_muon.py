@@ -751,3 +751,16 @@ def test_the_recorded_step_moves_every_filter_as_the_formula_says():
         assert bool(moved.any())
         apart, total = apart + float((q.detach().cpu().double() - s - moved).norm()) ** 2, total + float(moved.norm()) ** 2
     assert apart < (2e-2) ** 2 * total, math.sqrt(apart / total)
+
+
+def test_a_groups_own_numbers_are_checked():
+    """What a group sets for itself is held to what the optimiser's defaults are held to: two and a half steps are not two."""
+    make = lambda: torch.nn.Parameter(torch.zeros(4, 4))
+    opt = muon.Muon([{"params": [make()], "momentum": 0.5, "steps": 3}])
+    for kw, error in ((dict(steps=2.5), hip.BflowHipError), (dict(steps=0), hip.BflowHipError), (dict(eps=0.0), hip.BflowHipError), (dict(coefficients=(1.0,)), hip.BflowHipError),
+                      (dict(momentum=1.0), ValueError), (dict(weight_decay=-0.1), ValueError), (dict(lr=float("nan")), ValueError)):
+        with pytest.raises(error):
+            opt.add_param_group({"params": [make()], **kw})
+        with pytest.raises(error):
+            muon.Muon([{"params": [make()], **kw}])
+    assert len(opt.param_groups) == 1 and opt.param_groups[0]["momentum"] == 0.5

@@ -49,8 +49,9 @@ __device__ __forceinline__ i32x4 cut(i32x4 v, int k, int K) {
     return v;
 }
 
-// BM x BN tile; wave (wm, wn) keeps WM x WN of it.  8192^3 in 256 x 256 tiles: 487 us, 2.26 POP/s (the library's 8-bit product, without scales: 528 us),
-// matrix cores busy 60 % of the cycles at a clock that power holds down.
+// BM x BN tile; wave (wm, wn) keeps WM x WN of it.  8192^3 in 256 x 256 tiles, many calls in a row: 475 us, 2.32 POP/s (the library's 8-bit product, to 32-bit
+// integers without scales, in turn with it: 452); single calls on a rested card 516 (483).  Matrix cores busy 60 % of the cycles at a clock that power
+// holds down.
 template <int BM, int BN, int WM, int WN>
 struct ByteTile {
     static constexpr int M = BM, N = BN, ACROSS = BN / WN, WAVES = (BM / WM) * ACROSS, THREADS = 64 * WAVES, MT = WM / 32, NT = WN / 32;
@@ -430,7 +431,8 @@ __device__ __forceinline__ unsigned wave_most(unsigned v) {
     return v;
 }
 
-// One wave for a row: x (rows, K), ld elements apart -> q (rows, ldq), zeros behind K.
+// One wave for a row: x (rows, K), ld elements apart -> q (rows, ldq), zeros behind K; the row is read twice, an element a lane, so that few or long rows
+// wait for one load after another.  bf16: 1 x 4096 16 us, 64 x 4096 19, 8192 x 8192 87 (the second reading from the caches: 2.3 TB/s); 4800 x 567 in fp32 7.4.
 template <int DT>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const void* x, long long ld, long long rows, int K, signed char* q, int ldq, float* scale) {
     const int lane = threadIdx.x & 63;
@@ -515,7 +517,8 @@ __global__ __launch_bounds__(1024) void quantize_pixels_kernel(Maps m, int D, in
     }
 }
 
-// The conv engine's operand: hi and lo planes, 32 channels of a pixel together.  Four lanes a row, eight channels each of a block of 32.
+// The conv engine's operand: hi and lo planes, 32 channels of a pixel together.  Four lanes a row, eight channels each of a block of 32.  1 and 4 maps of
+// 256 x 60 x 80, both operands of a volume: 13 us (24.6 MB in, 6.1 out, 2.3 TB/s).
 __global__ __launch_bounds__(256) void quantize_packed_kernel(Maps mm, int KB, int h, int w) {
     int b;
     const int item = operand_of(mm, b), rows = mm.rows[item], np = mm.v[item].np;
@@ -594,7 +597,8 @@ extern "C" int bflow_i8_gemm(const bflow_i8_gemm_t* d, bflow_stream_t stream) {
     if (d->K <= 256 && d->M >= 256 && d->N >= 256 && g.wide && d->N % (16 / size) == 0 && d->lda <= 1 << 20 && (long long)STREAM_ROWS * d->ldo * size < (1LL << 31))
         return launch_stream(g, d->dtype, (unsigned)batch, st);
     // Tiles by the rounds that they take on 256 CUs, priced by what a round took at K = 4096: 256 tiles of 256 x 256 79 us, 512 of 128 x 128 (two on a
-    // CU) 44, 1024 of 64 x 64 (four) 28.  4096^3: 79 / 88 / 112 us; 2048^3: 38 / 19 / 18; 1024^3: 23 / 11 / 6.2; 8192^3: 515 / 576 / 814.
+    // CU) 44, 1024 of 64 x 64 (four) 28.  Captured calls in a row, tiles of 256 / 128 / 64: 8192^3 470 / 534 / 802 us; 4096^3 67 / 75 / 105; 2048^3 31 / 15 /
+    // 16; 1024^3 18 / 9.3 / 5.8.
     auto price = [&](int side, long long room, int us) { return ((long long)ceil_div(d->M, side) * ceil_div(d->N, side) * batch + room - 1) / room * us; };
     const long long large = price(256, 256, 79), middle = price(128, 512, 44), small = price(64, 1024, 28);
     if (small <= middle && small <= large) return launch_tiles<Small>(g, d->dtype, (unsigned)batch, st);

@@ -272,7 +272,7 @@ __device__ __forceinline__ int g_of(const char* ws, long long off, int drop) { r
 // --------------------------------------------------------------------------------------------------------------------------- products
 // BM x BN tile of A B^T.  A group of waves has WM x WN of it each; KG groups share the contraction (a stage holds a chunk for each) and are summed
 // in LDS, in a fixed order.  Three matrix passes over the 32 columns of a chunk.
-// At 4096 x 4096 (three passes counted): X 1.10 PFLOP/s of fp16, B 1.00, matrix cores busy 65 and 55 % of the cycles at a clock that power holds down.
+// At 4096 x 4096 (three passes counted): X 1.10 PFLOP/s of fp16, A and B 1.00, matrix cores busy 65 and 55 % of the cycles at a clock that power holds down.
 // A library product of plain fp16 reaches 1.49 here.
 template <int BM_, int BN_, int WM, int WN, int KG_, int STAGES>
 struct Product {

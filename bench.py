@@ -47,7 +47,7 @@ PEAK_HBM_GBS = 8000.0                      # MI355X_MICROARCH.md: HBM3E 8 TB/s (
 MFMA_STREAM_SUSTAINED_GHZ = 1.5
 PEAK_CLOCK_GHZ = 2.4
 K5_SUSTAINED_GHZ = 1.7                     # shader clock of K5 under load (cycle stamps / wall clock per workgroup: profiles/r0x_k5_stamps_split8.txt, 1.66-1.8)
-PMC_FILE = "r06_pmc.json"                  # rocprofv3 --pmc evidence of this round (tools/collect_profiles.sh)
+PMC_FILE = "pmc.json"                      # rocprofv3 --pmc evidence (tools/collect_profiles.sh)
 
 
 def kernel_source_hash() -> str:

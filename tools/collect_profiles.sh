@@ -1,6 +1,6 @@
 #!/bin/bash
 # Runs ON the GPU box (via gpurun): produces the round-6 evidence files of profiles/ under gpurun_out/profiles/ (tools only; the only
-# writer of profiles/r06_pmc*, r06_bench.json, r06_rocprofv3_*; the A/B files quoted in DESIGN.md section 12 were written by the commands
+# writer of profiles/pmc*, r06_bench.json, r06_rocprofv3_*; the A/B files quoted in DESIGN.md section 12 were written by the commands
 # named in them).     usage: gpurun --timeout 3000 -- tools/collect_profiles.sh
 # FAILS if the MFMA calibration pass or any kernel's counters are missing (tools/pmc_to_json.py): a table with holes is not evidence.
 set -uo pipefail
@@ -29,10 +29,10 @@ done
 # calibration launch (tools/micro/fp8_cross rate_kernel: a pure MFMA stream on every SIMD, 100 % busy by construction) under the same counters
 rm -rf /tmp/pmc; timeout 300 rocprofv3 --pmc $SQ --output-format csv -d /tmp/pmc -- "$REPO/tools/micro/fp8_cross" > /tmp/pmc.log 2>&1
 f=$(find /tmp/pmc -name "*counter_collection.csv" | head -1); [ -n "$f" ] && cp "$f" "$OUT/calib_MFMA.csv"
-python "$REPO/tools/pmc_to_json.py" "$OUT" "$OUT/${R}_pmc.json" > "$OUT/${R}_pmc_summary.txt" || { echo "collect_profiles: counters incomplete" >&2; cat "$OUT/${R}_pmc_summary.txt"; exit 1; }
+python "$REPO/tools/pmc_to_json.py" "$OUT" "$OUT/pmc.json" > "$OUT/pmc_summary.txt" || { echo "collect_profiles: counters incomplete" >&2; cat "$OUT/pmc_summary.txt"; exit 1; }
 # the bench quotes the PMC traffic of kernels built from the SAME sources (kernel_source_hash): counters first, then the bench reads them
-[ -n "${QUICK:-}" ] && { cat "$OUT/${R}_pmc_summary.txt"; ls -la "$OUT"; exit 0; }
-cp "$OUT/${R}_pmc.json" "$REPO/profiles/${R}_pmc.json"
+[ -n "${QUICK:-}" ] && { cat "$OUT/pmc_summary.txt"; ls -la "$OUT"; exit 0; }
+cp "$OUT/pmc.json" "$REPO/profiles/pmc.json"
 
 # ---- (2) the bench line, and the kernel traces: C2 ONLY (the frame's budget per kernel) and the full default command
 timeout 1200 python "$REPO/bench.py" --steps 30 --warmup 5 > "$OUT/${R}_bench.json" 2> "$OUT/bench.stderr"
@@ -68,7 +68,7 @@ for key, meta in metas.items():
         keep = [r for r in rows if meta["regex"] in r["Kernel_Name"]]
         keep = keep[-(int(meta.get("reps", 5)) * 2 * (4 if c == "MFMA" else 1)):] if key != "calib" else keep
         if rows:
-            with open(os.path.join(d, f"{R}_pmc_{c}_{key}.csv"), "w", newline="") as fh:
+            with open(os.path.join(d, f"pmc_{c}_{key}.csv"), "w", newline="") as fh:
                 w = csv.DictWriter(fh, fieldnames=list(rows[0].keys())); w.writeheader(); w.writerows(keep)
         os.remove(p)
 PY

@@ -73,9 +73,13 @@ Round-6 files (`r06_*`).  `tools/collect_profiles.sh` on ONE `gpurun` MI355X box
 the probes listed first (it fails if the MFMA calibration pass or any kernel's counters are missing); the A/B files further down were written by
 the commands quoted inside them while the kernels were developed (each on ONE box, alternating — the boxes of the pool differ by ±4…7 %).  This
 page: `tools/make_profiles_readme.py` (fails on a roofline row without counters).  Earlier rounds: `README_r05.md`, `README_r04.md`.
-`r06_pmc.json` records a hash of the kernel sources it was collected on ({pm["kernel_source_hash"]}); `bench.py` quotes its `traffic` only while
-the sources still hash to the same value.  Every roofline entry of the bench line carries the shader clock measured IN THE RUN
+`r06_pmc.json` records a hash of the kernel sources it was collected on ({pm["kernel_source_hash"]}), as does `pmc.json`; `bench.py` quotes the latter's
+`traffic` only while the sources still hash to the same value.  Every roofline entry of the bench line carries the shader clock measured IN THE RUN
 (`bflow_shader_clock_stamp`: `s_memtime` against `s_memrealtime` of the same CUs around the timed launches): a slow box is a reading, not a guess.
+
+`pmc.json`, `pmc_summary.txt`, `pmc_{{FETCH_SIZE,WRITE_SIZE,MFMA}}_<key>.csv` and `bench.json` are the same passes and the same line on the present sources, which
+are compiled without packed 32-bit float instructions; `bench.py` reads `pmc.json`.  `operators_*.txt`: the matrix products of `newton_schulz.hip` and
+`int8_gemm.hip` (kernel times, counters, accuracy against 64 bits, the 8-bit product beside the library's, frames by correlation arithmetic).
 
 | File | Command | What it shows |
 |---|---|---|

@@ -1,6 +1,6 @@
 #!/usr/bin/env python
 """Folds the rocprofv3 --pmc counter CSVs of tools/collect_profiles.sh (one FETCH_SIZE / WRITE_SIZE / MFMA set per roofline kernel + the
-MFMA calibration launch + the PROBE line of tools/roofline_probe.py per key) into profiles/r06_pmc.json.
+MFMA calibration launch + the PROBE line of tools/roofline_probe.py per key) into profiles/pmc.json.
    usage: pmc_to_json.py <dir with <key>_{FETCH_SIZE,WRITE_SIZE,MFMA}.csv, <key>_meta.json, calib_MFMA.csv> <out.json>
 FAILS (exit 1) when the calibration pass or any key's counters are missing: a table with holes is not evidence."""
 import csv, json, os, sys
